@@ -58,6 +58,14 @@ SIGNATURES = {
                                  P, *S3, P, P, c_size, P], c_int),
     "fpx_decode_attention_noalloc": ([P, *S3, P, *S3, P, *S3, c_int, c_int, c_int, c_int, c_int, c_int,
                                       c_double, P, *S3, P, P], c_int),
+    "fpx_paged_page_bytes": ([c_int, c_int, c_int, c_int], c_size),
+    "fpx_paged_append": ([c_int, P, *S3, P, *S3, P, *S3, c_int, c_int, c_int, c_int, c_int, P, c_int, c_int,
+                          P, c_int, c_int, P, c_i64, c_int, P, P, P, *S3, P, *S3, c_int, P], c_int),
+    "fpx_paged_gather": ([c_int, P, c_int, c_int, P, c_i64, c_int, P, P, c_int, c_int, c_int, c_int,
+                          P, *S3, P, *S3, c_int, P], c_int),
+    "fpx_paged_decode_workspace_bytes": ([c_int, c_int, c_int, c_int, c_int, c_int], c_size),
+    "fpx_paged_decode_attention": ([c_int, P, *S3, c_int, c_int, c_int, c_int, c_int, c_double, P, c_int, c_int,
+                                    P, c_i64, c_int, P, P, P, *S3, P, P, c_size, P], c_int),
     "fpx_ar_buffer_bytes": ([c_int], c_size),
     "fpx_ar_create": ([c_size, ctypes.POINTER(c_void_p), ctypes.POINTER(ctypes.c_char)], c_int),
     "fpx_ar_open": ([ctypes.POINTER(ctypes.c_char), ctypes.POINTER(c_void_p)], c_int),
@@ -133,7 +141,8 @@ def strides3(t: torch.Tensor):
 
 
 def device_error(reset: bool = True) -> int:
-    """The device error word of libfpx (1 = a bounded wait in a kernel gave up); synchronises."""
+    """The device error word of libfpx (1 = a bounded wait in a kernel gave up, 2 = an index in device
+    memory, a page or a position, named nothing); synchronises."""
     code = ctypes.c_int(0)
     rc = lib().fpx_device_error(ctypes.byref(code), 1 if reset else 0)
     if rc != 0:

@@ -1,0 +1,293 @@
+"""The paged KV cache on libfpx: append with rotation, decode attention, gather.
+
+The reference keeps HF's dynamic cache, one dense bf16 tensor a layer (``evaluate.py:357-405``);
+a cache in pages lets sequences of any lengths share one pool, and the 4-bit form holds four
+times the tokens and is read in a quarter of the time, which is what bounds a decode step at
+long context.
+
+A pool is a tensor ``[pages, Hkv, page_size, row]``: bf16 with ``row = 2 d``, or uint8 with
+``row = 9 d / 8 + 2`` for the 4-bit form (groups of 32 dims; the bytes' order is the kernels' own,
+``paged_gather`` reads them back). ``new_pool`` makes one; ``PagedKVCache`` keeps the pools of a
+model's layers with their page table.
+
+Every call takes ``page_table`` [B, max_pages] int32 (a sequence's pages in order) and ``starts``
+[B] int32: row i of sequence b stands at position ``starts[b] + i``. ``counts`` [B] int32 says how
+many of the call's rows are rows; those behind are padding. A negative start makes a sequence
+inactive. All three are read on the device, so a captured step follows them. An index that
+names nothing (a page outside the pool, a position past the table) is skipped, and sets
+``_capi.device_error`` to 2.
+"""
+
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+
+from ._capi import FpxError, call, lib, ptr, stream
+
+FORMATS = {"bf16": 0, "int4": 1}
+MAX_ROWS = 64  # query rows of a sequence in one paged_decode_attention
+
+
+def row_elements(format: str, head_dim: int) -> int:
+    """Pool elements (bf16, or bytes of int4) of one token and KV head."""
+    if format not in FORMATS:
+        raise ValueError(f"unknown page format {format!r}; choose from {tuple(FORMATS)}")
+    if head_dim not in (128, 256):
+        raise FpxError(f"head dim {head_dim} is not compiled (128 or 256)")
+    return 2 * head_dim if format == "bf16" else 9 * head_dim // 8 + 2
+
+
+def new_pool(pages: int, kv_heads: int, head_dim: int = 128, page_size: int = 64, format: str = "int4",
+             device="cuda", layers: int | None = None) -> torch.Tensor:
+    """An unwritten pool [pages, Hkv, page_size, row], with ``layers`` a stack of them."""
+    if page_size < 16 or page_size > 1024 or page_size & (page_size - 1):
+        raise FpxError("page_size must be a power of two, 16 .. 1024")
+    if pages <= 0 or kv_heads <= 0:
+        raise ValueError("a pool needs pages and KV heads")
+    shape = (pages, kv_heads, page_size, row_elements(format, head_dim))
+    return torch.empty(shape if layers is None else (layers, *shape),
+                       dtype=torch.bfloat16 if format == "bf16" else torch.uint8, device=device)
+
+
+def rope_table(positions: int, rotary: int = 128, theta: float = 1e6, device="cuda") -> torch.Tensor:
+    """[positions, rotary] fp32: cosines, then sines, of position * theta^(-2 i / rotary). Angles are
+    taken in 64 bits: in 32 a far position's angle is off by more than bf16 rounds."""
+    inv = theta ** (-torch.arange(0, rotary, 2, device=device, dtype=torch.float64) / rotary)
+    angle = torch.arange(positions, device=device, dtype=torch.float64)[:, None] * inv
+    return torch.cat((angle.cos(), angle.sin()), 1).float()
+
+
+def _pool(pool: torch.Tensor):
+    """(format id, head dim) of a pool tensor."""
+    if pool.dim() != 4:
+        raise FpxError("a pool is [pages, Hkv, page_size, row]")
+    row = pool.shape[3]
+    if pool.dtype == torch.bfloat16:
+        form, dim = 0, row // 2
+    elif pool.dtype == torch.uint8:
+        form, dim = 1, (row - 2) * 8 // 9
+    else:
+        raise TypeError("a pool is bfloat16, or uint8 in the 4-bit form")
+    if dim not in (128, 256) or row != (2 * dim if form == 0 else 9 * dim // 8 + 2):
+        raise FpxError(f"a pool's rows of {row} elements are of no compiled head dim")
+    if not pool.is_contiguous():
+        raise FpxError("a pool must be contiguous")
+    return form, dim
+
+
+def _where(pool, page_table, starts, counts, batch, kv_heads, head_dim):
+    """Checks the tensors that say where rows lie; (format, arguments of the C calls)."""
+    form, dim = _pool(pool)
+    if dim != head_dim or pool.shape[1] != kv_heads:
+        raise FpxError(f"the pool holds {pool.shape[1]} KV heads of {dim}, the call {kv_heads} of {head_dim}")
+    if page_table.dtype != torch.int32 or starts.dtype != torch.int32 or (counts is not None and counts.dtype != torch.int32):
+        raise TypeError("page_table, starts and counts must be int32")
+    if page_table.dim() != 2 or page_table.shape[0] != batch or (page_table.shape[1] > 1 and page_table.stride(1) != 1):
+        raise FpxError("page_table must be [B, max_pages] with contiguous rows")
+    for t in (starts, counts):
+        if t is not None and (t.shape != (batch,) or not t.is_contiguous()):
+            raise FpxError("starts and counts must be [B], contiguous")
+    stride = page_table.stride(0) if batch > 1 else page_table.shape[1]
+    return form, (ptr(pool), pool.shape[0], pool.shape[2], ptr(page_table), stride, page_table.shape[1], ptr(starts),
+                  ptr(counts))
+
+
+def _device(*tensors):
+    """The tensors' common CUDA device."""
+    dev = None
+    for t in tensors:
+        if t is None:
+            continue
+        if t.device.type != "cuda":
+            raise FpxError("fpx ops run on CUDA tensors only (there is no CPU path)")
+        if dev is not None and t.device != dev:
+            raise FpxError("all tensors of a call must be on one device")
+        dev = t.device
+    return dev
+
+
+def _call(dev, name, *args):
+    """The C call on dev's current stream, with dev as the current device (its default stream has no
+    device of its own to be bound to)."""
+    if dev.index == torch.cuda.current_device():
+        call(name, *args, stream(dev))
+    else:
+        with torch.cuda.device(dev):
+            call(name, *args, stream(dev))
+
+
+def _bf16(*tensors):
+    for t in tensors:
+        if t is not None and t.dtype != torch.bfloat16:
+            raise TypeError("q, k, v and their outputs must be bfloat16")
+
+
+def _shape(t, shape, name):
+    if tuple(t.shape) != tuple(shape):
+        raise FpxError(f"{name} must be {tuple(shape)}, is {tuple(t.shape)}")
+
+
+def _strides(t: torch.Tensor):
+    """Element strides of dims 0 .. 2; those of dims of one entry, which are never used, as 0."""
+    if t.stride(-1) != 1:
+        raise FpxError("the last dimension must be contiguous")
+    return tuple(s if n > 1 else 0 for s, n in zip(t.stride()[:3], t.shape))
+
+
+def _output(t, shape, name):
+    _shape(t, shape, name)
+    if any(s == 0 and n > 1 for s, n in zip(t.stride(), t.shape)):
+        raise FpxError(f"{name} must not be an expanded tensor")
+    return t
+
+
+@torch.no_grad()
+def paged_append(k, v, pool, page_table, starts, counts=None, q=None, rope=None, q_out=None, k_out=None):
+    """Stores new rows k, v [B, L, Hkv, d] bf16 in the pages, keys rotated by ``rope``.
+
+    ``rope`` is a table like ``rope_table``'s, [positions, rotary] fp32 (NeoX pairs (i, i + rotary / 2) of
+    the first ``rotary`` dims), or None: no rotation. ``q`` [B, L, H, d]: queries, rotated into ``q_out``
+    (may be q), which is returned; without ``q_out`` into a new tensor, whose padding rows are zero.
+    ``k_out`` [B, L, Hkv, d] (may be k) also takes the rotated keys in bf16. With ``q_out`` given (or no q),
+    padding rows are left as they are.
+    Rotation is in fp32 and rounds once, to bf16 or to the 4-bit codes. Sequences of one call must not
+    write the same page."""
+    dev = _device(k, v, pool, page_table, starts, counts, q, rope, q_out, k_out)
+    _bf16(k, v, q, q_out, k_out)
+    if k.dim() != 4:
+        raise FpxError("k and v must be [B, L, Hkv, d]")
+    batch, length, kv_heads, dim = k.shape
+    _shape(v, k.shape, "v")
+    form, where = _where(pool, page_table, starts, counts, batch, kv_heads, dim)
+    rope_len = rotary = zero = 0
+    if rope is not None:
+        if rope.dtype != torch.float32 or rope.dim() != 2 or not rope.is_contiguous():
+            raise FpxError("rope must be a contiguous fp32 [positions, rotary] table")
+        rope_len, rotary = rope.shape
+    if q is None:
+        if q_out is not None:
+            raise FpxError("q_out without q")
+        heads, q_args, o_args = 0, (None, 0, 0, 0), (None, 0, 0, 0)
+    else:
+        if q.dim() != 4:
+            raise FpxError("q must be [B, L, H, d]")
+        heads = q.shape[2]
+        _shape(q, (batch, length, heads, dim), "q")
+        if q_out is None:
+            zero, q_out = 1, torch.empty(q.shape, dtype=q.dtype, device=dev)
+        _output(q_out, q.shape, "q_out")
+        q_args, o_args = (ptr(q), *_strides(q)), (ptr(q_out), *_strides(q_out))
+    if k_out is not None:
+        _output(k_out, k.shape, "k_out")
+    if batch == 0 or length == 0:
+        return q_out
+    ko_args = (None, 0, 0, 0) if k_out is None else (ptr(k_out), *_strides(k_out))
+    _call(dev, "fpx_paged_append", form, *q_args, ptr(k), *_strides(k), ptr(v), *_strides(v), batch, length, heads,
+          kv_heads, dim, ptr(rope), rope_len, rotary, *where, *o_args, *ko_args, zero)
+    return q_out
+
+
+@torch.no_grad()
+def paged_gather(pool, page_table, starts, counts, length: int, k_out=None, v_out=None):
+    """Rows back as bf16: (k, v) [B, length, Hkv, d], for a prefill over a cached prefix. Rows behind
+    ``counts`` (None: every row counts) are left as they are in given outputs, and zero in new ones."""
+    _, dim = _pool(pool)
+    dev = _device(pool, page_table, starts, counts, k_out, v_out)
+    batch, kv_heads = starts.shape[0], pool.shape[1]
+    form, where = _where(pool, page_table, starts, counts, batch, kv_heads, dim)
+    _bf16(k_out, v_out)
+    shape = (batch, length, kv_heads, dim)
+    if (k_out is None) != (v_out is None):
+        raise FpxError("give both of k_out and v_out, or neither")
+    zero = int(k_out is None)
+    if zero:
+        k_out, v_out = (torch.empty(shape, dtype=torch.bfloat16, device=dev) for _ in range(2))
+    _output(k_out, shape, "k_out")
+    _output(v_out, shape, "v_out")
+    if batch and length:
+        _call(dev, "fpx_paged_gather", form, *where, batch, length, kv_heads, dim, ptr(k_out), *_strides(k_out),
+              ptr(v_out), *_strides(v_out), zero)
+    return k_out, v_out
+
+
+@torch.no_grad()
+def paged_decode_attention(q, pool, page_table, starts, scale: float, counts=None, out=None, lse=None, ws=None):
+    """Attention of q [B, Lq, H, d] bf16 to the cached tokens, causal by position: row i of sequence b
+    sees positions 0 .. starts[b] + i, its own with them (append first). Returns bf16 [B, Lq, H, d]
+    (``out`` if given); ``lse`` fp32 [B, Lq, H] takes the natural-log sums. Padding rows give 0 and -inf.
+
+    For the few rows of a decode or verification step: Lq <= 64. A longer continuation reads its
+    prefix with ``paged_gather`` and runs ``prefill_attention``. ``ws`` is a uint8 workspace of
+    ``paged_decode_workspace_bytes``; without it each call takes its own from torch's allocator, so calls on
+    several streams or in several graphs share nothing."""
+    dev = _device(q, pool, page_table, starts, counts, out, lse, ws)
+    _bf16(q, out)
+    if q.dim() != 4:
+        raise FpxError("q must be [B, Lq, H, d]")
+    batch, rows, heads, dim = q.shape
+    kv_heads = pool.shape[1]
+    form, where = _where(pool, page_table, starts, counts, batch, kv_heads, dim)
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    _output(out, q.shape, "out")
+    if lse is not None and (lse.dtype != torch.float32 or not lse.is_contiguous() or lse.shape != q.shape[:3]):
+        raise FpxError("lse must be a contiguous fp32 [B, Lq, H]")
+    if batch == 0 or rows == 0:
+        return out
+    if ws is None:
+        ws = torch.empty(max(1, int(lib().fpx_paged_decode_workspace_bytes(form, batch, rows, heads, kv_heads, dim))),
+                         dtype=torch.uint8, device=dev)
+    _call(dev, "fpx_paged_decode_attention", form, ptr(q), *_strides(q), batch, rows, heads, kv_heads, dim,
+          float(scale), *where, ptr(out), *_strides(out), ptr(lse), ptr(ws), ws.numel())
+    return out
+
+
+def paged_decode_workspace_bytes(pool, batch: int, rows: int, heads: int) -> int:
+    """Bytes of ``paged_decode_attention``'s workspace, whatever the sequences' lengths."""
+    form, dim = _pool(pool)
+    return int(lib().fpx_paged_decode_workspace_bytes(form, batch, rows, heads, pool.shape[1], dim))
+
+
+# The same calls as PyTorch custom ops, for torch.compile and fake tensors.
+
+
+@torch.library.custom_op("fpx::paged_append", mutates_args=("pool",))
+def _append_op(k: torch.Tensor, v: torch.Tensor, pool: torch.Tensor, page_table: torch.Tensor, starts: torch.Tensor,
+               counts: Optional[torch.Tensor], q: Optional[torch.Tensor],
+               rope: Optional[torch.Tensor]) -> torch.Tensor:
+    out = paged_append(k, v, pool, page_table, starts, counts, q, rope)
+    return k.new_empty(0) if out is None else out
+
+
+@_append_op.register_fake
+def _(k, v, pool, page_table, starts, counts, q, rope):
+    return k.new_empty(0 if q is None else q.shape)
+
+
+@torch.library.custom_op("fpx::paged_gather", mutates_args=())
+def _gather_op(pool: torch.Tensor, page_table: torch.Tensor, starts: torch.Tensor, counts: Optional[torch.Tensor],
+               length: int) -> tuple[torch.Tensor, torch.Tensor]:
+    return paged_gather(pool, page_table, starts, counts, length)
+
+
+@_gather_op.register_fake
+def _(pool, page_table, starts, counts, length):
+    shape = (starts.shape[0], length, pool.shape[1], _pool(pool)[1])
+    return pool.new_empty(shape, dtype=torch.bfloat16), pool.new_empty(shape, dtype=torch.bfloat16)
+
+
+@torch.library.custom_op("fpx::paged_decode_attention", mutates_args=())
+def _decode_op(q: torch.Tensor, pool: torch.Tensor, page_table: torch.Tensor, starts: torch.Tensor,
+               counts: Optional[torch.Tensor], scale: float) -> torch.Tensor:
+    return paged_decode_attention(q, pool, page_table, starts, scale, counts)
+
+
+@_decode_op.register_fake
+def _(q, pool, page_table, starts, counts, scale):
+    return q.new_empty(q.shape)
+
+
+__all__ = ["FORMATS", "new_pool", "rope_table", "row_elements", "paged_append", "paged_gather",
+           "paged_decode_attention", "paged_decode_workspace_bytes", "FpxError"]

@@ -41,6 +41,19 @@ enum fpx_status {
   FPX_ERR_TIMEOUT = -6      /* a bounded device-side wait gave up (see fpx_device_error) */
 };
 
+/* fpx_device_error codes. */
+enum fpx_device_code {
+  FPX_DEVICE_OK = 0,
+  FPX_DEVICE_WAIT = 1,     /* a bounded wait inside a kernel gave up */
+  FPX_DEVICE_BAD_INDEX = 2 /* a page, position or table row that a kernel read from device memory does not exist */
+};
+
+/* Forms of a KV-cache page. */
+enum fpx_page_format {
+  FPX_PAGES_BF16 = 0,
+  FPX_PAGES_INT4 = 1 /* 4-bit codes in groups of 32 dims: 9 d / 8 + 2 bytes a token and KV head */
+};
+
 /* attention.py:15-24 METHODS, in order. */
 enum fpx_method {
   FPX_METHOD_DENSE = 0,
@@ -78,8 +91,9 @@ int fpx_version(void);
  * bf16 high + low halves, two passes (default), 1 = fp32 CUDA cores (cross-check). */
 int fpx_set_option(int key, int value);
 
-/* Reads (and with reset != 0 clears) the device error word set when a bounded wait inside a
- * kernel gave up (1 = wait timeout); synchronous. No reference counterpart. */
+/* Reads (and with reset != 0 clears) the device error word: an fpx_device_code, the highest that
+ * was set (a bounded wait inside a kernel gave up, or an index in device memory named nothing);
+ * synchronous. No reference counterpart. */
 int fpx_device_error(int *code, int reset);
 
 /* ---- routing ------------------------------------------------------------------------ */
@@ -292,6 +306,61 @@ int fpx_decode_attention_noalloc(const void *q, int64_t q_sb, int64_t q_sl, int6
                                  int B, int Lq, int S, int H, int Hkv, int d, double scale,
                                  void *out, int64_t o_sb, int64_t o_sl, int64_t o_sh, float *lse,
                                  fpx_stream_t stream);
+
+/* ---- the paged KV cache (no reference counterpart) ------------------------------------ */
+/* A pool holds `pages` pages of page_size tokens (a power of two, 16 .. 1024) for every KV head,
+ * [pages][Hkv][fpx_paged_page_bytes(format, 1, d, page_size)] bytes, 16-byte aligned, without
+ * gaps. Row b of the int32 page table [B, max_pages] (row stride table_stride) names sequence b's
+ * pages in order. d = 128 or 256.
+ *
+ * Each call works on L (Lq) rows of B sequences: row i of sequence b stands at position
+ * starts[b] + i. With counts, only the first counts[b] rows are rows; those behind are padding
+ * (counts is clamped to 0 .. L; NULL: every row counts). A sequence with starts[b] < 0 is
+ * inactive: all its rows are padding. Sequences of one call must not write the same page.
+ *
+ * Table, starts and counts are device memory, so a captured step can be replayed as they
+ * change. What they name is checked where it is used: a page outside the pool, a position past
+ * max_pages * page_size or past the rotation table is skipped, and sets the device error word to
+ * FPX_DEVICE_BAD_INDEX. A skipped page's keys take no part in attention and read back as zero. */
+
+/* Bytes of one page (0: no such page). */
+size_t fpx_paged_page_bytes(int format, int Hkv, int d, int page_size);
+
+/* Rotates (NeoX pairs (i, i + rotary / 2) of the first `rotary` dims) and stores new rows: k, v
+ * [B, L, Hkv, d] go into the pages (int4 pages: quantised from the fp32 rotation), the rotated
+ * queries [B, L, H, d] to q_out (may be q), and with k_out the rotated keys in bf16 there too
+ * (may be k). H = 0 with q = q_out = NULL: keys and values alone. rope: fp32
+ * [rope_len][rotary], cosines then sines of each position (16-byte aligned, rotary a multiple of
+ * 8), or NULL: no rotation. Padding rows are left as they are, unless zero_padding is set. Head rows are
+ * 8-byte aligned, strides multiples of 4 elements. With zero_padding != 0, padding rows (and skipped ones) of q_out and
+ * k_out become zero. A value group (32 dims) with an infinity or
+ * a NaN reads back from int4 pages as NaN. */
+int fpx_paged_append(int format, const void *q, int64_t q_sb, int64_t q_sl, int64_t q_sh, const void *k,
+                     int64_t k_sb, int64_t k_sl, int64_t k_sh, const void *v, int64_t v_sb, int64_t v_sl,
+                     int64_t v_sh, int B, int L, int H, int Hkv, int d, const float *rope, int rope_len, int rotary,
+                     void *pool, int pages, int page_size, const int32_t *table, int64_t table_stride, int max_pages,
+                     const int32_t *starts, const int32_t *counts, void *q_out, int64_t qo_sb, int64_t qo_sl,
+                     int64_t qo_sh, void *k_out, int64_t ko_sb, int64_t ko_sl, int64_t ko_sh, int zero_padding,
+                     fpx_stream_t stream);
+
+/* Reads rows back as bf16: k, v [B, L, Hkv, d] (head rows 8-byte aligned, strides multiples of 4
+ * elements). Padding rows are left as they are, or with zero_padding != 0 become zero. */
+int fpx_paged_gather(int format, const void *pool, int pages, int page_size, const int32_t *table,
+                     int64_t table_stride, int max_pages, const int32_t *starts, const int32_t *counts, int B, int L,
+                     int Hkv, int d, void *k, int64_t k_sb, int64_t k_sl, int64_t k_sh, void *v, int64_t v_sb,
+                     int64_t v_sl, int64_t v_sh, int zero_padding, fpx_stream_t stream);
+
+/* Attention of q [B, Lq, H, d] (16-byte aligned rows) to the cached keys, causal by position: a
+ * row sees positions 0 .. its own, which fpx_paged_append has stored. Lq <= 64, H / Hkv <= 16,
+ * B * Lq * H <= 2^24. out bf16 with element strides, lse fp32 [B, Lq, H] natural log or NULL;
+ * padding rows give 0 and -inf. Bytes of workspace do not depend on the sequences' lengths; it
+ * needs no initial value, and two calls that may overlap need two. */
+size_t fpx_paged_decode_workspace_bytes(int format, int B, int Lq, int H, int Hkv, int d);
+int fpx_paged_decode_attention(int format, const void *q, int64_t q_sb, int64_t q_sl, int64_t q_sh, int B, int Lq,
+                               int H, int Hkv, int d, double scale, const void *pool, int pages, int page_size,
+                               const int32_t *table, int64_t table_stride, int max_pages, const int32_t *starts,
+                               const int32_t *counts, void *out, int64_t o_sb, int64_t o_sl, int64_t o_sh, float *lse,
+                               void *workspace, size_t workspace_bytes, fpx_stream_t stream);
 
 #ifdef __cplusplus
 }
