@@ -70,9 +70,24 @@ struct PageView {
     if (starts[b] < 0) return 0;
     return counts ? max(0, min(counts[b], L)) : L;
   }
+  // The same with the start, both words read at once; a row past int32 positions counts, and fails where it is used.
+  FPX_INLINE void rows(int b, int L, int &start, int &count) const {
+    const int c = counts ? counts[b] : L;
+    start = starts[b];
+    count = start < 0 ? 0 : max(0, min(c, L));
+  }
   FPX_INLINE void fail() const {
     if (error) atomicMax(error, FPX_DEVICE_BAD_INDEX);
   }
+};
+
+// Host: element strides of a [B, L, heads, d] tensor; those of one-entry dims, which multiply
+// nothing, as zero.
+struct RowStrides {
+  int64_t b, l, h;
+  RowStrides(int64_t sb, int64_t sl, int64_t sh, int B, int L, int heads)
+      : b(B > 1 ? sb : 0), l(L > 1 ? sl : 0), h(heads > 1 ? sh : 0) {}
+  bool multiples_of(int n) const { return b % n == 0 && l % n == 0 && h % n == 0; }
 };
 
 // Host: fills a PageView and checks what can be checked there; returns an fpx_status.

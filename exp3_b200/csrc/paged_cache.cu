@@ -347,8 +347,8 @@ extern "C" size_t fpx_paged_page_bytes(int format, int Hkv, int d, int page_size
   return 0;
 }
 
-static bool row_aligned(const void *p, int64_t a, int64_t b, int64_t c) {  // 8-byte pieces of a head row
-  return !(reinterpret_cast<uintptr_t>(p) & 7) && a % 4 == 0 && b % 4 == 0 && c % 4 == 0;
+static bool row_aligned(const void *p, const RowStrides &s) {  // 8-byte pieces of a head row
+  return !(reinterpret_cast<uintptr_t>(p) & 7) && s.multiples_of(4);
 }
 
 extern "C" int fpx_paged_append(int format, const void *q, int64_t q_sb, int64_t q_sl, int64_t q_sh, const void *k,
@@ -369,15 +369,16 @@ extern "C" int fpx_paged_append(int format, const void *q, int64_t q_sb, int64_t
     if (rope_len <= 0) return FPX_ERR_INVALID;
     if (rotary < 8 || rotary > d || rotary % 8 || (reinterpret_cast<uintptr_t>(rope) & 15)) return FPX_ERR_SHAPE;
   }
-  if (!row_aligned(k, k_sb, k_sl, k_sh) || !row_aligned(v, v_sb, v_sl, v_sh) ||
-      (H && (!row_aligned(q, q_sb, q_sl, q_sh) || !row_aligned(q_out, qo_sb, qo_sl, qo_sh))) ||
-      (k_out && !row_aligned(k_out, ko_sb, ko_sl, ko_sh)))
+  const RowStrides qs(q_sb, q_sl, q_sh, B, L, H), ks(k_sb, k_sl, k_sh, B, L, Hkv), vs(v_sb, v_sl, v_sh, B, L, Hkv),
+      qo(qo_sb, qo_sl, qo_sh, B, L, H), ko(ko_sb, ko_sl, ko_sh, B, L, Hkv);
+  if (!row_aligned(k, ks) || !row_aligned(v, vs) || (H && (!row_aligned(q, qs) || !row_aligned(q_out, qo))) ||
+      (k_out && !row_aligned(k_out, ko)))
     return FPX_ERR_SHAPE;
-  p.q = static_cast<const __nv_bfloat16 *>(q); p.q_sb = q_sb; p.q_sl = q_sl; p.q_sh = q_sh;
-  p.k = static_cast<const __nv_bfloat16 *>(k); p.k_sb = k_sb; p.k_sl = k_sl; p.k_sh = k_sh;
-  p.v = static_cast<const __nv_bfloat16 *>(v); p.v_sb = v_sb; p.v_sl = v_sl; p.v_sh = v_sh;
-  p.q_out = static_cast<__nv_bfloat16 *>(q_out); p.qo_sb = qo_sb; p.qo_sl = qo_sl; p.qo_sh = qo_sh;
-  p.k_out = static_cast<__nv_bfloat16 *>(k_out); p.ko_sb = ko_sb; p.ko_sl = ko_sl; p.ko_sh = ko_sh;
+  p.q = static_cast<const __nv_bfloat16 *>(q); p.q_sb = qs.b; p.q_sl = qs.l; p.q_sh = qs.h;
+  p.k = static_cast<const __nv_bfloat16 *>(k); p.k_sb = ks.b; p.k_sl = ks.l; p.k_sh = ks.h;
+  p.v = static_cast<const __nv_bfloat16 *>(v); p.v_sb = vs.b; p.v_sl = vs.l; p.v_sh = vs.h;
+  p.q_out = static_cast<__nv_bfloat16 *>(q_out); p.qo_sb = qo.b; p.qo_sl = qo.l; p.qo_sh = qo.h;
+  p.k_out = static_cast<__nv_bfloat16 *>(k_out); p.ko_sb = ko.b; p.ko_sl = ko.l; p.ko_sh = ko.h;
   p.rope = rope; p.rope_len = rope_len; p.rotary = rotary;
   p.B = B; p.L = L; p.H = H; p.Hkv = Hkv; p.zero_padding = zero_padding != 0;
   const int64_t blocks = ((int64_t)B * L + 3) / 4;
@@ -409,9 +410,10 @@ extern "C" int fpx_paged_gather(int format, const void *pool, int pages, int pag
   const int rc = make_page_view(&p.pv, format, pool, pages, page_size, table, table_stride, max_pages, starts, counts,
                                Hkv, d);
   if (rc) return rc;
-  if (!row_aligned(k, k_sb, k_sl, k_sh) || !row_aligned(v, v_sb, v_sl, v_sh)) return FPX_ERR_SHAPE;
-  p.k = static_cast<__nv_bfloat16 *>(k); p.k_sb = k_sb; p.k_sl = k_sl; p.k_sh = k_sh;
-  p.v = static_cast<__nv_bfloat16 *>(v); p.v_sb = v_sb; p.v_sl = v_sl; p.v_sh = v_sh;
+  const RowStrides ks(k_sb, k_sl, k_sh, B, L, Hkv), vs(v_sb, v_sl, v_sh, B, L, Hkv);
+  if (!row_aligned(k, ks) || !row_aligned(v, vs)) return FPX_ERR_SHAPE;
+  p.k = static_cast<__nv_bfloat16 *>(k); p.k_sb = ks.b; p.k_sl = ks.l; p.k_sh = ks.h;
+  p.v = static_cast<__nv_bfloat16 *>(v); p.v_sb = vs.b; p.v_sl = vs.l; p.v_sh = vs.h;
   p.B = B; p.L = L; p.Hkv = Hkv; p.zero_padding = zero_padding != 0;
   const int64_t blocks = ((int64_t)B * L + 3) / 4;
   if (blocks > 0x7fffffff || Hkv > 65535) return FPX_ERR_SHAPE;

@@ -18,8 +18,8 @@
 //   bf16 pages: P is split in two bf16 terms, so that it does not round before the output does.
 //
 // Work is split evenly over the CTAs of one launch, whatever the sequences' lengths: the
-// granules (16 tokens) of all (sequence, row block, KV head) units lie end to end, each CTA
-// takes an equal run of them, and its four warps every fourth granule, each through its own
+// steps (one or two granules of 16 tokens) of all (sequence, row block, KV head) units lie end to
+// end, each CTA takes an equal run of them, and its four warps every fourth step, each through its own
 // ring of bulk copies (no barrier between warps inside a unit). A unit inside one CTA is
 // finished there; the pieces of the others are merged in CTA order by the second launch, so
 // results do not depend on timing.
@@ -39,30 +39,31 @@ struct PagedDecodeParams {
   float *lse;  // [B][Lq][H] or null
   int B, Lq, H, Hkv, group, blocks;  // blocks: row blocks of 8 NT (query row, head of the group) pairs
   float scale_log2;
-  int ctas, min_granules;
-  int64_t *prefix;  // [B * blocks + 1] granules of all heads before an item (b, row block)
-  float *part_o;    // [ctas + units][8 NT][d]
-  float *part_ml;   // [ctas + units][8 NT][2]
+  int ctas, min_steps;
+  int *prefix;     // [B * blocks + 1] steps of all heads before an item (b, row block)
+  float *part_o;   // [ctas + units][8 NT][d]
+  float *part_ml;  // [ctas + units][8 NT][2]
 };
 
-constexpr int kWarps = 4;
-constexpr float kRaise = 8.f;  // the running maximum follows when a logit passes it by this (log2)
+constexpr float kRaise = 8.f;      // the running reference follows when a logit passes it by this (log2)
+constexpr float kLowest = -3e38f;  // reference before any logit: below all of them, and finite
 
 // Keys that row block rb of sequence b needs: all up to its last row's position.
 template <int NT>
-FPX_INLINE int item_keys(const PagedDecodeParams &p, int b, int rb) {
-  const int count = p.pv.count(b, p.Lq);
+FPX_INLINE int item_keys(const PagedDecodeParams &p, int start, int count, int rb) {
   const int first = rb * 8 * NT;
   if (first >= count * p.group) return 0;
   const int last = min(count * p.group, first + 8 * NT) - 1;
-  const int64_t keys = (int64_t)p.pv.starts[b] + last / p.group + 1;
+  const int64_t keys = (int64_t)start + last / p.group + 1;
   if (keys > p.pv.capacity()) {
     p.pv.fail();
     return p.pv.capacity();
   }
   return (int)keys;
 }
-FPX_INLINE int granules_of(int keys) { return (keys + kGranule - 1) / kGranule; }
+// A step is the GS granules of one ring stage.
+template <int GS>
+FPX_INLINE int steps_of(int keys) { return (keys + GS * kGranule - 1) / (GS * kGranule); }
 
 FPX_INLINE uint32_t and_or(uint32_t a, uint32_t b, uint32_t c) {
   uint32_t d;
@@ -79,6 +80,12 @@ FPX_INLINE void mma_f16_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+FPX_INLINE void mma_bf16_zero(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {  // D = A B
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};\n"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
 }
 FPX_INLINE uint32_t hmul2u(uint32_t a, uint32_t b) {
   __half2 r = __hmul2(*reinterpret_cast<__half2 *>(&a), *reinterpret_cast<__half2 *>(&b));
@@ -104,19 +111,18 @@ FPX_INLINE void bulk_load(void *dst, const void *src, uint32_t bytes, uint64_t *
                : "memory");
 }
 
-template <int FMT, int D, int NT, int ST>
+template <int FMT, int D, int NT, int GS, int W, int ST>
 struct PagedSmem {
   union {
-    uint8_t ring[kWarps][ST][Granule<FMT, D>::kBytes];
+    uint8_t ring[W][ST][GS * Granule<FMT, D>::kBytes];
     struct {
-      float o[kWarps][8 * NT][D];
-      float m[kWarps][8 * NT], l[kWarps][8 * NT];
+      float o[W][8 * NT][D];
+      float m[W][8 * NT], l[W][8 * NT];
     } merge;
   };
-  uint64_t full[kWarps][ST];
-  int64_t scan[kWarps];
-  int64_t total, base;
-  int item, abort;
+  uint64_t full[W][ST];
+  int scan[W];
+  int item, base, abort;
 };
 
 // The warp's share of a unit: its columns' running reference m, sums l and O^T.
@@ -128,24 +134,30 @@ struct Columns {
 
 // Raises the reference m where a logit has passed it by kRaise (always on a first finite logit),
 // and rescales what was summed under the old one.
-template <int D, int NT>
-FPX_INLINE void follow(Columns<D, NT> &c, const float (&y)[NT][4]) {
+template <int D, int NT, int GS>
+FPX_INLINE void follow(Columns<D, NT> &c, const float (&y)[GS][NT][4]) {
+  float top[NT][2];
   bool up = false;
 #pragma unroll
   for (int n = 0; n < NT; ++n)
 #pragma unroll
-    for (int e = 0; e < 2; ++e) up |= fmaxf(y[n][e], y[n][e + 2]) > c.m[n][e] + kRaise;
+    for (int e = 0; e < 2; ++e) {
+      top[n][e] = fmaxf(y[0][n][e], y[0][n][e + 2]);
+#pragma unroll
+      for (int h = 1; h < GS; ++h) top[n][e] = tc::fmax3(top[n][e], y[h][n][e], y[h][n][e + 2]);
+      up |= top[n][e] > c.m[n][e] + kRaise;
+    }
   if (!__any_sync(0xffffffffu, up)) return;
 #pragma unroll
   for (int n = 0; n < NT; ++n)
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      float x = fmaxf(y[n][e], y[n][e + 2]);
+      float x = top[n][e];
       x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
       x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
       x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
       const float m = fmaxf(c.m[n][e], x);
-      const float keep = c.m[n][e] == -INFINITY ? 0.f : tc::ex2(c.m[n][e] - m);
+      const float keep = tc::ex2(c.m[n][e] - m);
       c.m[n][e] = m;
       c.l[n][e] *= keep;
 #pragma unroll
@@ -160,7 +172,9 @@ FPX_INLINE void follow(Columns<D, NT> &c, const float (&y)[NT][4]) {
 template <int FMT, int D, int NT>
 struct Queries {
   uint32_t b[D / 16][NT][2];
-  float start[FMT == FPX_PAGES_INT4 ? D / 32 : 1][NT][2];  // -136 sum(q) of a group, columns 2t, 2t + 1
+  // int4: the codes' offset, -136 sum(q) of each group, as three bf16 terms: it multiplies the groups' scales in one more
+  // product of four groups x (high, middle, low) for every 128 dims
+  uint32_t off[FMT == FPX_PAGES_INT4 ? D / 128 : 1][NT][2];
 };
 template <int FMT, int D, int NT>
 FPX_INLINE void load_queries(Queries<FMT, D, NT> &f, const PagedDecodeParams &p, int b, int row0, int rows, int kvh,
@@ -173,23 +187,35 @@ FPX_INLINE void load_queries(Queries<FMT, D, NT> &f, const PagedDecodeParams &p,
     const __nv_bfloat16 *q = p.q + b * p.q_sb + (int64_t)(live ? r / p.group : 0) * p.q_sl +
                              (int64_t)(kvh * p.group + (live ? r % p.group : 0)) * p.q_sh;
     if constexpr (FMT == FPX_PAGES_INT4) {
+      uint4 w[D / 32];
 #pragma unroll
-      for (int j = 0; j < D / 32; ++j) {
-        uint4 w = make_uint4(0, 0, 0, 0);
-        if (live) w = *reinterpret_cast<const uint4 *>(q + 32 * j + 8 * t);
-        // the codes' pairs are (i, i + 4) of a lane's eight dims
-        f.b[2 * j][n][0] = __byte_perm(w.x, w.z, 0x5410);
-        f.b[2 * j][n][1] = __byte_perm(w.x, w.z, 0x7632);
-        f.b[2 * j + 1][n][0] = __byte_perm(w.y, w.w, 0x5410);
-        f.b[2 * j + 1][n][1] = __byte_perm(w.y, w.w, 0x7632);
-        const uint32_t v[4] = {w.x, w.y, w.z, w.w};
-        float sum = 0.f;
+      for (int j = 0; j < D / 32; ++j)
+        w[j] = live ? *reinterpret_cast<const uint4 *>(q + 32 * j + 8 * t) : make_uint4(0, 0, 0, 0);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) sum += __uint_as_float(v[i] << 16) + __uint_as_float(v[i] & 0xffff0000u);
-        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-        f.start[j][n][0] = -136.f * __shfl_sync(0xffffffffu, sum, 8 * t);
-        f.start[j][n][1] = -136.f * __shfl_sync(0xffffffffu, sum, 8 * t + 4);
+      for (int J = 0; J < D / 128; ++J) {
+        float sum[4];
+#pragma unroll
+        for (int jj = 0; jj < 4; ++jj) {
+          const int j = 4 * J + jj;
+          // the codes' pairs are (i, i + 4) of a lane's eight dims
+          f.b[2 * j][n][0] = __byte_perm(w[j].x, w[j].z, 0x5410);
+          f.b[2 * j][n][1] = __byte_perm(w[j].x, w[j].z, 0x7632);
+          f.b[2 * j + 1][n][0] = __byte_perm(w[j].y, w[j].w, 0x5410);
+          f.b[2 * j + 1][n][1] = __byte_perm(w[j].y, w[j].w, 0x7632);
+          const uint32_t v[4] = {w[j].x, w[j].y, w[j].z, w[j].w};
+          float x = 0.f;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) x += __uint_as_float(v[i] << 16) + __uint_as_float(v[i] & 0xffff0000u);
+          x += __shfl_xor_sync(0xffffffffu, x, 1);
+          x += __shfl_xor_sync(0xffffffffu, x, 2);
+          sum[jj] = -136.f * x;
+        }
+        // k = 2 t, 2 t + 1 of the product: groups 2 (t & 1), + 1; terms high (t < 2), middle; k + 8: low, none
+        const float x0 = t & 1 ? sum[2] : sum[0], x1 = t & 1 ? sum[3] : sum[1];
+        const float h0 = __bfloat162float(__float2bfloat16_rn(x0)), h1 = __bfloat162float(__float2bfloat16_rn(x1));
+        const float m0 = __bfloat162float(__float2bfloat16_rn(x0 - h0)), m1 = __bfloat162float(__float2bfloat16_rn(x1 - h1));
+        f.off[J][n][0] = t < 2 ? pack_bf16(h0, h1) : pack_bf16(m0, m1);
+        f.off[J][n][1] = t < 2 ? pack_bf16(x0 - h0 - m0, x1 - h1 - m1) : 0u;
       }
     } else {
 #pragma unroll
@@ -201,16 +227,11 @@ FPX_INLINE void load_queries(Queries<FMT, D, NT> &f, const PagedDecodeParams &p,
   }
 }
 
-// One granule: keys key0 .. key0 + 15, of which the unit's rows see those below `seen` (all of
-// them unless `edge`); limit: the keys that this lane's columns see.
+// S^T of one granule: y[n] = keys (g, g + 8) x columns (2 t, 2 t + 1), without the softmax's scale.
 template <int FMT, int D, int NT>
-FPX_INLINE void attend_granule(Columns<D, NT> &c, const Queries<FMT, D, NT> &f, uint8_t *gran, int key0, bool edge,
-                               int seen, const int (&limit)[NT][2], float scale_log2, int lane) {
+FPX_INLINE void scores(float (&y)[NT][4], const Queries<FMT, D, NT> &f, const uint8_t *gran, int lane) {
   using G = Granule<FMT, D>;
   const int g = lane >> 2, t = lane & 3;
-  float y[NT][4];
-#pragma unroll
-  for (int n = 0; n < NT; ++n) y[n][0] = y[n][1] = y[n][2] = y[n][3] = 0.f;
   if constexpr (FMT == FPX_PAGES_INT4) {
 #pragma unroll
     for (int J = 0; J < D / 128; ++J) {
@@ -218,9 +239,20 @@ FPX_INLINE void attend_granule(Columns<D, NT> &c, const Queries<FMT, D, NT> &f, 
       const uint2 sa = *reinterpret_cast<const uint2 *>(gran + G::kKScales + g * (D / 16) + 8 * J);
       const uint2 sb = *reinterpret_cast<const uint2 *>(gran + G::kKScales + (g + 8) * (D / 16) + 8 * J);
       const uint32_t wa[4] = {ka.x, ka.y, ka.z, ka.w}, wb[4] = {kb.x, kb.y, kb.z, kb.w};
+      {
+        const uint32_t xa = t & 1 ? sa.y : sa.x, xb = t & 1 ? sb.y : sb.x;
+        const uint32_t a[4] = {xa, xb, xa, xb};
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          if (J == 0)
+            mma_bf16_zero(y[n], a, f.off[J][n][0], f.off[J][n][1]);
+          else
+            mma_bf16_16816(y[n], a, f.off[J][n][0], f.off[J][n][1]);
+        }
+      }
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const uint32_t lo = 0x000f000fu, one = 0x43004300u;
+        const uint32_t lo = 0x000f000fu, one = 0x43004300u;  // bf16 128 + n
         const uint32_t a0[4] = {and_or(wa[j], lo, one), and_or(wb[j], lo, one), and_or(wa[j] >> 4, lo, one),
                                 and_or(wb[j] >> 4, lo, one)};
         const uint32_t a1[4] = {and_or(wa[j] >> 8, lo, one), and_or(wb[j] >> 8, lo, one), and_or(wa[j] >> 12, lo, one),
@@ -231,8 +263,8 @@ FPX_INLINE void attend_granule(Columns<D, NT> &c, const Queries<FMT, D, NT> &f, 
         const int gr = 4 * J + j;
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-          float acc[4] = {f.start[gr][n][0], f.start[gr][n][1], f.start[gr][n][0], f.start[gr][n][1]};
-          mma_bf16_16816(acc, a0, f.b[2 * gr][n][0], f.b[2 * gr][n][1]);
+          float acc[4];
+          mma_bf16_zero(acc, a0, f.b[2 * gr][n][0], f.b[2 * gr][n][1]);
           mma_bf16_16816(acc, a1, f.b[2 * gr + 1][n][0], f.b[2 * gr + 1][n][1]);
           y[n][0] = fmaf(fa, acc[0], y[n][0]);
           y[n][1] = fmaf(fa, acc[1], y[n][1]);
@@ -244,6 +276,8 @@ FPX_INLINE void attend_granule(Columns<D, NT> &c, const Queries<FMT, D, NT> &f, 
   } else {
     const int r = (lane & 7) + (lane & 8), hi = lane >> 4;
 #pragma unroll
+    for (int n = 0; n < NT; ++n) y[n][0] = y[n][1] = y[n][2] = y[n][3] = 0.f;
+#pragma unroll
     for (int kk = 0; kk < D / 16; ++kk) {
       uint32_t a[4];
       ldmatrix_x4(a[0], a[1], a[2], a[3], smem_u32(gran + r * G::kRow + (((2 * kk + hi) ^ (r & 7)) << 4)));
@@ -251,32 +285,15 @@ FPX_INLINE void attend_granule(Columns<D, NT> &c, const Queries<FMT, D, NT> &f, 
       for (int n = 0; n < NT; ++n) mma_bf16_16816(y[n], a, f.b[kk][n][0], f.b[kk][n][1]);
     }
   }
-  float ea = 0.f, eb = 0.f;  // row exponents of the two keys' values
+}
+
+// O^T += V^T P^T of one granule; y: the probabilities; wa, wb: 2^-e of the two keys (int4). EDGE: tokens
+// from `have` on are not there (unseen, or on a missing page), and may hold anything.
+template <int FMT, int D, int NT, bool EDGE>
+FPX_INLINE void values(Columns<D, NT> &c, const float (&y)[NT][4], float wa, float wb, uint8_t *gran, int have, int lane) {
+  using G = Granule<FMT, D>;
+  const int g = lane >> 2, t = lane & 3;
   if constexpr (FMT == FPX_PAGES_INT4) {
-    ea = __uint_as_float((uint32_t)*reinterpret_cast<const uint16_t *>(gran + G::kVExps + 2 * g) << 16);
-    eb = __uint_as_float((uint32_t)*reinterpret_cast<const uint16_t *>(gran + G::kVExps + 2 * g + 16) << 16);
-    if (edge) {  // nothing of a key that no row sees may enter: the memory may never have been written
-      ea = key0 + g < seen ? ea : 0.f;
-      eb = key0 + g + 8 < seen ? eb : 0.f;
-    }
-  }
-#pragma unroll
-  for (int n = 0; n < NT; ++n)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      y[n][e] = fmaf(y[n][e], scale_log2, e < 2 ? ea : eb);
-      if (edge && key0 + g + (e < 2 ? 0 : 8) >= limit[n][e & 1]) y[n][e] = -INFINITY;
-    }
-  follow<D, NT>(c, y);
-#pragma unroll
-  for (int n = 0; n < NT; ++n)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float m = c.m[n][e & 1];
-      y[n][e] = tc::ex2(y[n][e] - (m == -INFINITY ? 0.f : m));
-    }
-  if constexpr (FMT == FPX_PAGES_INT4) {
-    const float wa = tc::ex2(-ea), wb = tc::ex2(-eb);
     uint32_t pb[NT][2];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
@@ -285,9 +302,8 @@ FPX_INLINE void attend_granule(Columns<D, NT> &c, const Queries<FMT, D, NT> &f, 
       pb[n][0] = transpose8(pack_f16(y[n][0], y[n][1]));
       pb[n][1] = transpose8(pack_f16(y[n][2], y[n][3]));
     }
-    // scales of the token pairs t and t + 4; those of unseen tokens are zero
-    const uint32_t keep0 = edge ? (key0 + 2 * t < seen ? 0xffffu : 0u) | (key0 + 2 * t + 1 < seen ? 0xffff0000u : 0u) : ~0u;
-    const uint32_t keep1 = edge ? (key0 + 2 * t + 8 < seen ? 0xffffu : 0u) | (key0 + 2 * t + 9 < seen ? 0xffff0000u : 0u) : ~0u;
+    const uint32_t keep0 = (2 * t < have ? 0xffffu : 0u) | (2 * t + 1 < have ? 0xffff0000u : 0u);
+    const uint32_t keep1 = (2 * t + 8 < have ? 0xffffu : 0u) | (2 * t + 9 < have ? 0xffff0000u : 0u);
 #pragma unroll
     for (int J = 0; J < D / 128; ++J) {
       const uint4 va = lds128(gran + G::kVCodes + v_chunk(2 * t, J, g)), vb = lds128(gran + G::kVCodes + v_chunk(2 * t + 8, J, g));
@@ -307,7 +323,7 @@ FPX_INLINE void attend_granule(Columns<D, NT> &c, const Queries<FMT, D, NT> &f, 
         const int i = 8 * J + 2 * j;
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-          const uint32_t b0 = hmul2u(pb[n][0], r0[j] & keep0), b1 = hmul2u(pb[n][1], r1[j] & keep1);
+          const uint32_t b0 = hmul2u(pb[n][0], EDGE ? r0[j] & keep0 : r0[j]), b1 = hmul2u(pb[n][1], EDGE ? r1[j] & keep1 : r1[j]);
           mma_f16_16816(c.o[i][n], a0, b0, b1);
           mma_f16_16816(c.o[i + 1][n], a1, b0, b1);
         }
@@ -327,10 +343,10 @@ FPX_INLINE void attend_granule(Columns<D, NT> &c, const Queries<FMT, D, NT> &f, 
         pl[n][e] = transpose8(pack_bf16(x0 - __uint_as_float(h << 16), x1 - __uint_as_float(h & 0xffff0000u)));
       }
     const int r = (lane & 7) + ((lane >> 4) << 3), hi = (lane >> 3) & 1;
-    if (edge) {  // rows of V that no row sees may hold anything
+    if (EDGE) {
       for (int i = lane; i < kGranule * (D / 8); i += 32) {
         const int row = i / (D / 8);
-        if (key0 + row >= seen) *reinterpret_cast<uint4 *>(gran + row * G::kRow + 2 * D + 16 * (i % (D / 8))) = make_uint4(0, 0, 0, 0);
+        if (row >= have) *reinterpret_cast<uint4 *>(gran + row * G::kRow + 2 * D + 16 * (i % (D / 8))) = make_uint4(0, 0, 0, 0);
       }
       __syncwarp();
     }
@@ -347,6 +363,50 @@ FPX_INLINE void attend_granule(Columns<D, NT> &c, const Queries<FMT, D, NT> &f, 
   }
 }
 
+// One step: GS granules from key0 on. EDGE: the unit's rows see only keys below `seen`, this lane's
+// columns those below limit, and the granules of `dead` are on missing pages.
+template <int FMT, int D, int NT, int GS, bool EDGE>
+FPX_INLINE void attend_step(Columns<D, NT> &c, const Queries<FMT, D, NT> &f, uint8_t *stage, int key0, int seen,
+                            const int (&limit)[NT][2], uint32_t dead, float scale_log2, int lane) {
+  using G = Granule<FMT, D>;
+  const int g = lane >> 2;
+  float y[GS][NT][4], w[GS][2];
+  int have[GS];
+#pragma unroll
+  for (int h = 0; h < GS; ++h) {
+    uint8_t *gran = stage + h * G::kBytes;
+    scores<FMT, D, NT>(y[h], f, gran, lane);
+    have[h] = !EDGE ? kGranule : (dead >> h) & 1 ? 0 : max(0, seen - key0 - kGranule * h);
+    w[h][0] = w[h][1] = 1.f;
+    float e[2] = {0.f, 0.f};  // row exponents of the two keys' values
+    if constexpr (FMT == FPX_PAGES_INT4) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        e[i] = __uint_as_float((uint32_t)*reinterpret_cast<const uint16_t *>(gran + G::kVExps + 2 * g + 16 * i) << 16);
+        if (EDGE && g + 8 * i >= have[h]) e[i] = 0.f;
+        w[h][i] = tc::ex2(-e[i]);
+      }
+    }
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        y[h][n][i] = fmaf(y[h][n][i], scale_log2, e[i >> 1]);
+        const int k = g + 8 * (i >> 1);
+        if (EDGE && (k >= have[h] || key0 + kGranule * h + k >= limit[n][i & 1])) y[h][n][i] = -INFINITY;
+      }
+  }
+  follow<D, NT, GS>(c, y);
+#pragma unroll
+  for (int h = 0; h < GS; ++h) {
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) y[h][n][i] = tc::ex2(y[h][n][i] - c.m[n][i & 1]);
+    values<FMT, D, NT, EDGE>(c, y[h], w[h][0], w[h][1], stage + h * G::kBytes, have[h], lane);
+  }
+}
+
 // Dim of O^T row `row` (0 or 8 + g: the accumulator's two rows) of tile i: the V codes' layout
 // gives a lane four neighbouring dims over two tiles, ldmatrix the plain order.
 template <int FMT>
@@ -354,54 +414,65 @@ FPX_INLINE int out_dim(int i, int g, int second) {
   return FMT == FPX_PAGES_INT4 ? 16 * (i & ~1) + 4 * g + 2 * (i & 1) + second : 16 * i + 8 * second + g;
 }
 
-template <int FMT, int D, int NT, int ST, int OCC>
-__global__ void __launch_bounds__(32 * kWarps, OCC) paged_decode_kernel(const __grid_constant__ PagedDecodeParams p) {
+template <int FMT, int D, int NT, int GS, int W, int ST, int OCC>
+__global__ void __launch_bounds__(32 * W, OCC) paged_decode_kernel(const __grid_constant__ PagedDecodeParams p) {
   using G = Granule<FMT, D>;
-  using Smem = PagedSmem<FMT, D, NT, ST>;
-  constexpr int kRows = 8 * NT;
+  using Smem = PagedSmem<FMT, D, NT, GS, W, ST>;
+  constexpr int kStep = GS * kGranule, kBytes = GS * G::kBytes;
+  constexpr uint32_t kAll = (1u << GS) - 1;
+  constexpr int kRows = 8 * NT, kThreads = 32 * W;
   extern __shared__ __align__(128) uint8_t smem_raw[];
   Smem &sh = *reinterpret_cast<Smem *>(smem_raw);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   const int items = p.B * p.blocks;
-
-  // This CTA's run of granules, and the item that it starts in.
-  const int chunk = (items + 32 * kWarps - 1) / (32 * kWarps);
-  const int i0 = min(items, tid * chunk), i1 = min(items, i0 + chunk);
-  int64_t mine = 0;
-  for (int i = i0; i < i1; ++i) mine += (int64_t)granules_of(item_keys<NT>(p, i / p.blocks, i % p.blocks)) * p.Hkv;
-  int64_t incl = mine;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int64_t x = __shfl_up_sync(0xffffffffu, incl, o);
-    if (lane >= o) incl += x;
-  }
-  if (lane == 31) sh.scan[warp] = incl;
   if (lane < ST) tc::mbar_init(&sh.full[warp][lane], 1);
   if (tid == 0) sh.abort = 0;
   tc::fence_barrier_init();
-  __syncthreads();
-  int64_t total = 0, before = incl - mine;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+
+  // This CTA's run of steps, and the item that it starts in.
+  const int chunk = (items + kThreads - 1) / kThreads;
+  const int i0 = min(items, tid * chunk), i1 = min(items, i0 + chunk);
+  auto steps_in = [&](int i) {
+    const int b = i / p.blocks;
+    int start, count;
+    p.pv.rows(b, p.Lq, start, count);
+    return steps_of<GS>(item_keys<NT>(p, start, count, i - b * p.blocks)) * p.Hkv;
+  };
+  int mine = 0;
+  for (int i = i0; i < i1; ++i) mine += steps_in(i);
+  int before = mine;
 #pragma unroll
-  for (int w = 0; w < kWarps; ++w) {
+  for (int o = 1; o < 32; o <<= 1) {
+    const int x = __shfl_up_sync(0xffffffffu, before, o);
+    if (lane >= o) before += x;
+  }
+  if (lane == 31) sh.scan[warp] = before;
+  before -= mine;
+  __syncthreads();
+  int total = 0;
+#pragma unroll
+  for (int w = 0; w < W; ++w) {
     if (w < warp) before += sh.scan[w];
     total += sh.scan[w];
   }
   if (blockIdx.x == 0) {  // for the merge
-    int64_t at = before;
+    int at = before;
     for (int i = i0; i < i1; ++i) {
       p.prefix[i] = at;
-      at += (int64_t)granules_of(item_keys<NT>(p, i / p.blocks, i % p.blocks)) * p.Hkv;
+      at += chunk == 1 ? mine : steps_in(i);
     }
     if (tid == 0) p.prefix[items] = total;
   }
-  const int64_t per = max((int64_t)p.min_granules, (total + p.ctas - 1) / p.ctas);
-  int64_t lo = blockIdx.x * per;
-  const int64_t hi = min(total, lo + per);
+  const int per = max(p.min_steps, (total + p.ctas - 1) / p.ctas);
+  int lo = (int)min((int64_t)blockIdx.x * per, (int64_t)total);
+  const int hi = min(total, lo + per);
   if (lo >= hi) return;
   if (before <= lo && lo < before + mine) {
-    int64_t at = before;
+    int at = before;
     for (int i = i0; i < i1; ++i) {
-      const int64_t n = (int64_t)granules_of(item_keys<NT>(p, i / p.blocks, i % p.blocks)) * p.Hkv;
+      const int n = chunk == 1 ? mine : steps_in(i);
       if (lo < at + n) {
         sh.item = i;
         sh.base = at;
@@ -412,43 +483,57 @@ __global__ void __launch_bounds__(32 * kWarps, OCC) paged_decode_kernel(const __
   }
   __syncthreads();
 
-  int item = sh.item;
-  int64_t base = sh.base;
-  uint32_t issued = 0, taken = 0, bad = 0;  // granules of this warp's ring; bad: stages whose page does not exist
+  int item = sh.item, base = sh.base;
+  uint32_t issued = 0, taken = 0, dead = 0;  // steps through this warp's ring; dead: GS bits a stage
   bool stopped = false;
   while (lo < hi) {
-    const int b = item / p.blocks, rb = item % p.blocks;
-    const int seen = item_keys<NT>(p, b, rb), n_gran = granules_of(seen);
-    if (n_gran == 0 || lo >= base + (int64_t)n_gran * p.Hkv) {  // hi > lo: another item has granules left
-      base += (int64_t)n_gran * p.Hkv;
+    const int b = item / p.blocks, rb = item - b * p.blocks;
+    int start, count;
+    p.pv.rows(b, p.Lq, start, count);
+    const int seen = item_keys<NT>(p, start, count, rb), n_steps = steps_of<GS>(seen);
+    if (lo - base >= n_steps * p.Hkv) {  // hi > lo: another item has steps left
+      base += n_steps * p.Hkv;
       ++item;
       continue;
     }
-    const int kvh = (int)((lo - base) / n_gran), g0 = (int)((lo - base) % n_gran);
-    const int g1 = (int)min((int64_t)n_gran, g0 + (hi - lo));
-    const int start = p.pv.starts[b], rows = p.pv.count(b, p.Lq) * p.group, row0 = rb * kRows;
+    const int kvh = (lo - base) / n_steps, g0 = (lo - base) - kvh * n_steps;
+    const int g1 = min(n_steps, g0 + (hi - lo));
+    const int rows = count * p.group, row0 = rb * kRows;
 
-    // Ring: copy granule g0 + warp + 4 i into stage (issued mod ST).
+    // Ring: copy step g0 + warp + W i into stage (issued mod ST).
     const int32_t *table = p.pv.table + (int64_t)b * p.pv.table_stride;
     const uint8_t *heads = p.pv.pool + (int64_t)kvh * p.pv.head_bytes;
-    const int todo = g1 - g0 > warp ? (g1 - g0 - warp + kWarps - 1) / kWarps : 0;
+    const int todo = g1 - g0 > warp ? (g1 - g0 - warp + W - 1) / W : 0;
+    const int last_page = (seen - 1) >> (p.pv.page_shift + 4);
     int sent = 0, page = 0;
     auto issue = [&]() {
-      if ((sent & 31) == 0) {
-        const int gi = g0 + warp + kWarps * (sent + lane);
-        page = gi < g1 ? table[gi >> p.pv.page_shift] : 0;
-      }
-      const int gi = g0 + warp + kWarps * sent;
-      const int pg = __shfl_sync(0xffffffffu, page, sent & 31);
-      const bool ok = (unsigned)pg < (unsigned)p.pv.pages;
+      const int first = GS * (g0 + warp + W * sent);  // granule
       const int st = issued % ST;
-      bad = ok ? bad & ~(1u << st) : bad | (1u << st);
-      if (lane == 0) {
-        if (!ok) p.pv.fail();
-        tc::mbar_expect_tx(&sh.full[warp][st], G::kBytes);
-        bulk_load(sh.ring[warp][st],
-                  heads + (int64_t)(ok ? pg : 0) * p.pv.page_bytes + (int64_t)(gi & ((1 << p.pv.page_shift) - 1)) * G::kBytes,
-                  G::kBytes, &sh.full[warp][st]);
+      uint64_t *bar = &sh.full[warp][st];
+      uint8_t *dst = sh.ring[warp][st];
+      if (GS == 1 || p.pv.page_shift > 0) {  // all granules on one page
+        if ((sent & 31) == 0) page = table[min((GS * (g0 + warp + W * (sent + lane))) >> p.pv.page_shift, last_page)];
+        const int pg = __shfl_sync(0xffffffffu, page, sent & 31);
+        const bool ok = (unsigned)pg < (unsigned)p.pv.pages;
+        dead = (dead & ~(kAll << (GS * st))) | (ok ? 0u : kAll << (GS * st));
+        if (lane == 0) {
+          if (!ok) p.pv.fail();
+          tc::mbar_expect_tx(bar, kBytes);
+          bulk_load(dst, heads + (int64_t)(ok ? pg : 0) * p.pv.page_bytes + (first & ((1 << p.pv.page_shift) - 1)) * G::kBytes,
+                    kBytes, bar);
+        }
+      } else {  // a page each; the second granule of a sequence's last step may not exist
+        if ((sent & 15) == 0) page = table[min(2 * (g0 + warp + W * (sent + (lane >> 1))) + (lane & 1), last_page)];
+        const bool both = first + 1 <= last_page;
+        const int pa = __shfl_sync(0xffffffffu, page, 2 * (sent & 15)), pb = __shfl_sync(0xffffffffu, page, 2 * (sent & 15) + 1);
+        const bool oka = (unsigned)pa < (unsigned)p.pv.pages, okb = both && (unsigned)pb < (unsigned)p.pv.pages;
+        dead = (dead & ~(kAll << (GS * st))) | ((oka ? 0u : 1u) | (okb ? 0u : 2u)) << (GS * st);
+        if (lane == 0) {
+          if (!oka || (both && !okb)) p.pv.fail();
+          tc::mbar_expect_tx(bar, (okb ? 2 : 1) * G::kBytes);
+          bulk_load(dst, heads + (int64_t)(oka ? pa : 0) * p.pv.page_bytes, G::kBytes, bar);
+          if (okb) bulk_load(dst + G::kBytes, heads + (int64_t)pb * p.pv.page_bytes, G::kBytes, bar);
+        }
       }
       ++issued;
       ++sent;
@@ -463,7 +548,7 @@ __global__ void __launch_bounds__(32 * kWarps, OCC) paged_decode_kernel(const __
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int r = row0 + 8 * n + 2 * t + e;
-        limit[n][e] = r < rows ? min(seen, start + r / p.group + 1) : seen;
+        limit[n][e] = r < rows ? (int)min((int64_t)seen, (int64_t)start + r / p.group + 1) : seen;
         least = min(least, limit[n][e]);
       }
     least = min(least, __shfl_xor_sync(0xffffffffu, least, 1));
@@ -471,7 +556,7 @@ __global__ void __launch_bounds__(32 * kWarps, OCC) paged_decode_kernel(const __
     Columns<D, NT> c;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      c.m[n][0] = c.m[n][1] = -INFINITY;
+      c.m[n][0] = c.m[n][1] = kLowest;
       c.l[n][0] = c.l[n][1] = 0.f;
 #pragma unroll
       for (int i = 0; i < D / 16; ++i) c.o[i][n][0] = c.o[i][n][1] = c.o[i][n][2] = c.o[i][n][3] = 0.f;
@@ -480,21 +565,23 @@ __global__ void __launch_bounds__(32 * kWarps, OCC) paged_decode_kernel(const __
       const int st = taken % ST;
       if (!tc::mbar_wait_warp(&sh.full[warp][st], (taken / ST) & 1, &sh.abort)) {
         stopped = true;  // the copy did not arrive: report it and let the launch end
-        if (lane == 0 && p.pv.error) atomicMax(p.pv.error, 1);
+        if (lane == 0 && p.pv.error) atomicMax(p.pv.error, FPX_DEVICE_WAIT);
         break;
       }
       ++taken;
-      const int key0 = (g0 + warp + kWarps * i) * kGranule;
-      const bool lost = (bad >> st) & 1;
-      if (!lost) attend_granule<FMT, D, NT>(c, f, sh.ring[warp][st], key0, key0 + kGranule > least, seen, limit, p.scale_log2, lane);
+      const int key0 = (g0 + warp + W * i) * kStep;
+      const uint32_t gone = (dead >> (GS * st)) & kAll;
+      if (key0 + kStep <= least && !gone)
+        attend_step<FMT, D, NT, GS, false>(c, f, sh.ring[warp][st], key0, seen, limit, 0u, p.scale_log2, lane);
+      else
+        attend_step<FMT, D, NT, GS, true>(c, f, sh.ring[warp][st], key0, seen, limit, gone, p.scale_log2, lane);
       if (sent < todo) {
-        // the granule's reads (and the zeros written behind a sequence's end) come before the next copy into the stage
+        // the step's reads (and the zeros written over unseen values) come before the next copy into the stage
         if (FMT == FPX_PAGES_BF16) tc::fence_proxy_async();
         __syncwarp();
         issue();
       }
     }
-
     if (stopped)  // copies still in flight end before this memory is used again, or this long later
       for (; taken < issued; ++taken) {
         const long long from = clock64();
@@ -502,7 +589,7 @@ __global__ void __launch_bounds__(32 * kWarps, OCC) paged_decode_kernel(const __
         }
       }
 
-    // Merge the four warps through the ring's memory.
+    // Merge the warps through the ring's memory.
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -511,7 +598,7 @@ __global__ void __launch_bounds__(32 * kWarps, OCC) paged_decode_kernel(const __
         c.l[n][e] += __shfl_xor_sync(0xffffffffu, c.l[n][e], 8);
         c.l[n][e] += __shfl_xor_sync(0xffffffffu, c.l[n][e], 16);
       }
-    __syncthreads();  // every warp has read its last granule
+    __syncthreads();  // every warp has read its last step
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -528,38 +615,36 @@ __global__ void __launch_bounds__(32 * kWarps, OCC) paged_decode_kernel(const __
         }
       }
     __syncthreads();
-    const bool whole = g0 == 0 && g1 == n_gran;
+    const bool whole = g0 == 0 && g1 == n_steps;
     const int64_t slot = blockIdx.x + (int64_t)item * p.Hkv + kvh;
-    for (int r = 0; r < kRows && row0 + r < rows; ++r) {
-      float m = -INFINITY, l = 0.f, o[D / 128] = {};
+    constexpr int kQuads = D / 4;
+    for (int i = tid; i < kRows * kQuads; i += kThreads) {
+      const int r = i / kQuads, d = 4 * (i % kQuads);
+      if (row0 + r >= rows) break;
+      float m = sh.merge.m[0][r], l = 0.f;
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w) m = fmaxf(m, sh.merge.m[w][r]);
+      for (int w = 1; w < W; ++w) m = fmaxf(m, sh.merge.m[w][r]);
+      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w) {
-        const float mw = sh.merge.m[w][r];
-        const float s = mw == -INFINITY ? 0.f : exp2f(mw - m);
-        l += sh.merge.l[w][r] * s;
-#pragma unroll
-        for (int J = 0; J < D / 128; ++J) o[J] += sh.merge.o[w][r][tid + 128 * J] * s;
+      for (int w = 0; w < W; ++w) {
+        const float s = tc::ex2(sh.merge.m[w][r] - m);
+        const float4 x = *reinterpret_cast<const float4 *>(&sh.merge.o[w][r][d]);
+        l = fmaf(sh.merge.l[w][r], s, l);
+        o.x = fmaf(x.x, s, o.x); o.y = fmaf(x.y, s, o.y); o.z = fmaf(x.z, s, o.z); o.w = fmaf(x.w, s, o.w);
       }
       if (whole) {
         const int row = (row0 + r) / p.group, h = kvh * p.group + (row0 + r) % p.group;
         const float inv = l == 0.f ? 0.f : 1.f / l;
-#pragma unroll
-        for (int J = 0; J < D / 128; ++J)
-          p.out[b * p.o_sb + row * p.o_sl + h * p.o_sh + tid + 128 * J] = __float2bfloat16_rn(o[J] * inv);
-        if (p.lse && tid == 0)
-          p.lse[((int64_t)b * p.Lq + row) * p.H + h] = l == 0.f ? -INFINITY : m * kLn2 + logf(l);
+        __nv_bfloat16 *out = p.out + b * p.o_sb + row * p.o_sl + h * p.o_sh + d;
+        out[0] = __float2bfloat16_rn(o.x * inv); out[1] = __float2bfloat16_rn(o.y * inv);
+        out[2] = __float2bfloat16_rn(o.z * inv); out[3] = __float2bfloat16_rn(o.w * inv);
+        if (p.lse && d == 0) p.lse[((int64_t)b * p.Lq + row) * p.H + h] = l == 0.f ? -INFINITY : m * kLn2 + logf(l);
       } else {
-#pragma unroll
-        for (int J = 0; J < D / 128; ++J) p.part_o[(slot * kRows + r) * D + tid + 128 * J] = o[J];
-        if (tid == 0) {
-          p.part_ml[2 * (slot * kRows + r)] = m;
-          p.part_ml[2 * (slot * kRows + r) + 1] = l;
-        }
+        *reinterpret_cast<float4 *>(&p.part_o[(slot * kRows + r) * D + d]) = o;
+        if (d == 0) *reinterpret_cast<float2 *>(&p.part_ml[2 * (slot * kRows + r)]) = make_float2(m, l);
       }
     }
-    tc::fence_proxy_async();  // these writes of shared memory come before the next unit's copies
+    tc::fence_proxy_async();  // these accesses of shared memory come before the next unit's copies
     __syncthreads();
     lo += g1 - g0;
   }
@@ -570,32 +655,35 @@ __global__ void __launch_bounds__(32 * kWarps, OCC) paged_decode_kernel(const __
 constexpr int kMergeThreads = 256;
 template <int D, int NT>
 __global__ void __launch_bounds__(kMergeThreads) paged_merge_kernel(const __grid_constant__ PagedDecodeParams p) {
-  asm volatile("griddepcontrol.wait;" ::: "memory");
   constexpr int kPieces = kMergeThreads / (D / 4), kRows = 8 * NT;
   const int r = blockIdx.y, kvh = blockIdx.x % p.Hkv, item = blockIdx.x / p.Hkv;
   const int b = item / p.blocks, rr = (item % p.blocks) * kRows + r;
-  if (rr >= p.Lq * p.group) return;
   const int row = rr / p.group, h = kvh * p.group + rr % p.group;
   const int tid = threadIdx.x, piece = tid / (D / 4), d = 4 * (tid % (D / 4));
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (rr >= p.Lq * p.group) return;
+  int start, count;
+  p.pv.rows(b, p.Lq, start, count);
   __nv_bfloat16 *out = p.out + b * p.o_sb + row * p.o_sl + h * p.o_sh;
   float *lse = p.lse ? p.lse + ((int64_t)b * p.Lq + row) * p.H + h : nullptr;
-  const int64_t base = p.prefix[item], n = (p.prefix[item + 1] - base) / p.Hkv, total = p.prefix[p.B * p.blocks];
-  if (row >= p.pv.count(b, p.Lq) || n == 0) {
+  const int base = p.prefix[item], n = (p.prefix[item + 1] - base) / p.Hkv, total = p.prefix[p.B * p.blocks];
+  if (row >= count || n == 0) {
     if (piece == 0) {
       for (int e = 0; e < 4; ++e) out[d + e] = __float2bfloat16_rn(0.f);
       if (lse && d == 0) *lse = -INFINITY;
     }
     return;
   }
-  const int64_t per = max((int64_t)p.min_granules, (total + p.ctas - 1) / p.ctas);
-  const int64_t first = base + kvh * n;
-  const int c0 = (int)(first / per), c1 = (int)((first + n - 1) / per);
+  const int per = max(p.min_steps, (total + p.ctas - 1) / p.ctas);
+  const int first = base + kvh * n;
+  const int c0 = first / per, c1 = (first + n - 1) / per;
   if (c0 == c1) return;  // finished by its CTA
   const int64_t slot0 = c0 + (int64_t)item * p.Hkv + kvh;
   const int pieces = c1 - c0 + 1;
   __shared__ float red[kMergeThreads / 32];
   __shared__ __align__(16) float part[kPieces][D];
-  float m = -INFINITY;
+  __shared__ float sums[kPieces];
+  float m = kLowest;
   for (int i = tid; i < pieces; i += kMergeThreads) m = fmaxf(m, p.part_ml[2 * ((slot0 + i) * kRows + r)]);
   m = block_max<kMergeThreads>(m, red);
   float l = 0.f;
@@ -605,14 +693,11 @@ __global__ void __launch_bounds__(kMergeThreads) paged_merge_kernel(const __grid
     const int64_t at = (slot0 + i) * kRows + r;
     const float2 ml = *reinterpret_cast<const float2 *>(p.part_ml + 2 * at);
     const float4 x = *reinterpret_cast<const float4 *>(p.part_o + at * D + d);
-    const float s = ml.x == -INFINITY ? 0.f : exp2f(ml.x - m);
+    const float s = tc::ex2(ml.x - m);
     l = fmaf(ml.y, s, l);
-    if (s != 0.f) {
-      o.x = fmaf(x.x, s, o.x); o.y = fmaf(x.y, s, o.y); o.z = fmaf(x.z, s, o.z); o.w = fmaf(x.w, s, o.w);
-    }
+    o.x = fmaf(x.x, s, o.x); o.y = fmaf(x.y, s, o.y); o.z = fmaf(x.z, s, o.z); o.w = fmaf(x.w, s, o.w);
   }
   *reinterpret_cast<float4 *>(&part[piece][d]) = o;
-  __shared__ float sums[kPieces];
   if (d == 0) sums[piece] = l;
   __syncthreads();
   l = 0.f;
@@ -633,13 +718,13 @@ __global__ void __launch_bounds__(kMergeThreads) paged_merge_kernel(const __grid
 constexpr int kSms = 148;
 
 template <int FMT, int D, int NT>
-struct Shape;  // stages of a warp's ring, CTAs of an SM
-template <> struct Shape<FPX_PAGES_INT4, 128, 1> { static constexpr int kStages = 4, kOcc = 4; };
-template <> struct Shape<FPX_PAGES_INT4, 128, 2> { static constexpr int kStages = 4, kOcc = 3; };
-template <> struct Shape<FPX_PAGES_INT4, 256, 1> { static constexpr int kStages = 4, kOcc = 2; };
-template <> struct Shape<FPX_PAGES_BF16, 128, 1> { static constexpr int kStages = 2, kOcc = 3; };
-template <> struct Shape<FPX_PAGES_BF16, 128, 2> { static constexpr int kStages = 2, kOcc = 3; };
-template <> struct Shape<FPX_PAGES_BF16, 256, 1> { static constexpr int kStages = 3, kOcc = 1; };
+struct Shape;  // granules of a step, warps of a CTA, stages of a warp's ring, CTAs of an SM
+template <> struct Shape<FPX_PAGES_INT4, 128, 1> { static constexpr int kGranules = 2, kWarps = 4, kStages = 2, kOcc = 4; };
+template <> struct Shape<FPX_PAGES_INT4, 128, 2> { static constexpr int kGranules = 2, kWarps = 4, kStages = 3, kOcc = 3; };
+template <> struct Shape<FPX_PAGES_INT4, 256, 1> { static constexpr int kGranules = 2, kWarps = 4, kStages = 2, kOcc = 2; };
+template <> struct Shape<FPX_PAGES_BF16, 128, 1> { static constexpr int kGranules = 1, kWarps = 4, kStages = 2, kOcc = 3; };
+template <> struct Shape<FPX_PAGES_BF16, 128, 2> { static constexpr int kGranules = 1, kWarps = 4, kStages = 2, kOcc = 3; };
+template <> struct Shape<FPX_PAGES_BF16, 256, 1> { static constexpr int kGranules = 1, kWarps = 4, kStages = 3, kOcc = 1; };
 
 struct Layout {
   int nt, blocks, ctas, rows;
@@ -648,6 +733,11 @@ struct Layout {
 };
 static size_t up256(size_t x) { return (x + 255) & ~size_t(255); }
 
+template <int FMT, int D, int NT>
+constexpr int grid_ctas() {
+  return kSms * Shape<FMT, D, NT>::kOcc;
+}
+
 // Column tiles: two where one would leave rows over, except at head dim 256 (registers).
 static Layout layout_of(int format, int B, int Lq, int H, int Hkv, int d) {
   Layout w{};
@@ -655,33 +745,42 @@ static Layout layout_of(int format, int B, int Lq, int H, int Hkv, int d) {
   w.nt = d == 128 && rows > 8 ? 2 : 1;
   w.rows = 8 * w.nt;
   w.blocks = (int)((rows + w.rows - 1) / w.rows);
-  const int occ = format == FPX_PAGES_INT4 ? (d == 256 ? 2 : w.nt == 1 ? 4 : 3) : (d == 256 ? 1 : 3);
-  w.ctas = kSms * occ;
+  if (format == FPX_PAGES_INT4)
+    w.ctas = d == 256 ? grid_ctas<FPX_PAGES_INT4, 256, 1>()
+                      : w.nt == 1 ? grid_ctas<FPX_PAGES_INT4, 128, 1>() : grid_ctas<FPX_PAGES_INT4, 128, 2>();
+  else
+    w.ctas = d == 256 ? grid_ctas<FPX_PAGES_BF16, 256, 1>()
+                      : w.nt == 1 ? grid_ctas<FPX_PAGES_BF16, 128, 1>() : grid_ctas<FPX_PAGES_BF16, 128, 2>();
   w.units = (int64_t)B * w.blocks * Hkv;
-  w.prefix = up256(((size_t)B * w.blocks + 1) * sizeof(int64_t));
+  w.prefix = up256(((size_t)B * w.blocks + 1) * sizeof(int));
   w.ml = up256((size_t)(w.ctas + w.units) * w.rows * 2 * sizeof(float));
   w.bytes = w.prefix + w.ml + (size_t)(w.ctas + w.units) * w.rows * d * sizeof(float);
   return w;
 }
 
 template <int FMT, int D, int NT>
-static int launch(const PagedDecodeParams &p, const Layout &w, cudaStream_t stream) {
+static int launch(PagedDecodeParams &p, const Layout &w, cudaStream_t stream) {
   using S = Shape<FMT, D, NT>;
-  const int smem = (int)sizeof(PagedSmem<FMT, D, NT, S::kStages>);
-  static_assert(sizeof(PagedSmem<FMT, D, NT, S::kStages>) <= 227 * 1024, "shared memory of one CTA");
-  const auto kernel = paged_decode_kernel<FMT, D, NT, S::kStages, S::kOcc>;
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return FPX_ERR_CUDA;
-  kernel<<<w.ctas, 32 * kWarps, smem, stream>>>(p);
-  FPX_CHECK_LAUNCH();
+  using Smem = PagedSmem<FMT, D, NT, S::kGranules, S::kWarps, S::kStages>;
+  static_assert(sizeof(Smem) <= 227 * 1024, "shared memory of one CTA");
+  const auto kernel = paged_decode_kernel<FMT, D, NT, S::kGranules, S::kWarps, S::kStages, S::kOcc>;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(Smem)) != cudaSuccess)
+    return FPX_ERR_CUDA;
+  p.min_steps = S::kWarps;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)w.units, w.rows);
-  cfg.blockDim = dim3(kMergeThreads);
+  cfg.gridDim = dim3(w.ctas);
+  cfg.blockDim = dim3(32 * S::kWarps);
+  cfg.dynamicSmemBytes = sizeof(Smem);
   cfg.stream = stream;
   cudaLaunchAttribute attr{};
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
+  if (cudaLaunchKernelEx(&cfg, kernel, p) != cudaSuccess) return FPX_ERR_CUDA;
+  cfg.gridDim = dim3((unsigned)w.units, w.rows);
+  cfg.blockDim = dim3(kMergeThreads);
+  cfg.dynamicSmemBytes = 0;
   if (cudaLaunchKernelEx(&cfg, paged_merge_kernel<D, NT>, p) != cudaSuccess) return FPX_ERR_CUDA;
   return FPX_OK;
 }
@@ -715,18 +814,21 @@ extern "C" int fpx_paged_decode_attention(int format, const void *q, int64_t q_s
   if (rc) return rc;
   if (H % Hkv) return FPX_ERR_SHAPE;
   if (!decode_sizes_ok(B, Lq, H, Hkv)) return FPX_ERR_UNSUPPORTED;
-  if ((reinterpret_cast<uintptr_t>(q) & 15) || q_sb % 8 || q_sl % 8 || q_sh % 8) return FPX_ERR_SHAPE;
+  const RowStrides qs(q_sb, q_sl, q_sh, B, Lq, H);
+  if ((reinterpret_cast<uintptr_t>(q) & 15) || !qs.multiples_of(8)) return FPX_ERR_SHAPE;
   const Layout w = layout_of(format, B, Lq, H, Hkv, d);
   if (!workspace || workspace_bytes < w.bytes || (reinterpret_cast<uintptr_t>(workspace) & 15)) return FPX_ERR_WORKSPACE;
-  p.q = static_cast<const __nv_bfloat16 *>(q); p.q_sb = q_sb; p.q_sl = q_sl; p.q_sh = q_sh;
+  p.q = static_cast<const __nv_bfloat16 *>(q); p.q_sb = qs.b; p.q_sl = qs.l; p.q_sh = qs.h;
   p.out = static_cast<__nv_bfloat16 *>(out); p.o_sb = o_sb; p.o_sl = o_sl; p.o_sh = o_sh;
   p.lse = lse;
   p.B = B; p.Lq = Lq; p.H = H; p.Hkv = Hkv; p.group = H / Hkv; p.blocks = w.blocks;
   p.scale_log2 = (float)scale * kLog2e;
   p.ctas = w.ctas;
-  p.min_granules = kWarps;
+  // 32-bit counts of steps: what the table could name in all
+  if ((int64_t)B * w.blocks * Hkv * ((int64_t)max_pages << p.pv.page_shift) > 0x7fffffff - (1 << 24))
+    return FPX_ERR_UNSUPPORTED;
   uint8_t *ws = static_cast<uint8_t *>(workspace);
-  p.prefix = reinterpret_cast<int64_t *>(ws);
+  p.prefix = reinterpret_cast<int *>(ws);
   p.part_ml = reinterpret_cast<float *>(ws + w.prefix);
   p.part_o = reinterpret_cast<float *>(ws + w.prefix + w.ml);
   if (format == FPX_PAGES_INT4) {

@@ -20,11 +20,12 @@ names nothing (a page outside the pool, a position past the table) is skipped, a
 
 from __future__ import annotations
 
+import functools
 from typing import Optional
 
 import torch
 
-from ._capi import FpxError, call, lib, ptr, stream
+from ._capi import FpxError, call, lib
 
 FORMATS = {"bf16": 0, "int4": 1}
 MAX_ROWS = 64  # query rows of a sequence in one paged_decode_attention
@@ -64,9 +65,9 @@ def _pool(pool: torch.Tensor):
     if pool.dim() != 4:
         raise FpxError("a pool is [pages, Hkv, page_size, row]")
     row = pool.shape[3]
-    if pool.dtype == torch.bfloat16:
+    if pool.dtype is torch.bfloat16:
         form, dim = 0, row // 2
-    elif pool.dtype == torch.uint8:
+    elif pool.dtype is torch.uint8:
         form, dim = 1, (row - 2) * 8 // 9
     else:
         raise TypeError("a pool is bfloat16, or uint8 in the 4-bit form")
@@ -80,70 +81,72 @@ def _pool(pool: torch.Tensor):
 def _where(pool, page_table, starts, counts, batch, kv_heads, head_dim):
     """Checks the tensors that say where rows lie; (format, arguments of the C calls)."""
     form, dim = _pool(pool)
-    if dim != head_dim or pool.shape[1] != kv_heads:
-        raise FpxError(f"the pool holds {pool.shape[1]} KV heads of {dim}, the call {kv_heads} of {head_dim}")
-    if page_table.dtype != torch.int32 or starts.dtype != torch.int32 or (counts is not None and counts.dtype != torch.int32):
+    pages, pool_heads, page_size, _ = pool.shape
+    if dim != head_dim or pool_heads != kv_heads:
+        raise FpxError(f"the pool holds {pool_heads} KV heads of {dim}, the call {kv_heads} of {head_dim}")
+    if page_table.dtype is not torch.int32 or starts.dtype is not torch.int32:
         raise TypeError("page_table, starts and counts must be int32")
     if page_table.dim() != 2 or page_table.shape[0] != batch or (page_table.shape[1] > 1 and page_table.stride(1) != 1):
         raise FpxError("page_table must be [B, max_pages] with contiguous rows")
-    for t in (starts, counts):
-        if t is not None and (t.shape != (batch,) or not t.is_contiguous()):
+    if starts.shape != (batch,) or not starts.is_contiguous():
+        raise FpxError("starts and counts must be [B], contiguous")
+    count_ptr = None
+    if counts is not None:
+        if counts.dtype is not torch.int32:
+            raise TypeError("page_table, starts and counts must be int32")
+        if counts.shape != (batch,) or not counts.is_contiguous():
             raise FpxError("starts and counts must be [B], contiguous")
-    stride = page_table.stride(0) if batch > 1 else page_table.shape[1]
-    return form, (ptr(pool), pool.shape[0], pool.shape[2], ptr(page_table), stride, page_table.shape[1], ptr(starts),
-                  ptr(counts))
+        count_ptr = counts.data_ptr()
+    max_pages = page_table.shape[1]
+    stride = page_table.stride(0) if batch > 1 else max_pages
+    return form, (pool.data_ptr(), pages, page_size, page_table.data_ptr(), stride, max_pages, starts.data_ptr(),
+                  count_ptr)
 
 
-def _device(*tensors):
+def _device(first, *tensors):
     """The tensors' common CUDA device."""
-    dev = None
+    dev = first.device
+    if dev.type != "cuda":
+        raise FpxError("fpx ops run on CUDA tensors only (there is no CPU path)")
     for t in tensors:
-        if t is None:
-            continue
-        if t.device.type != "cuda":
-            raise FpxError("fpx ops run on CUDA tensors only (there is no CPU path)")
-        if dev is not None and t.device != dev:
-            raise FpxError("all tensors of a call must be on one device")
-        dev = t.device
+        if t is not None and t.device != dev:
+            raise FpxError("all tensors of a call must be on one CUDA device")
     return dev
 
 
 def _call(dev, name, *args):
     """The C call on dev's current stream, with dev as the current device (its default stream has no
     device of its own to be bound to)."""
+    stream = torch._C._cuda_getCurrentRawStream(dev.index)
     if dev.index == torch.cuda.current_device():
-        call(name, *args, stream(dev))
+        call(name, *args, stream)
     else:
         with torch.cuda.device(dev):
-            call(name, *args, stream(dev))
+            call(name, *args, stream)
 
 
-def _bf16(*tensors):
-    for t in tensors:
-        if t is not None and t.dtype != torch.bfloat16:
-            raise TypeError("q, k, v and their outputs must be bfloat16")
-
-
-def _shape(t, shape, name):
-    if tuple(t.shape) != tuple(shape):
+def _rows(t, shape, name):
+    """(address, strides) of a bf16 tensor [B, L, heads, d] of the given shape."""
+    if t.dtype is not torch.bfloat16:
+        raise TypeError("q, k, v and their outputs must be bfloat16")
+    if t.shape != shape:
         raise FpxError(f"{name} must be {tuple(shape)}, is {tuple(t.shape)}")
-
-
-def _strides(t: torch.Tensor):
-    """Element strides of dims 0 .. 2; those of dims of one entry, which are never used, as 0."""
-    if t.stride(-1) != 1:
+    sb, sl, sh, sd = t.stride()
+    if sd != 1:
         raise FpxError("the last dimension must be contiguous")
-    return tuple(s if n > 1 else 0 for s, n in zip(t.stride()[:3], t.shape))
+    return t.data_ptr(), sb, sl, sh
 
 
 def _output(t, shape, name):
-    _shape(t, shape, name)
-    if any(s == 0 and n > 1 for s, n in zip(t.stride(), t.shape)):
+    rows = _rows(t, shape, name)
+    if 0 in rows[1:] and any(s == 0 and n > 1 for s, n in zip(rows[1:], shape)):
         raise FpxError(f"{name} must not be an expanded tensor")
-    return t
+    return rows
 
 
-@torch.no_grad()
+_NONE = (None, 0, 0, 0)
+
+
 def paged_append(k, v, pool, page_table, starts, counts=None, q=None, rope=None, q_out=None, k_out=None):
     """Stores new rows k, v [B, L, Hkv, d] bf16 in the pages, keys rotated by ``rope``.
 
@@ -155,64 +158,64 @@ def paged_append(k, v, pool, page_table, starts, counts=None, q=None, rope=None,
     Rotation is in fp32 and rounds once, to bf16 or to the 4-bit codes. Sequences of one call must not
     write the same page."""
     dev = _device(k, v, pool, page_table, starts, counts, q, rope, q_out, k_out)
-    _bf16(k, v, q, q_out, k_out)
-    if k.dim() != 4:
+    shape = k.shape
+    if len(shape) != 4:
         raise FpxError("k and v must be [B, L, Hkv, d]")
-    batch, length, kv_heads, dim = k.shape
-    _shape(v, k.shape, "v")
+    batch, length, kv_heads, dim = shape
+    k_rows, v_rows = _rows(k, shape, "k"), _rows(v, shape, "v")
     form, where = _where(pool, page_table, starts, counts, batch, kv_heads, dim)
-    rope_len = rotary = zero = 0
+    rope_len = rotary = zero = heads = 0
+    rope_ptr = None
     if rope is not None:
-        if rope.dtype != torch.float32 or rope.dim() != 2 or not rope.is_contiguous():
+        if rope.dtype is not torch.float32 or rope.dim() != 2 or not rope.is_contiguous():
             raise FpxError("rope must be a contiguous fp32 [positions, rotary] table")
         rope_len, rotary = rope.shape
+        rope_ptr = rope.data_ptr()
+    q_rows = qo_rows = ko_rows = _NONE
     if q is None:
         if q_out is not None:
             raise FpxError("q_out without q")
-        heads, q_args, o_args = 0, (None, 0, 0, 0), (None, 0, 0, 0)
     else:
         if q.dim() != 4:
             raise FpxError("q must be [B, L, H, d]")
         heads = q.shape[2]
-        _shape(q, (batch, length, heads, dim), "q")
+        q_rows = _rows(q, (batch, length, heads, dim), "q")
         if q_out is None:
-            zero, q_out = 1, torch.empty(q.shape, dtype=q.dtype, device=dev)
-        _output(q_out, q.shape, "q_out")
-        q_args, o_args = (ptr(q), *_strides(q)), (ptr(q_out), *_strides(q_out))
+            zero, q_out = 1, torch.empty_like(q, memory_format=torch.contiguous_format)
+        qo_rows = _output(q_out, q.shape, "q_out")
     if k_out is not None:
-        _output(k_out, k.shape, "k_out")
-    if batch == 0 or length == 0:
-        return q_out
-    ko_args = (None, 0, 0, 0) if k_out is None else (ptr(k_out), *_strides(k_out))
-    _call(dev, "fpx_paged_append", form, *q_args, ptr(k), *_strides(k), ptr(v), *_strides(v), batch, length, heads,
-          kv_heads, dim, ptr(rope), rope_len, rotary, *where, *o_args, *ko_args, zero)
+        ko_rows = _output(k_out, shape, "k_out")
+    if batch and length:
+        _call(dev, "fpx_paged_append", form, *q_rows, *k_rows, *v_rows, batch, length, heads, kv_heads, dim, rope_ptr,
+              rope_len, rotary, *where, *qo_rows, *ko_rows, zero)
     return q_out
 
 
-@torch.no_grad()
 def paged_gather(pool, page_table, starts, counts, length: int, k_out=None, v_out=None):
     """Rows back as bf16: (k, v) [B, length, Hkv, d], for a prefill over a cached prefix. Rows behind
     ``counts`` (None: every row counts) are left as they are in given outputs, and zero in new ones."""
-    _, dim = _pool(pool)
     dev = _device(pool, page_table, starts, counts, k_out, v_out)
+    _, dim = _pool(pool)
     batch, kv_heads = starts.shape[0], pool.shape[1]
     form, where = _where(pool, page_table, starts, counts, batch, kv_heads, dim)
-    _bf16(k_out, v_out)
     shape = (batch, length, kv_heads, dim)
     if (k_out is None) != (v_out is None):
         raise FpxError("give both of k_out and v_out, or neither")
     zero = int(k_out is None)
     if zero:
-        k_out, v_out = (torch.empty(shape, dtype=torch.bfloat16, device=dev) for _ in range(2))
-    _output(k_out, shape, "k_out")
-    _output(v_out, shape, "v_out")
+        k_out = torch.empty(shape, dtype=torch.bfloat16, device=dev)
+        v_out = torch.empty(shape, dtype=torch.bfloat16, device=dev)
+    k_rows, v_rows = _output(k_out, shape, "k_out"), _output(v_out, shape, "v_out")
     if batch and length:
-        _call(dev, "fpx_paged_gather", form, *where, batch, length, kv_heads, dim, ptr(k_out), *_strides(k_out),
-              ptr(v_out), *_strides(v_out), zero)
+        _call(dev, "fpx_paged_gather", form, *where, batch, length, kv_heads, dim, *k_rows, *v_rows, zero)
     return k_out, v_out
 
 
-@torch.no_grad()
+@functools.lru_cache(maxsize=256)
+def _workspace_bytes(form, batch, rows, heads, kv_heads, dim) -> int:
+    return int(lib().fpx_paged_decode_workspace_bytes(form, batch, rows, heads, kv_heads, dim))
+
+
 def paged_decode_attention(q, pool, page_table, starts, scale: float, counts=None, out=None, lse=None, ws=None):
     """Attention of q [B, Lq, H, d] bf16 to the cached tokens, causal by position: row i of sequence b
     sees positions 0 .. starts[b] + i, its own with them (append first). Returns bf16 [B, Lq, H, d]
@@ -223,31 +226,30 @@ def paged_decode_attention(q, pool, page_table, starts, scale: float, counts=Non
     ``paged_decode_workspace_bytes``; without it each call takes its own from torch's allocator, so calls on
     several streams or in several graphs share nothing."""
     dev = _device(q, pool, page_table, starts, counts, out, lse, ws)
-    _bf16(q, out)
-    if q.dim() != 4:
+    shape = q.shape
+    if len(shape) != 4:
         raise FpxError("q must be [B, Lq, H, d]")
-    batch, rows, heads, dim = q.shape
-    kv_heads = pool.shape[1]
+    batch, rows, heads, dim = shape
+    q_rows = _rows(q, shape, "q")
+    kv_heads = pool.shape[1] if pool.dim() == 4 else 0
     form, where = _where(pool, page_table, starts, counts, batch, kv_heads, dim)
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-    _output(out, q.shape, "out")
-    if lse is not None and (lse.dtype != torch.float32 or not lse.is_contiguous() or lse.shape != q.shape[:3]):
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    o_rows = _output(out, shape, "out")
+    if lse is not None and (lse.dtype is not torch.float32 or not lse.is_contiguous() or lse.shape != shape[:3]):
         raise FpxError("lse must be a contiguous fp32 [B, Lq, H]")
-    if batch == 0 or rows == 0:
-        return out
-    if ws is None:
-        ws = torch.empty(max(1, int(lib().fpx_paged_decode_workspace_bytes(form, batch, rows, heads, kv_heads, dim))),
-                         dtype=torch.uint8, device=dev)
-    _call(dev, "fpx_paged_decode_attention", form, ptr(q), *_strides(q), batch, rows, heads, kv_heads, dim,
-          float(scale), *where, ptr(out), *_strides(out), ptr(lse), ptr(ws), ws.numel())
+    if batch and rows:
+        if ws is None:
+            ws = torch.empty(_workspace_bytes(form, batch, rows, heads, kv_heads, dim), dtype=torch.uint8, device=dev)
+        _call(dev, "fpx_paged_decode_attention", form, *q_rows, batch, rows, heads, kv_heads, dim, scale, *where,
+              *o_rows, None if lse is None else lse.data_ptr(), ws.data_ptr(), ws.numel())
     return out
 
 
 def paged_decode_workspace_bytes(pool, batch: int, rows: int, heads: int) -> int:
     """Bytes of ``paged_decode_attention``'s workspace, whatever the sequences' lengths."""
     form, dim = _pool(pool)
-    return int(lib().fpx_paged_decode_workspace_bytes(form, batch, rows, heads, pool.shape[1], dim))
+    return _workspace_bytes(form, batch, rows, heads, pool.shape[1], dim)
 
 
 # The same calls as PyTorch custom ops, for torch.compile and fake tensors.

@@ -58,7 +58,7 @@ ODD = ctypes.c_void_p((1 << 20) + 2)
     (-1, dict(max_pages=0)), (-1, dict(q=None)), (-1, dict(q_out=None)), (-1, dict(H=0)), (-1, dict(rope_len=0)),
     (-3, dict(d=64)), (-3, dict(page_size=24)), (-3, dict(page_size=8)), (-3, dict(page_size=2048)),
     (-2, dict(stride=3)), (-2, dict(rotary=12)), (-2, dict(rotary=136)), (-2, dict(rotary=0)), (-2, dict(k=ODD)),
-    (-2, dict(ks=(0, 130, 128))), (-2, dict(vs=(0, 128, 2))), (-2, dict(qs=(0, 257, 128))), (-2, dict(qo=(1, 256, 128))),
+    (-2, dict(ks=(0, 130, 128))), (-2, dict(Hkv=2, vs=(0, 256, 2))), (-2, dict(qs=(0, 257, 128))), (-2, dict(B=2, qo=(1, 256, 128))),
     (-2, dict(k_out=ODD)), (-2, dict(k_out=A, ko=(0, 2, 128))), (-2, dict(pool=ctypes.c_void_p((1 << 20) + 8))),
     (-2, dict(rope=ctypes.c_void_p((1 << 20) + 4)))])
 def test_append_refuses(status, change):
@@ -94,7 +94,7 @@ def decode(**change):
 @pytest.mark.parametrize("status,change", [
     (-1, dict(q=None)), (-1, dict(out=None)), (-1, dict(Lq=0)), (-1, dict(format=3)), (-1, dict(pool=None)),
     (-1, dict(starts=None)), (-2, dict(H=3, Hkv=2)), (-3, dict(Lq=65)), (-3, dict(H=17)), (-3, dict(d=64)),
-    (-3, dict(B=1 << 24)), (-2, dict(qs=(0, 260, 128))), (-2, dict(q=ctypes.c_void_p((1 << 20) + 8))), (-5, dict(ws=None)),
+    (-3, dict(B=1 << 24)), (-2, dict(Lq=2, qs=(0, 260, 128))), (-2, dict(q=ctypes.c_void_p((1 << 20) + 8))), (-5, dict(ws=None)),
     (-5, dict(ws_bytes=1000)), (-5, dict(ws=ctypes.c_void_p((1 << 20) + 8)))])
 def test_decode_refuses(status, change):
     assert decode(**change) == status
