@@ -8,10 +8,10 @@
 // *columns* of both products, S^T = K Q^T and O^T = V^T P^T: keys are the 16 rows of
 // mma.sync's A operand, which 4-bit codes expand into straight from shared memory in the
 // layout paged.cuh describes, and 8 columns waste little for the usual groups of 4 to 8.
-//   K: a code n becomes the fp16 1024 + n or 1024 + 16 n by one and-or (0x6400 | n, in place), two
-//      pairs of codes a shift; the query's dims of the latter are divided by 16. The offsets are
-//      -1032 q and -72 q, taken out by a product of the groups' scales with sum(q) over the group,
-//      and the group's scale multiplies the group's sum.
+//   K: a nibble alone in a half, n or 16 n in place, is the fp16 number n 2^-24 or n 2^-20
+//      (subnormal, exact in the product): one mask a pair of codes, one shift for two pairs. The
+//      query's dims of the latter are divided by 16. The offset -8 sum(q) comes from one more
+//      product with the groups' scales, and a group's scale multiplies the group's sum.
 //   V: codes become the fp16 n - 8 (two logic operations and one exact fma a pair); the scales
 //      r < 2 multiply the probabilities, in fp16 (11 bits: its rounding stays below the bf16 of the
 //      output). The row exponent 2^e joins the logit: u = exp2(s + e - m) <= 2^8 whatever the
@@ -194,14 +194,14 @@ FPX_INLINE void follow(Columns<D, NT> &c, const float (&y)[GS][NT][4]) {
 
 // Query fragments of a unit (B operands of S^T = K Q^T), column n = lane / 4 of each tile.
 //
-// int4: a query row times a power of two that brings its largest element to 2^10 .. 2^11, in
-// fp16: exact but for elements 2^24 times smaller than that. The dims whose codes the product takes
+// int4: a query row times a power of two that brings its largest element to 2^14 .. 2^15, in
+// fp16: exact but for elements 2^20 times smaller than that. The dims whose codes the product takes
 // sixteenfold (the odd nibbles, in place) are divided by 16.
 template <int FMT, int D, int NT>
 struct Queries {
   uint32_t b[D / 16][NT][2];
-  // int4: what the codes' offsets add, -1032 or -72 times the query, summed over each group, as three bf16 terms: it
-  // multiplies the groups' scales in one more product of four groups x (high, middle, low) for every 128 dims
+  // int4: what the codes' offset adds, -8 times the query, summed over each group, as three bf16 terms: it multiplies
+  // the groups' scales in one more product of four groups x (high, middle, low) for every 128 dims
   uint32_t off[FMT == FPX_PAGES_INT4 ? D / 128 : 1][NT][2];
   float scale[NT][2];  // from S^T to log2 units, columns 2 t, 2 t + 1
 };
@@ -228,9 +228,9 @@ FPX_INLINE void load_queries(Queries<FMT, D, NT> &f, const PagedDecodeParams &p,
         for (uint32_t v : {w[j].x, w[j].y, w[j].z, w[j].w}) top = max(top, max((v << 16) & 0x7fff0000u, v & 0x7fff0000u));
       top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      const int up = top == 0 ? 0 : min(10 + 127 - (int)(top >> 23), 126);  // at least 10 - 128
+      const int up = top == 0 ? 0 : min(14 + 127 - (int)(top >> 23), 103);  // at least 14 - 128
       const float mul = __uint_as_float((uint32_t)(127 + up) << 23);
-      const float back = p.scale_log2 * __uint_as_float((uint32_t)(127 - max(up, -126)) << 23);
+      const float back = p.scale_log2 * __uint_as_float((uint32_t)(127 + 24 - up) << 23);  // codes stand for n 2^-24
       f.scale[n][0] = __shfl_sync(0xffffffffu, back, 8 * t);
       f.scale[n][1] = __shfl_sync(0xffffffffu, back, 8 * t + 4);
 #pragma unroll
@@ -251,10 +251,10 @@ FPX_INLINE void load_queries(Queries<FMT, D, NT> &f, const PagedDecodeParams &p,
           f.b[2 * j][n][1] = pack_f16(x[1] * 0.0625f, x[5] * 0.0625f);
           f.b[2 * j + 1][n][0] = pack_f16(x[2], x[6]);
           f.b[2 * j + 1][n][1] = pack_f16(x[3] * 0.0625f, x[7] * 0.0625f);
-          float s = -1032.f * ((x[0] + x[4]) + (x[2] + x[6])) - 72.f * ((x[1] + x[5]) + (x[3] + x[7]));
+          float s = ((x[0] + x[4]) + (x[2] + x[6])) + ((x[1] + x[5]) + (x[3] + x[7]));
           s += __shfl_xor_sync(0xffffffffu, s, 1);
           s += __shfl_xor_sync(0xffffffffu, s, 2);
-          sum[jj] = s;
+          sum[jj] = s * -0x1p-21f;  // -8 2^-24
         }
         // k = 2 t, 2 t + 1 of the product: groups 2 (t & 1), + 1; terms high (t < 2), middle; k + 8: low, none
         const float x0 = t & 1 ? sum[2] : sum[0], x1 = t & 1 ? sum[3] : sum[1];
@@ -308,10 +308,10 @@ FPX_INLINE void scores(float (&y)[NT][4], const Queries<FMT, D, NT> &f, uint32_t
       for (int n = 0; n < NT; ++n) mma_bf16(y[n], s4, f.off[J][n][0], f.off[J][n][1]);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const uint32_t lo = 0x000f000fu, hi = 0x00f000f0u, k = 0x64006400u;  // fp16 1024 + n, 1024 + 16 n
+        const uint32_t lo = 0x000f000fu, hi = 0x00f000f0u;
         const uint32_t va = wa[j] >> 8, vb = wb[j] >> 8;
-        const uint32_t a0[4] = {and_or(wa[j], lo, k), and_or(wb[j], lo, k), and_or(wa[j], hi, k), and_or(wb[j], hi, k)};
-        const uint32_t a1[4] = {and_or(va, lo, k), and_or(vb, lo, k), and_or(va, hi, k), and_or(vb, hi, k)};
+        const uint32_t a0[4] = {wa[j] & lo, wb[j] & lo, wa[j] & hi, wb[j] & hi};
+        const uint32_t a1[4] = {va & lo, vb & lo, va & hi, vb & hi};
         const uint32_t ua = j < 2 ? sa.x : sa.y, ub = j < 2 ? sb.x : sb.y;
         const float fa = __uint_as_float(j & 1 ? ua & 0xffff0000u : ua << 16);
         const float fb = __uint_as_float(j & 1 ? ub & 0xffff0000u : ub << 16);
