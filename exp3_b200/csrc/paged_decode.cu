@@ -108,6 +108,11 @@ FPX_INLINE uint32_t pack_f16(float lo, float hi) {
   __half2 v = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<uint32_t *>(&v);
 }
+FPX_INLINE float ex2_neg(float x) {  // 2^-x
+  float y;
+  asm("{\n\t.reg .f32 t;\n\tneg.f32 t, %1;\n\tex2.approx.ftz.f32 %0, t;\n\t}\n" : "=f"(y) : "f"(x));
+  return y;
+}
 // Loads from a shared-memory address (the granules arrive by bulk copies: ordered by the barrier's wait).
 FPX_INLINE uint4 lds128(uint32_t a) {
   uint4 v;
@@ -120,8 +125,8 @@ FPX_INLINE uint2 lds64(uint32_t a) {
   return v;
 }
 FPX_INLINE uint32_t lds16(uint32_t a) {
-  uint16_t v;
-  asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(a) : "memory");
+  uint32_t v;
+  asm volatile("ld.shared.u16 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
   return v;
 }
 FPX_INLINE void bulk_load(void *dst, const void *src, uint32_t bytes, uint64_t *bar) {
@@ -136,7 +141,7 @@ FPX_INLINE void bulk_load(void *dst, const void *src, uint32_t bytes, uint64_t *
 template <int FMT, int D, int NT, int GS, int W, int ST>
 struct PagedSmem {
   struct Merge {
-    float o[W][8 * NT][D];
+    float o[W][8 * NT][D + 4];  // rows 4 words apart in the banks: the lanes of a store then differ in theirs
     float m[W][8 * NT], l[W][8 * NT];
   };
   static constexpr bool kApart = FMT == FPX_PAGES_INT4;
@@ -430,13 +435,6 @@ FPX_INLINE void blank(uint32_t gran, int have, int lane) {
   }
 }
 
-// Dim of O^T row `row` (0 or 8 + g: the accumulator's two rows) of tile i: the V codes' layout
-// gives a lane four neighbouring dims over two tiles, ldmatrix the plain order.
-template <int FMT>
-FPX_INLINE int out_dim(int i, int g, int second) {
-  return FMT == FPX_PAGES_INT4 ? 16 * (i & ~1) + 4 * g + 2 * (i & 1) + second : 16 * i + 8 * second + g;
-}
-
 template <int FMT, int D, int NT, int GS, int W, int ST, int OCC>
 __global__ void __launch_bounds__(32 * W, OCC) paged_decode_kernel(const __grid_constant__ PagedDecodeParams p) {
   using G = Granule<FMT, D>;
@@ -531,44 +529,60 @@ __global__ void __launch_bounds__(32 * W, OCC) paged_decode_kernel(const __grid_
     g1 = min(n_steps, g0 + (hi - lo));
   };
 
-  // Ring: step g0 + warp + W i of the part goes into stage (issued mod ST).
-  uint32_t issued = 0, taken = 0, dead = 0;  // steps through this warp's ring; dead: GS bits a stage
-  int todo = 0, sent = 0, page = 0;
+  // Ring: step g0 + warp + W i of the part goes into the next stage. A lane works out where one of the
+  // next 32 steps lies (16 where each granule has a page of its own).
+  const bool paired = GS == 2 && p.pv.page_shift == 0;
+  int todo = 0, sent = 0, put = 0, get = 0;  // stages to fill and to read next
+  uint32_t phase = 0, dead = 0;              // a bit a stage: parity of its next wait; GS bits a stage: missing granules
+  uint32_t here = 0;                         // bit i: the page of lane i's granules exists
+  uint64_t source = 0;
   bool stopped = false;
   auto issue = [&]() {
-    const int32_t *table = p.pv.table + (int64_t)b * p.pv.table_stride;
-    const uint8_t *heads = p.pv.pool + (int64_t)kvh * p.pv.head_bytes;
-    const int last_page = (seen - 1) >> (p.pv.page_shift + 4);
-    const int first = GS * (g0 + warp + W * sent);  // granule
-    const int st = issued % ST;
-    uint64_t *bar = &sh.full[warp][st];
-    uint8_t *dst = ring_bytes + st * kBytes;
-    if (GS == 1 || p.pv.page_shift > 0) {  // all granules on one page
-      if ((sent & 31) == 0) page = table[min((GS * (g0 + warp + W * (sent + lane))) >> p.pv.page_shift, last_page)];
-      const int pg = __shfl_sync(0xffffffffu, page, sent & 31);
-      const bool ok = (unsigned)pg < (unsigned)p.pv.pages;
-      dead = (dead & ~(kAll << (GS * st))) | (ok ? 0u : kAll << (GS * st));
+    const int per_block = paired ? 16 : 32;
+    const int slot = sent & (per_block - 1);
+    if (slot == 0) {
+      const int step = g0 + warp + W * (sent + (paired ? lane >> 1 : lane));
+      const int granule = GS * step + (paired ? lane & 1 : 0);
+      const int last_page = (seen - 1) >> (p.pv.page_shift + 4);
+      const int at_page = granule >> p.pv.page_shift;
+      const int page = p.pv.table[(int64_t)b * p.pv.table_stride + min(at_page, last_page)];
+      const bool wanted = at_page <= last_page && step < g1, ok = (unsigned)page < (unsigned)p.pv.pages;
+      if (wanted && !ok) p.pv.fail();
+      here = __ballot_sync(0xffffffffu, wanted && ok);
+      source = reinterpret_cast<uint64_t>(p.pv.pool) + (int64_t)kvh * p.pv.head_bytes +
+               (int64_t)(ok ? page : 0) * p.pv.page_bytes + (granule & ((1 << p.pv.page_shift) - 1)) * G::kBytes;
+    }
+    const uint64_t src = __shfl_sync(0xffffffffu, source, paired ? 2 * slot : slot);
+    uint64_t *bar = &sh.full[warp][put];
+    uint8_t *dst = ring_bytes + put * kBytes;
+    dead &= ~(kAll << (GS * put));
+    if (!paired) {
+      if (!((here >> slot) & 1)) dead |= kAll << (GS * put);
       if (lane == 0) {
-        if (!ok) p.pv.fail();
         tc::mbar_expect_tx(bar, kBytes);
-        bulk_load(dst, heads + (int64_t)(ok ? pg : 0) * p.pv.page_bytes + (first & ((1 << p.pv.page_shift) - 1)) * G::kBytes,
-                  kBytes, bar);
+        bulk_load(dst, reinterpret_cast<const void *>(src), kBytes, bar);
       }
-    } else {  // a page each; the second granule of a sequence's last step may not exist
-      if ((sent & 15) == 0) page = table[min(2 * (g0 + warp + W * (sent + (lane >> 1))) + (lane & 1), last_page)];
-      const bool both = first + 1 <= last_page;
-      const int pa = __shfl_sync(0xffffffffu, page, 2 * (sent & 15)), pb = __shfl_sync(0xffffffffu, page, 2 * (sent & 15) + 1);
-      const bool oka = (unsigned)pa < (unsigned)p.pv.pages, okb = both && (unsigned)pb < (unsigned)p.pv.pages;
-      dead = (dead & ~(kAll << (GS * st))) | ((oka ? 0u : 1u) | (okb ? 0u : 2u)) << (GS * st);
+    } else {  // the second granule of a sequence's last step may not exist
+      const uint64_t src2 = __shfl_sync(0xffffffffu, source, 2 * slot + 1);
+      const uint32_t two = (here >> (2 * slot)) & 3u;
+      dead |= (two ^ 3u) << (GS * put);
       if (lane == 0) {
-        if (!oka || (both && !okb)) p.pv.fail();
-        tc::mbar_expect_tx(bar, (okb ? 2 : 1) * G::kBytes);
-        bulk_load(dst, heads + (int64_t)(oka ? pa : 0) * p.pv.page_bytes, G::kBytes, bar);
-        if (okb) bulk_load(dst + G::kBytes, heads + (int64_t)pb * p.pv.page_bytes, G::kBytes, bar);
+        tc::mbar_expect_tx(bar, two & 2 ? 2 * G::kBytes : G::kBytes);
+        bulk_load(dst, reinterpret_cast<const void *>(src), G::kBytes, bar);
+        if (two & 2) bulk_load(dst + G::kBytes, reinterpret_cast<const void *>(src2), G::kBytes, bar);
       }
     }
-    ++issued;
+    put = put + 1 == ST ? 0 : put + 1;
     ++sent;
+  };
+  auto arrived = [&](int stage) {  // the copy that was put there last
+    if (!tc::mbar_wait_warp(&sh.full[warp][stage], (phase >> stage) & 1, &sh.abort)) {
+      stopped = true;  // it did not arrive: report it and let the launch end
+      if (lane == 0 && p.pv.error) atomicMax(p.pv.error, FPX_DEVICE_WAIT);
+      return false;
+    }
+    phase ^= 1u << stage;
+    return true;
   };
   auto begin = [&]() {  // the part's first copy; the others follow once its queries are loaded, so that
     todo = g1 - g0 > warp ? (g1 - g0 - warp + W - 1) / W : 0;  // every warp's first is early in the queue
@@ -603,22 +617,12 @@ __global__ void __launch_bounds__(32 * W, OCC) paged_decode_kernel(const __grid_
     }
     // Software pipeline: the next step's scores share a block with this step's values, so that each
     // covers the other's latencies.
-    auto arrived = [&](uint32_t n) {  // the copy of step n of this ring
-      if (!stopped && !tc::mbar_wait_warp(&sh.full[warp][n % ST], (n / ST) & 1, &sh.abort)) {
-        stopped = true;  // it did not: report it and let the launch end
-        if (lane == 0 && p.pv.error) atomicMax(p.pv.error, FPX_DEVICE_WAIT);
-      }
-      return !stopped;
-    };
     float y[GS][NT][4];
-    if (todo > 0 && arrived(taken)) {
-#pragma unroll
-      for (int h = 0; h < GS; ++h) scores<FMT, D, NT>(y[h], f, ring + (taken % ST) * kBytes + h * G::kBytes, at, lane);
-    }
-    for (int i = 0; i < todo && !stopped; ++i) {
-      const uint32_t st = taken % ST, stage = ring + st * kBytes;
+    Weights<FMT, NT> pw[GS];
+    auto weigh = [&](int i) {  // from the scores of step i, which lies in stage `get`, to its probabilities
+      const uint32_t stage = ring + get * kBytes;
       const int key0 = (g0 + warp + W * i) * kStep;
-      const uint32_t gone = (dead >> (GS * st)) & kAll;
+      const uint32_t gone = (dead >> (GS * get)) & kAll;
       const bool edge = key0 + kStep > least || gone;
       if (edge) {
 #pragma unroll
@@ -633,10 +637,13 @@ __global__ void __launch_bounds__(32 * W, OCC) paged_decode_kernel(const __grid_
 #pragma unroll
       for (int h = 0; h < GS; ++h) {
         float e[2] = {0.f, 0.f};  // row exponents of the two keys' values
+        w[h][0] = w[h][1] = 1.f;
+        if (FMT == FPX_PAGES_INT4) {
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          if (FMT == FPX_PAGES_INT4) e[k] = __uint_as_float(lds16(stage + h * G::kBytes + at.ve + 16 * k) << 16);
-          w[h][k] = tc::ex2(-e[k]);
+          for (int k = 0; k < 2; ++k) {
+            e[k] = __uint_as_float(lds16(stage + h * G::kBytes + at.ve + 16 * k) << 16);
+            w[h][k] = ex2_neg(e[k]);
+          }
         }
 #pragma unroll
         for (int n = 0; n < NT; ++n)
@@ -653,7 +660,6 @@ __global__ void __launch_bounds__(32 * W, OCC) paged_decode_kernel(const __grid_
               if (((gone >> h) & 1) || key0 + kGranule * h + g + 8 * (k >> 1) >= limit[n][k & 1]) y[h][n][k] = -INFINITY;
       }
       follow<D, NT, GS>(c, y);
-      Weights<FMT, NT> pw[GS];
 #pragma unroll
       for (int h = 0; h < GS; ++h) {
 #pragma unroll
@@ -665,27 +671,37 @@ __global__ void __launch_bounds__(32 * W, OCC) paged_decode_kernel(const __grid_
         }
         transpose_weights<FMT, NT>(pw[h], y[h]);
       }
-      if (i + 1 < todo && arrived(taken + 1)) {
-        const uint32_t next = ring + ((taken + 1) % ST) * kBytes;
+    };
+    if (todo > 0 && !stopped && arrived(get)) {
+#pragma unroll
+      for (int h = 0; h < GS; ++h) scores<FMT, D, NT>(y[h], f, ring + get * kBytes + h * G::kBytes, at, lane);
+      for (int i = 0; i + 1 < todo; ++i) {
+        weigh(i);
+        const int after = get + 1 == ST ? 0 : get + 1;
+        if (!arrived(after)) break;
+        const uint32_t stage = ring + get * kBytes, next = ring + after * kBytes;
 #pragma unroll
         for (int h = 0; h < GS; ++h) {
           scores<FMT, D, NT>(y[h], f, next + h * G::kBytes, at, lane);
           values<FMT, D, NT>(c, pw[h], stage + h * G::kBytes, at, lane);
         }
-      } else {
-#pragma unroll
-        for (int h = 0; h < GS; ++h) values<FMT, D, NT>(c, pw[h], stage + h * G::kBytes, at, lane);
+        get = after;
+        if (sent < todo) {
+          __syncwarp();  // every lane has read the stage
+          issue();
+        }
       }
-      ++taken;
-      if (sent < todo && !stopped) {
-        __syncwarp();  // every lane has read the stage
-        issue();
+      if (!stopped) {
+        weigh(todo - 1);
+#pragma unroll
+        for (int h = 0; h < GS; ++h) values<FMT, D, NT>(c, pw[h], ring + get * kBytes + h * G::kBytes, at, lane);
+        get = get + 1 == ST ? 0 : get + 1;
       }
     }
     if (stopped)  // copies still in flight end before this memory is used again, or this long later
-      for (; taken < issued; ++taken) {
+      for (int st = 0; st < ST; ++st) {
         const long long from = clock64();
-        while (!tc::mbar_test(&sh.full[warp][taken % ST], (taken / ST) & 1) && clock64() - from < tc::kWaitCycles) {
+        while (!tc::mbar_test(&sh.full[warp][st], (phase >> st) & 1) && clock64() - from < tc::kWaitCycles / 8) {
         }
       }
 
@@ -719,10 +735,17 @@ __global__ void __launch_bounds__(32 * W, OCC) paged_decode_kernel(const __grid_
           merge.m[warp][col] = c.m[n][e];
           merge.l[warp][col] = c.l[n][e];
         }
+        if constexpr (FMT == FPX_PAGES_INT4) {  // the value codes' layout gives a lane four neighbouring dims over two tiles
 #pragma unroll
-        for (int i = 0; i < D / 16; ++i) {
-          merge.o[warp][col][out_dim<FMT>(i, g, 0)] = c.o[i][n][e];
-          merge.o[warp][col][out_dim<FMT>(i, g, 1)] = c.o[i][n][e + 2];
+          for (int i = 0; i < D / 16; i += 2)
+            *reinterpret_cast<float4 *>(&merge.o[warp][col][16 * i + 4 * g]) =
+                make_float4(c.o[i][n][e], c.o[i][n][e + 2], c.o[i + 1][n][e], c.o[i + 1][n][e + 2]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < D / 16; ++i) {
+            merge.o[warp][col][16 * i + g] = c.o[i][n][e];
+            merge.o[warp][col][16 * i + 8 + g] = c.o[i][n][e + 2];
+          }
         }
       }
     __syncthreads();
