@@ -65,6 +65,10 @@ FPX_INLINE int item_keys(const PagedDecodeParams &p, int start, int count, int r
 // A step is the GS granules of one ring stage.
 template <int GS>
 FPX_INLINE int steps_of(int keys) { return (keys + GS * kGranule - 1) / (GS * kGranule); }
+// What a unit counts in the partition: its steps and, in front of them, what beginning a unit costs a CTA
+// (queries, first copies, merge) in steps.
+constexpr int kPad = 4;
+FPX_INLINE int padded(int steps) { return steps ? steps + kPad : 0; }
 
 FPX_INLINE uint32_t and_or(uint32_t a, uint32_t b, uint32_t c) {
   uint32_t d;
@@ -459,7 +463,7 @@ __global__ void __launch_bounds__(32 * W, OCC) paged_decode_kernel(const __grid_
     const int b = i / p.blocks;
     int start, count;
     p.pv.rows(b, p.Lq, start, count);
-    return steps_of<GS>(item_keys<NT>(p, start, count, i - b * p.blocks)) * p.Hkv;
+    return padded(steps_of<GS>(item_keys<NT>(p, start, count, i - b * p.blocks))) * p.Hkv;
   };
   int mine = 0;
   for (int i = i0; i < i1; ++i) mine += steps_in(i);
@@ -508,25 +512,31 @@ __global__ void __launch_bounds__(32 * W, OCC) paged_decode_kernel(const __grid_
   uint8_t *const ring_bytes = sh.ring(warp);
   const uint32_t ring = smem_u32(ring_bytes);
 
-  // The part of a unit that this CTA works on: steps g0 .. g1 - 1 of n_steps.
+  // The part of a unit that this CTA works on: steps g0 .. g1 - 1 of n_steps. lo is its place in the partition.
   int item = sh.item, base = sh.base;
   int b, rb, kvh, start, rows, seen, n_steps, g0, g1;
-  auto find = [&]() {  // from step lo on, lo < hi
-    for (;;) {
-      b = item / p.blocks;
-      rb = item - b * p.blocks;
-      int count;
-      p.pv.rows(b, p.Lq, start, count);
-      rows = count * p.group;
-      seen = item_keys<NT>(p, start, count, rb);
-      n_steps = steps_of<GS>(seen);
-      if (lo - base < n_steps * p.Hkv) break;
-      base += n_steps * p.Hkv;
-      ++item;
+  auto find = [&]() {  // the next part from lo on; false: none is left
+    while (lo < hi) {
+      for (;;) {
+        b = item / p.blocks;
+        rb = item - b * p.blocks;
+        int count;
+        p.pv.rows(b, p.Lq, start, count);
+        rows = count * p.group;
+        seen = item_keys<NT>(p, start, count, rb);
+        n_steps = steps_of<GS>(seen);
+        if (lo - base < padded(n_steps) * p.Hkv) break;
+        base += padded(n_steps) * p.Hkv;
+        ++item;
+      }
+      kvh = (lo - base) / (n_steps + kPad);
+      const int first = base + kvh * (n_steps + kPad) + kPad;  // the unit's first step
+      g0 = max(0, lo - first);
+      g1 = min(n_steps, hi - first);
+      lo = first + max(g1, 0);  // hi, or the unit's end
+      if (g1 > g0) return true;
     }
-    kvh = (lo - base) / n_steps;
-    g0 = (lo - base) - kvh * n_steps;
-    g1 = min(n_steps, g0 + (hi - lo));
+    return false;
   };
 
   // Ring: step g0 + warp + W i of the part goes into the next stage. A lane works out where one of the
@@ -589,7 +599,7 @@ __global__ void __launch_bounds__(32 * W, OCC) paged_decode_kernel(const __grid_
     sent = 0;
     if (todo > 0 && !stopped) issue();
   };
-  find();
+  if (!find()) return;
   begin();
   for (;;) {
     const int row0 = rb * kRows;
@@ -717,9 +727,7 @@ __global__ void __launch_bounds__(32 * W, OCC) paged_decode_kernel(const __grid_
     const bool whole = g0 == 0 && g1 == n_steps;
     const int64_t slot = blockIdx.x + (int64_t)item * p.Hkv + kvh;
     const int mb = b, mkvh = kvh, mrows = rows;
-    lo += g1 - g0;
-    const bool more = lo < hi;
-    if (more) find();
+    const bool more = find();
     if (Smem::kApart) {
       if (more) begin();
     } else {
@@ -811,8 +819,8 @@ __global__ void __launch_bounds__(kMergeThreads) paged_merge_kernel(const __grid
     return;
   }
   const int per = max(p.min_steps, (total + p.ctas - 1) / p.ctas);
-  const int first = base + kvh * n;
-  const int c0 = first / per, c1 = (first + n - 1) / per;
+  const int first = base + kvh * n;  // padding, then steps
+  const int c0 = (first + kPad) / per, c1 = (first + n - 1) / per;
   if (c0 == c1) return;  // finished by its CTA
   const int64_t slot0 = c0 + (int64_t)item * p.Hkv + kvh;
   const int pieces = c1 - c0 + 1;
@@ -980,7 +988,7 @@ extern "C" int fpx_paged_decode_attention(int format, const void *q, int64_t q_s
   p.scale_log2 = (float)scale * kLog2e;
   p.ctas = w.ctas;
   // 32-bit counts of steps: what the table could name in all
-  if ((int64_t)B * w.blocks * Hkv * ((int64_t)max_pages << p.pv.page_shift) > 0x7fffffff - (1 << 24))
+  if ((int64_t)B * w.blocks * Hkv * (((int64_t)max_pages << p.pv.page_shift) + kPad) > 0x7fffffff - (1 << 24))
     return FPX_ERR_UNSUPPORTED;
   uint8_t *ws = static_cast<uint8_t *>(workspace);
   p.prefix = reinterpret_cast<int *>(ws);
