@@ -104,9 +104,24 @@ FPX_INLINE float max_nan(float a, float b) {
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
   return d;
 }
-// The four codes of x / s, low nibble first. A scale of zero gives the middle code, 0 * s; so does
-// one that is no number or infinite, whose 0 * s is NaN.
-FPX_INLINE uint32_t codes4(const float (&x)[4], float s) {
+// The four codes of x / s, low nibble first.
+//
+// quick: s is a normal number between 2^-100 and 2^100 whose relative rounding is at most 2^-8, so |x / s| rounds to 7
+// at most; `inv` is 1 / s correctly rounded. Then q = x inv, and q + (x - q s) inv is x / s correctly rounded
+// (Markstein's theorem on division by a rounded reciprocal; s has no mantissa of ones), at a third of a division's
+// instructions. Adding 1.5 * 2^23 + 8 rounds to the nearest even integer and leaves the code in the low bits.
+// Otherwise: a scale of zero gives the middle code, 0 * s; so does one that is no number or infinite, whose 0 * s is
+// NaN.
+FPX_INLINE uint32_t codes4(const float (&x)[4], float s, float inv, bool quick) {
+  if (quick) {
+    uint32_t n[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float q = __fmul_rn(x[e], inv);
+      n[e] = __float_as_uint(__fadd_rn(__fmaf_rn(__fmaf_rn(-q, s, x[e]), inv, q), 12582920.f));
+    }
+    return ((n[3] * 16 + n[2]) * 16 + n[1]) * 16 + n[0];  // the low 16 bits: 1.5 * 2^23's are zero
+  }
   uint32_t w = 0;
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
@@ -139,7 +154,8 @@ FPX_INLINE void write_int4(uint8_t *gran, int t, const float (&x)[D / 128][4], i
 #pragma unroll
     for (int J = 0; J < D / 128; ++J) {
       const __half r = __float2half_rn(a[J] * down);
-      const uint32_t w = codes4(x[J], __half2float(r) * up);
+      const float s = __half2float(r) * up;
+      const uint32_t w = codes4(x[J], s, __frcp_rn(s), s > 0x1p-100f && s < 0x1p100f && __half2float(r) >= 0x1p-14f);
       *reinterpret_cast<uint16_t *>(gran + G::kVCodes + v_chunk(t, J, lane & 7) + 2 * j) = (uint16_t)w;
       if ((lane & 7) == 0)
         *reinterpret_cast<__half *>(gran + G::kVScales + (((t >> 1) * (D / 32) + 4 * J + j) * 2 + (t & 1)) * 2) = r;
@@ -150,7 +166,8 @@ FPX_INLINE void write_int4(uint8_t *gran, int t, const float (&x)[D / 128][4], i
 #pragma unroll
     for (int J = 0; J < D / 128; ++J) {
       const __nv_bfloat16 s = __float2bfloat16_rn(a[J]);
-      const uint32_t w = codes4(x[J], __bfloat162float(s));
+      const float f = __bfloat162float(s);
+      const uint32_t w = codes4(x[J], f, __frcp_rn(f), f > 0x1p-100f && f < 0x1p100f);
       *reinterpret_cast<uint16_t *>(gran + t * (D / 2) + J * 64 + (4 * p + j) * 4 + (lane & 1) * 2) = (uint16_t)w;
       if ((lane & 7) == 0) *reinterpret_cast<__nv_bfloat16 *>(gran + G::kKScales + (t * (D / 32) + 4 * J + j) * 2) = s;
     }
@@ -185,62 +202,99 @@ FPX_INLINE uint8_t *granule_of(const PageView &pv, int b, int pos, int kvh, int 
          (int64_t)(g & ((1 << pv.page_shift) - 1)) * granule_bytes;
 }
 
-constexpr int kAppendHeads = 4;  // head rows of a warp, loaded before the first is used
+constexpr int kQueryHeads = 8;  // query heads of a warp
+constexpr int kStoreHeads = 4;  // rows of [k heads | v heads] of a warp
 
-// One warp: one token, kAppendHeads consecutive head rows of [q heads | k heads | v heads].
-template <int FMT, int D>
-__global__ void __launch_bounds__(128) paged_append_kernel(const __grid_constant__ AppendParams p) {
-  const int lane = threadIdx.x & 31;
-  const int64_t token = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-  if (token >= (int64_t)p.B * p.L) return;
-  const int b = (int)(token / p.L), l = (int)(token % p.L);
-  const int heads = p.H + 2 * p.Hkv, h0 = blockIdx.y * kAppendHeads;
-  const int64_t pos64 = (int64_t)p.pv.starts[b] + l;
-  const bool row = l < p.pv.count(b, p.L), past = pos64 > 0x7ffffffe || (p.rope && pos64 >= p.rope_len);
-  if (!row || past) {
-    if (row) p.pv.fail();
-    if (p.zero_padding) {
-      const float zero[D / 128][4] = {};
-      for (int h = h0; h < min(h0 + kAppendHeads, p.H + p.Hkv); ++h) {
-        if (h < p.H)
-          store_row<D>(p.q_out + b * p.qo_sb + l * p.qo_sl + h * p.qo_sh, zero, lane);
-        else if (p.k_out)
-          store_row<D>(p.k_out + b * p.ko_sb + l * p.ko_sl + (h - p.H) * p.ko_sh, zero, lane);
+// Queries: D / 8 lanes a head row. A lane holds four dims and the four that they rotate with (or eight that do not
+// rotate), so a rotation stays in the lane; the token's cosines and sines are loaded once for all of the warp's heads.
+template <int D>
+FPX_INLINE void append_queries(const AppendParams &p, int b, int l, int pos, int h0, bool live, int lane) {
+  constexpr int kLanes = D / 8, kRows = 32 / kLanes, kPasses = kQueryHeads / kRows;
+  const int u = lane % kLanes, sub = lane / kLanes, rotary = p.rope ? p.rotary : 0;
+  const bool turns = 8 * u < rotary;
+  const int d0 = turns ? 4 * u : 8 * u, d1 = turns ? 4 * u + rotary / 2 : 8 * u + 4;
+  const __nv_bfloat16 *src = p.q + b * p.q_sb + l * p.q_sl;
+  __nv_bfloat16 *dst = p.q_out + b * p.qo_sb + l * p.qo_sl;
+  uint2 x[kPasses], y[kPasses];
+  if (live) {
+#pragma unroll
+    for (int i = 0; i < kPasses; ++i) {
+      const int h = h0 + kRows * i + sub;
+      if (h < p.H) {
+        x[i] = *reinterpret_cast<const uint2 *>(src + h * p.q_sh + d0);
+        y[i] = *reinterpret_cast<const uint2 *>(src + h * p.q_sh + d1);
       }
     }
+  }
+  float c[4], s[4];
+  if (turns && live) {
+    const float *row = p.rope + (int64_t)pos * rotary;
+    const float4 cv = *reinterpret_cast<const float4 *>(row + 4 * u), sv = *reinterpret_cast<const float4 *>(row + rotary / 2 + 4 * u);
+    c[0] = cv.x; c[1] = cv.y; c[2] = cv.z; c[3] = cv.w;
+    s[0] = sv.x; s[1] = sv.y; s[2] = sv.z; s[3] = sv.w;
+  }
+  __syncwarp();  // q_out may be q: a lane stores only after every lane has loaded
+#pragma unroll
+  for (int i = 0; i < kPasses; ++i) {
+    const int h = h0 + kRows * i + sub;
+    if (h >= p.H) continue;
+    uint2 ox = make_uint2(0, 0), oy = ox;
+    if (live) {
+      ox = x[i];
+      oy = y[i];
+      if (turns) {  // each product and each sum rounded (no fused multiply-add), as rotate_row
+        const float a[4] = {__uint_as_float(ox.x << 16), __uint_as_float(ox.x & 0xffff0000u), __uint_as_float(ox.y << 16),
+                            __uint_as_float(ox.y & 0xffff0000u)};
+        const float z[4] = {__uint_as_float(oy.x << 16), __uint_as_float(oy.x & 0xffff0000u), __uint_as_float(oy.y << 16),
+                            __uint_as_float(oy.y & 0xffff0000u)};
+        float m[4], n[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          m[e] = __fsub_rn(__fmul_rn(a[e], c[e]), __fmul_rn(z[e], s[e]));
+          n[e] = __fadd_rn(__fmul_rn(z[e], c[e]), __fmul_rn(a[e], s[e]));
+        }
+        ox = make_uint2(pack_bf16(m[0], m[1]), pack_bf16(m[2], m[3]));
+        oy = make_uint2(pack_bf16(n[0], n[1]), pack_bf16(n[2], n[3]));
+      }
+    }
+    *reinterpret_cast<uint2 *>(dst + h * p.qo_sh + d0) = ox;
+    *reinterpret_cast<uint2 *>(dst + h * p.qo_sh + d1) = oy;
+  }
+}
+
+// Keys and values into their pages: a warp a head row.
+template <int FMT, int D>
+FPX_INLINE void append_rows(const AppendParams &p, int b, int l, int pos, int r0, bool live, int lane) {
+  const int last = min(r0 + kStoreHeads, 2 * p.Hkv);
+  if (!live) {
+    const float zero[D / 128][4] = {};
+    for (int r = r0; r < min(last, p.Hkv) && p.k_out; ++r)
+      store_row<D>(p.k_out + b * p.ko_sb + l * p.ko_sl + r * p.ko_sh, zero, lane);
     return;
   }
-  const int pos = (int)pos64;
-  HeadRow<D> rows[kAppendHeads];
+  HeadRow<D> rows[kStoreHeads];
 #pragma unroll
-  for (int u = 0; u < kAppendHeads; ++u) {
-    const int h = h0 + u;
-    if (h >= heads) break;
-    const __nv_bfloat16 *src = h < p.H ? p.q + b * p.q_sb + l * p.q_sl + h * p.q_sh
-                               : h < p.H + p.Hkv ? p.k + b * p.k_sb + l * p.k_sl + (h - p.H) * p.k_sh
-                                                 : p.v + b * p.v_sb + l * p.v_sl + (h - p.H - p.Hkv) * p.v_sh;
-    rows[u] = load_row<D>(src, lane);
+  for (int i = 0; i < kStoreHeads; ++i) {
+    const int r = r0 + i;
+    if (r >= last) break;
+    rows[i] = load_row<D>(r < p.Hkv ? p.k + b * p.k_sb + l * p.k_sl + r * p.k_sh
+                                    : p.v + b * p.v_sb + l * p.v_sl + (r - p.Hkv) * p.v_sh, lane);
   }
   Turn<D> turn{};
   const int rotary = p.rope ? p.rotary : 0;
-  if (p.rope && h0 < p.H + p.Hkv) turn = load_turn<D>(p.rope + (int64_t)pos * rotary, rotary, lane);
-  __syncwarp();  // q_out may be q, k_out may be k: a lane stores only after every lane has loaded
+  if (p.rope && r0 < p.Hkv) turn = load_turn<D>(p.rope + (int64_t)pos * rotary, rotary, lane);
+  __syncwarp();  // k_out may be k: a lane stores only after every lane has loaded
 #pragma unroll
-  for (int u = 0; u < kAppendHeads; ++u) {
-    const int h = h0 + u;
-    if (h >= heads) break;
+  for (int i = 0; i < kStoreHeads; ++i) {
+    const int r = r0 + i;
+    if (r >= last) break;
     float x[D / 128][4];
-    if (h < p.H) {
-      rotate_row<D>(rows[u], turn, rotary, lane, x);
-      store_row<D>(p.q_out + b * p.qo_sb + l * p.qo_sl + h * p.qo_sh, x, lane);
-      continue;
-    }
-    const bool value = h >= p.H + p.Hkv;
-    const int kvh = h - p.H - (value ? p.Hkv : 0);
+    const bool value = r >= p.Hkv;
+    const int kvh = value ? r - p.Hkv : r;
     if (value)
-      unpack_row<D>(rows[u], x);
+      unpack_row<D>(rows[i], x);
     else
-      rotate_row<D>(rows[u], turn, rotary, lane, x);
+      rotate_row<D>(rows[i], turn, rotary, lane, x);
     if (!value && p.k_out) store_row<D>(p.k_out + b * p.ko_sb + l * p.ko_sl + kvh * p.ko_sh, x, lane);
     uint8_t *gran = granule_of(p.pv, b, pos, kvh, Granule<FMT, D>::kBytes);
     if (!gran) continue;
@@ -259,6 +313,29 @@ __global__ void __launch_bounds__(128) paged_append_kernel(const __grid_constant
   }
 }
 
+// A warp a token: blocks of the grid's second dim below query_chunks take kQueryHeads query heads each, the others
+// kStoreHeads rows for the pages.
+template <int FMT, int D>
+__global__ void __launch_bounds__(128) paged_append_kernel(const __grid_constant__ AppendParams p, int query_chunks) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int lane = threadIdx.x & 31;
+  const int64_t token = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+  if (token >= (int64_t)p.B * p.L) return;
+  const int b = (int)(token / p.L), l = (int)(token % p.L);
+  int start, count;
+  p.pv.rows(b, p.L, start, count);
+  const int64_t pos = (int64_t)start + l;
+  const bool row = l < count, past = pos > 0x7ffffffe || (p.rope && pos >= p.rope_len);
+  if (row && past) p.pv.fail();
+  const bool live = row && !past;
+  if (!live && !p.zero_padding) return;
+  if ((int)blockIdx.y < query_chunks)
+    append_queries<D>(p, b, l, (int)pos, blockIdx.y * kQueryHeads, live, lane);
+  else
+    append_rows<FMT, D>(p, b, l, (int)pos, (blockIdx.y - query_chunks) * kStoreHeads, live, lane);
+}
+
 struct GatherParams {
   PageView pv;
   __nv_bfloat16 *k, *v;
@@ -267,51 +344,161 @@ struct GatherParams {
   bool zero_padding;
 };
 
-// One warp: one token and KV head.
-template <int FMT, int D>
-__global__ void __launch_bounds__(128) paged_gather_kernel(const __grid_constant__ GatherParams p) {
-  using G = Granule<FMT, D>;
-  const int lane = threadIdx.x & 31, kvh = blockIdx.y;
-  const int64_t token = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-  if (token >= (int64_t)p.B * p.L) return;
-  const int b = (int)(token / p.L), l = (int)(token % p.L);
-  const bool row = l < p.pv.count(b, p.L);
-  if (!row && !p.zero_padding) return;
-  const int pos = (int)min((int64_t)p.pv.starts[b] + l, (int64_t)0x7fffffff), t = pos & (kGranule - 1);
-  const uint8_t *gran = row ? granule_of(p.pv, b, pos, kvh, G::kBytes) : nullptr;
-  __nv_bfloat16 *ko = p.k + b * p.k_sb + l * p.k_sl + kvh * p.k_sh, *vo = p.v + b * p.v_sb + l * p.v_sl + kvh * p.v_sh;
-  float k[D / 128][4] = {}, v[D / 128][4] = {};
-  if (gran) {
-    if constexpr (FMT == FPX_PAGES_BF16) {
-      HeadRow<D> kr, vr;
+// Rows of one granule that a warp writes: row of token t is first + t. live: bit t: it comes from the page; zero: it
+// becomes zero.
+struct GatherRows {
+  __nv_bfloat16 *k, *v;  // of row `first`, which may lie before the output's first
+  int64_t k_sl, v_sl;
+  uint32_t live, zero;
+};
+FPX_INLINE void gather_store8(__nv_bfloat16 *dst, const float *x) {  // two or four pairs of neighbours
+  *reinterpret_cast<uint2 *>(dst) = make_uint2(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]));
+}
+
+// int4: a lane reads 16 bytes of codes: of keys, its parts of four groups of one token (eight dims each), of values, four dims of four groups
+// of a token pair. Quads and eights of lanes write 64 contiguous bytes.
+template <int D>
+FPX_INLINE void gather_int4(const GatherRows &o, const uint8_t *gran, int lane) {
+  using G = Granule<FPX_PAGES_INT4, D>;
+  const int g = lane >> 2, t = lane & 3;
 #pragma unroll
-      for (int J = 0; J < D / 128; ++J) {
-        const int at = t * G::kRow + (((16 * J + (lane >> 1)) ^ (t & 7)) << 4) + ((lane & 1) << 3);
-        kr.w[J] = *reinterpret_cast<const uint2 *>(gran + at);
-        vr.w[J] = *reinterpret_cast<const uint2 *>(gran + at + 2 * D);
+  for (int J = 0; J < D / 128; ++J)
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const int token = g + 8 * half;
+      const bool live = (o.live >> token) & 1;
+      if (!live && !((o.zero >> token) & 1)) continue;
+      uint4 w = make_uint4(0x88888888u, 0x88888888u, 0x88888888u, 0x88888888u);
+      uint2 sc = make_uint2(0, 0);
+      if (live) {
+        w = *reinterpret_cast<const uint4 *>(gran + token * (D / 2) + 64 * J + 16 * t);
+        sc = *reinterpret_cast<const uint2 *>(gran + G::kKScales + token * (D / 16) + 8 * J);
       }
-      unpack_row<D>(kr, k);
-      unpack_row<D>(vr, v);
-    } else {
-      const int j = lane >> 3, part = (lane & 7) >> 1;
-      const float e = __bfloat162float(*reinterpret_cast<const __nv_bfloat16 *>(gran + G::kVExps + 2 * t));
-      const float up = __uint_as_float((uint32_t)((int)e + 127) << 23);
+      const uint32_t words[4] = {w.x, w.y, w.z, w.w};
+      __nv_bfloat16 *dst = o.k + token * o.k_sl + 128 * J + 8 * t;
 #pragma unroll
-      for (int J = 0; J < D / 128; ++J) {
-        const uint32_t kc = *reinterpret_cast<const uint16_t *>(gran + t * (D / 2) + J * 64 + (4 * part + j) * 4 + (lane & 1) * 2);
-        const uint32_t vc = *reinterpret_cast<const uint16_t *>(gran + G::kVCodes + v_chunk(t, J, lane & 7) + 2 * j);
-        const float ks = __bfloat162float(*reinterpret_cast<const __nv_bfloat16 *>(gran + G::kKScales + (t * (D / 32) + 4 * J + j) * 2));
-        const float vs = __half2float(*reinterpret_cast<const __half *>(gran + G::kVScales + (((t >> 1) * (D / 32) + 4 * J + j) * 2 + (t & 1)) * 2)) * up;
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t u = j < 2 ? sc.x : sc.y;
+        const float s = __uint_as_float(j & 1 ? u & 0xffff0000u : u << 16);
+        float x[8];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          k[J][i] = (float)((int)((kc >> (4 * i)) & 15u) - 8) * ks;
-          v[J][i] = (float)((int)((vc >> (4 * i)) & 15u) - 8) * vs;
+        for (int i = 0; i < 8; ++i) x[i] = (float)((int)((words[j] >> (4 * i)) & 15u) - 8) * s;
+        gather_store8(dst + 32 * j, x);
+        gather_store8(dst + 32 * j + 4, x + 4);
+      }
+    }
+  const int vg = lane & 7;
+#pragma unroll
+  for (int J = 0; J < D / 128; ++J)
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const int q = (lane >> 3) + 4 * half;  // token pair
+      const uint32_t mine = 3u << (2 * q);
+      if (!((o.live | o.zero) & mine)) continue;
+      uint4 w = make_uint4(0x88888888u, 0x88888888u, 0x88888888u, 0x88888888u), sc = make_uint4(0, 0, 0, 0);
+      uint32_t e2 = 0;
+      if (o.live & mine) {
+        w = *reinterpret_cast<const uint4 *>(gran + G::kVCodes + v_chunk(2 * q, J, vg));
+        sc = *reinterpret_cast<const uint4 *>(gran + G::kVScales + q * (D / 8) + 16 * J);
+        e2 = *reinterpret_cast<const uint32_t *>(gran + G::kVExps + 4 * q);
+      }
+      const uint32_t scales[4] = {sc.x, sc.y, sc.z, sc.w};
+#pragma unroll
+      for (int odd = 0; odd < 2; ++odd) {
+        const int token = 2 * q + odd;
+        const bool live = (o.live >> token) & 1;
+        if (!live && !((o.zero >> token) & 1)) continue;
+        const float e = __uint_as_float(odd ? e2 & 0xffff0000u : e2 << 16);
+        const float up = __uint_as_float((uint32_t)((int)e + 127) << 23);
+        const uint32_t words[2] = {odd ? w.z : w.x, odd ? w.w : w.y};
+        __nv_bfloat16 *dst = o.v + token * o.v_sl + 128 * J + 4 * vg;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const __half2 r2 = *reinterpret_cast<const __half2 *>(&scales[j]);
+          const float s = live ? __half2float(odd ? __high2half(r2) : __low2half(r2)) * up : 0.f;
+          float x[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) x[i] = live ? (float)((int)((words[j >> 1] >> (16 * (j & 1) + 4 * i)) & 15u) - 8) * s : 0.f;
+          gather_store8(dst + 32 * j, x);
         }
       }
     }
+}
+
+// bf16: 16-byte chunks, unswizzled; the output's rows may be 8-byte aligned only.
+template <int D>
+FPX_INLINE void gather_bf16(const GatherRows &o, const uint8_t *gran, int lane) {
+  using G = Granule<FPX_PAGES_BF16, D>;
+  constexpr int kChunks = D / 8;  // of K, and of V
+#pragma unroll 4
+  for (int i = lane; i < kGranule * 2 * kChunks; i += 32) {
+    const int token = i / (2 * kChunks), c = i % kChunks;
+    const bool value = (i / kChunks) & 1, live = (o.live >> token) & 1;
+    if (!live && !((o.zero >> token) & 1)) continue;
+    uint4 w = make_uint4(0, 0, 0, 0);
+    if (live) w = *reinterpret_cast<const uint4 *>(gran + token * G::kRow + (value ? 2 * D : 0) + ((c ^ (token & 7)) << 4));
+    __nv_bfloat16 *dst = (value ? o.v + token * o.v_sl : o.k + token * o.k_sl) + 8 * c;
+    *reinterpret_cast<uint2 *>(dst) = make_uint2(w.x, w.y);
+    *reinterpret_cast<uint2 *>(dst + 4) = make_uint2(w.z, w.w);
   }
-  store_row<D>(ko, k, lane);
-  store_row<D>(vo, v, lane);
+}
+
+// A warp a granule of one sequence and KV head: its rows are those of the call whose positions lie in it.
+template <int FMT, int D>
+__global__ void __launch_bounds__(128) paged_gather_kernel(const __grid_constant__ GatherParams p, int granules) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int lane = threadIdx.x & 31, kvh = blockIdx.y;
+  const int64_t index = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+  if (index >= (int64_t)p.B * granules) return;
+  const int b = (int)(index / granules), i = (int)(index % granules);
+  int start, count;
+  p.pv.rows(b, p.L, start, count);
+  if (start < 0) start = 0;
+  const int64_t place = (int64_t)(start >> 4) + i;  // granule of the sequence
+  const int64_t first = (place << 4) - start;       // row of its first token
+  if (first >= p.L) return;
+  GatherRows o;
+  uint32_t live = 0, zero = 0;
+#pragma unroll
+  for (int t = 0; t < kGranule; ++t) {
+    const int64_t row = first + t;
+    if (row >= 0 && row < count) live |= 1u << t;
+    if (row >= count && row < p.L && p.zero_padding) zero |= 1u << t;
+  }
+  const uint8_t *gran = nullptr;
+  if (live) {
+    gran = granule_of(p.pv, b, (int)min(place << 4, (int64_t)0x7fffffff), kvh, Granule<FMT, D>::kBytes);
+    if (!gran) {  // reported; the rows read back as zero
+      zero |= live;
+      live = 0;
+    }
+  }
+  o.live = live;
+  o.zero = zero;
+  o.k_sl = p.k_sl;
+  o.v_sl = p.v_sl;
+  o.k = p.k + b * p.k_sb + first * p.k_sl + kvh * p.k_sh;
+  o.v = p.v + b * p.v_sb + first * p.v_sl + kvh * p.v_sh;
+  if constexpr (FMT == FPX_PAGES_INT4)
+    gather_int4<D>(o, gran, lane);
+  else
+    gather_bf16<D>(o, gran, lane);
+}
+
+// A launch that may begin while the kernel before it ends (each kernel here waits for it).
+template <class K, class... A>
+static int launch_dependent(K kernel, dim3 grid, cudaStream_t stream, A... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(128);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, args...) == cudaSuccess ? FPX_OK : FPX_ERR_CUDA;
 }
 
 int make_page_view(PageView *view, int format, const void *pool, int pages, int page_size, const int32_t *table,
@@ -382,22 +569,12 @@ extern "C" int fpx_paged_append(int format, const void *q, int64_t q_sb, int64_t
   p.rope = rope; p.rope_len = rope_len; p.rotary = rotary;
   p.B = B; p.L = L; p.H = H; p.Hkv = Hkv; p.zero_padding = zero_padding != 0;
   const int64_t blocks = ((int64_t)B * L + 3) / 4;
-  const int chunks = (H + 2 * Hkv + kAppendHeads - 1) / kAppendHeads;
+  const int query_chunks = (H + kQueryHeads - 1) / kQueryHeads, chunks = query_chunks + (2 * Hkv + kStoreHeads - 1) / kStoreHeads;
   if (blocks > 0x7fffffff || chunks > 65535) return FPX_ERR_SHAPE;
-  const dim3 grid((unsigned)blocks, chunks);
-  if (format == FPX_PAGES_INT4) {
-    if (d == 256)
-      paged_append_kernel<FPX_PAGES_INT4, 256><<<grid, 128, 0, stream>>>(p);
-    else
-      paged_append_kernel<FPX_PAGES_INT4, 128><<<grid, 128, 0, stream>>>(p);
-  } else {
-    if (d == 256)
-      paged_append_kernel<FPX_PAGES_BF16, 256><<<grid, 128, 0, stream>>>(p);
-    else
-      paged_append_kernel<FPX_PAGES_BF16, 128><<<grid, 128, 0, stream>>>(p);
-  }
-  FPX_CHECK_LAUNCH();
-  return FPX_OK;
+  const auto kernel = format == FPX_PAGES_INT4
+                          ? (d == 256 ? paged_append_kernel<FPX_PAGES_INT4, 256> : paged_append_kernel<FPX_PAGES_INT4, 128>)
+                          : (d == 256 ? paged_append_kernel<FPX_PAGES_BF16, 256> : paged_append_kernel<FPX_PAGES_BF16, 128>);
+  return launch_dependent(kernel, dim3((unsigned)blocks, chunks), stream, p, query_chunks);
 }
 
 extern "C" int fpx_paged_gather(int format, const void *pool, int pages, int page_size, const int32_t *table,
@@ -415,20 +592,11 @@ extern "C" int fpx_paged_gather(int format, const void *pool, int pages, int pag
   p.k = static_cast<__nv_bfloat16 *>(k); p.k_sb = ks.b; p.k_sl = ks.l; p.k_sh = ks.h;
   p.v = static_cast<__nv_bfloat16 *>(v); p.v_sb = vs.b; p.v_sl = vs.l; p.v_sh = vs.h;
   p.B = B; p.L = L; p.Hkv = Hkv; p.zero_padding = zero_padding != 0;
-  const int64_t blocks = ((int64_t)B * L + 3) / 4;
+  const int granules = L / kGranule + 2;  // that L rows can touch
+  const int64_t blocks = ((int64_t)B * granules + 3) / 4;
   if (blocks > 0x7fffffff || Hkv > 65535) return FPX_ERR_SHAPE;
-  const dim3 grid((unsigned)blocks, Hkv);
-  if (format == FPX_PAGES_INT4) {
-    if (d == 256)
-      paged_gather_kernel<FPX_PAGES_INT4, 256><<<grid, 128, 0, stream>>>(p);
-    else
-      paged_gather_kernel<FPX_PAGES_INT4, 128><<<grid, 128, 0, stream>>>(p);
-  } else {
-    if (d == 256)
-      paged_gather_kernel<FPX_PAGES_BF16, 256><<<grid, 128, 0, stream>>>(p);
-    else
-      paged_gather_kernel<FPX_PAGES_BF16, 128><<<grid, 128, 0, stream>>>(p);
-  }
-  FPX_CHECK_LAUNCH();
-  return FPX_OK;
+  const auto kernel = format == FPX_PAGES_INT4
+                          ? (d == 256 ? paged_gather_kernel<FPX_PAGES_INT4, 256> : paged_gather_kernel<FPX_PAGES_INT4, 128>)
+                          : (d == 256 ? paged_gather_kernel<FPX_PAGES_BF16, 256> : paged_gather_kernel<FPX_PAGES_BF16, 128>);
+  return launch_dependent(kernel, dim3((unsigned)blocks, Hkv), stream, p, granules);
 }
