@@ -99,6 +99,13 @@ FPX_INLINE void rotate_row(const HeadRow<D> &r, const Turn<D> &t, int rotary, in
   }
 }
 
+// m / 7 correctly rounded, by the quick division of codes4 where nothing under- or overflows.
+FPX_INLINE float seventh(float m) {
+  if (!(m > 0x1p-100f && m < 0x1p100f)) return __fdiv_rn(m, 7.f);
+  constexpr float kInv = 1.f / 7.f;
+  const float q = __fmul_rn(m, kInv);
+  return __fmaf_rn(__fmaf_rn(-q, 7.f, m), kInv, q);
+}
 FPX_INLINE float max_nan(float a, float b) {
   float d;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
@@ -143,7 +150,7 @@ FPX_INLINE void write_int4(uint8_t *gran, int t, const float (&x)[D / 128][4], i
     float m = max_nan(max_nan(fabsf(x[J][0]), fabsf(x[J][1])), max_nan(fabsf(x[J][2]), fabsf(x[J][3])));
 #pragma unroll
     for (int o = 1; o < 8; o <<= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
-    a[J] = __fdiv_rn(m, 7.f);
+    a[J] = seventh(m);
     top = max_nan(top, a[J]);
   }
   if (VALUE) {
@@ -202,14 +209,15 @@ FPX_INLINE uint8_t *granule_of(const PageView &pv, int b, int pos, int kvh, int 
          (int64_t)(g & ((1 << pv.page_shift) - 1)) * granule_bytes;
 }
 
-constexpr int kQueryHeads = 8;  // query heads of a warp
-constexpr int kStoreHeads = 4;  // rows of [k heads | v heads] of a warp
+constexpr int kPasses = 8;                                     // of a warp over query heads
+constexpr int query_heads(int d) { return kPasses * 32 / (d / 8); }
+constexpr int kStoreRows = 8;                                  // rows of [k heads | v heads] of a warp
 
 // Queries: D / 8 lanes a head row. A lane holds four dims and the four that they rotate with (or eight that do not
 // rotate), so a rotation stays in the lane; the token's cosines and sines are loaded once for all of the warp's heads.
 template <int D>
 FPX_INLINE void append_queries(const AppendParams &p, int b, int l, int pos, int h0, bool live, int lane) {
-  constexpr int kLanes = D / 8, kRows = 32 / kLanes, kPasses = kQueryHeads / kRows;
+  constexpr int kLanes = D / 8, kRows = 32 / kLanes;
   const int u = lane % kLanes, sub = lane / kLanes, rotary = p.rope ? p.rotary : 0;
   const bool turns = 8 * u < rotary;
   const int d0 = turns ? 4 * u : 8 * u, d1 = turns ? 4 * u + rotary / 2 : 8 * u + 4;
@@ -262,30 +270,144 @@ FPX_INLINE void append_queries(const AppendParams &p, int b, int l, int pos, int
   }
 }
 
-// Keys and values into their pages: a warp a head row.
+// Keys and values into their pages, where the whole head or nothing of it rotates: D / 16 lanes a row. A lane holds
+// dims 8 u .. + 7 and 8 u + d / 2 .. + 7, which rotate with each other; four lanes hold a group of 32.
 template <int FMT, int D>
-FPX_INLINE void append_rows(const AppendParams &p, int b, int l, int pos, int r0, bool live, int lane) {
-  const int last = min(r0 + kStoreHeads, 2 * p.Hkv);
-  if (!live) {
-    const float zero[D / 128][4] = {};
-    for (int r = r0; r < min(last, p.Hkv) && p.k_out; ++r)
-      store_row<D>(p.k_out + b * p.ko_sb + l * p.ko_sl + r * p.ko_sh, zero, lane);
-    return;
-  }
-  HeadRow<D> rows[kStoreHeads];
+FPX_INLINE void append_rows(const AppendParams &p, int b, int l, int pos, uint8_t *gran, int r0, int lane) {
+  constexpr int kLanes = D / 16, kRows = 32 / kLanes;
+  const int u = lane % kLanes, last = min(r0 + kStoreRows, 2 * p.Hkv), t = pos & (kGranule - 1);
+  uint4 w[kStoreRows / kRows][2];
 #pragma unroll
-  for (int i = 0; i < kStoreHeads; ++i) {
-    const int r = r0 + i;
-    if (r >= last) break;
-    rows[i] = load_row<D>(r < p.Hkv ? p.k + b * p.k_sb + l * p.k_sl + r * p.k_sh
-                                    : p.v + b * p.v_sb + l * p.v_sl + (r - p.Hkv) * p.v_sh, lane);
+  for (int i = 0; i < kStoreRows / kRows; ++i) {
+    const int r = r0 + kRows * i + lane / kLanes;
+    w[i][0] = w[i][1] = make_uint4(0, 0, 0, 0);
+    if (r >= last) continue;
+    const __nv_bfloat16 *src = r < p.Hkv ? p.k + b * p.k_sb + l * p.k_sl + r * p.k_sh
+                                         : p.v + b * p.v_sb + l * p.v_sl + (r - p.Hkv) * p.v_sh;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {  // head rows are 8-byte aligned
+      const uint2 lo = *reinterpret_cast<const uint2 *>(src + 8 * u + h * (D / 2));
+      const uint2 hi = *reinterpret_cast<const uint2 *>(src + 8 * u + h * (D / 2) + 4);
+      w[i][h] = make_uint4(lo.x, lo.y, hi.x, hi.y);
+    }
   }
-  Turn<D> turn{};
-  const int rotary = p.rope ? p.rotary : 0;
-  if (p.rope && r0 < p.Hkv) turn = load_turn<D>(p.rope + (int64_t)pos * rotary, rotary, lane);
+  float c[8], s[8];
+  if (p.rope && r0 < p.Hkv) {
+    const float4 *row = reinterpret_cast<const float4 *>(p.rope + (int64_t)pos * D + 8 * u);
+    const float4 v[4] = {row[0], row[1], row[D / 8], row[D / 8 + 1]};
+    c[0] = v[0].x; c[1] = v[0].y; c[2] = v[0].z; c[3] = v[0].w; c[4] = v[1].x; c[5] = v[1].y; c[6] = v[1].z; c[7] = v[1].w;
+    s[0] = v[2].x; s[1] = v[2].y; s[2] = v[2].z; s[3] = v[2].w; s[4] = v[3].x; s[5] = v[3].y; s[6] = v[3].z; s[7] = v[3].w;
+  }
   __syncwarp();  // k_out may be k: a lane stores only after every lane has loaded
 #pragma unroll
-  for (int i = 0; i < kStoreHeads; ++i) {
+  for (int i = 0; i < kStoreRows / kRows; ++i) {
+    if (r0 + kRows * i >= last) break;
+    const int r = r0 + kRows * i + lane / kLanes;
+    const bool value = r >= p.Hkv, mine = r < last;
+    const int kvh = value ? r - p.Hkv : r;
+    float x[2][8];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const uint32_t v[4] = {w[i][h].x, w[i][h].y, w[i][h].z, w[i][h].w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        x[h][2 * e] = __uint_as_float(v[e] << 16);
+        x[h][2 * e + 1] = __uint_as_float(v[e] & 0xffff0000u);
+      }
+    }
+    if (!value && mine) {
+      if (p.rope) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {  // as rotate_row
+          const float a = x[0][e], z = x[1][e];
+          x[0][e] = __fsub_rn(__fmul_rn(a, c[e]), __fmul_rn(z, s[e]));
+          x[1][e] = __fadd_rn(__fmul_rn(z, c[e]), __fmul_rn(a, s[e]));
+        }
+      }
+    }
+    if (FMT == FPX_PAGES_BF16 || (!value && p.k_out)) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        w[i][h] = make_uint4(pack_bf16(x[h][0], x[h][1]), pack_bf16(x[h][2], x[h][3]), pack_bf16(x[h][4], x[h][5]),
+                             pack_bf16(x[h][6], x[h][7]));
+      if (!value && p.k_out && mine) {
+        __nv_bfloat16 *dst = p.k_out + b * p.ko_sb + l * p.ko_sl + kvh * p.ko_sh + 8 * u;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          *reinterpret_cast<uint2 *>(dst + h * (D / 2)) = make_uint2(w[i][h].x, w[i][h].y);
+          *reinterpret_cast<uint2 *>(dst + h * (D / 2) + 4) = make_uint2(w[i][h].z, w[i][h].w);
+        }
+      }
+    }
+    uint8_t *page = gran + (int64_t)kvh * p.pv.head_bytes;
+    if constexpr (FMT == FPX_PAGES_BF16) {
+      if (mine && gran) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          *reinterpret_cast<uint4 *>(page + t * Granule<FMT, D>::kRow + (value ? 2 * D : 0) + (((u + h * (D / 16)) ^ (t & 7)) << 4)) =
+              w[i][h];
+      }
+    } else {
+      using G = Granule<FPX_PAGES_INT4, D>;
+      float a[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float m = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) m = max_nan(m, fabsf(x[h][e]));
+        m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, 1));
+        m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, 2));
+        a[h] = seventh(m);
+      }
+      float top = max_nan(a[0], a[1]);
+#pragma unroll
+      for (int o = 4; o < kLanes; o <<= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
+      const int e = min(max((int)((__float_as_uint(top) >> 23) & 255u) - 127, -60), 126);
+      const float up = __uint_as_float((uint32_t)(e + 127) << 23), down = __uint_as_float((uint32_t)(127 - e) << 23);
+      if (!mine || !gran) continue;  // no lane of the warp waits for another below
+      const int part = u & 3;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int dim = 8 * u + h * (D / 2), J = dim >> 7, j = (dim & 127) >> 5;
+        const __half r16 = __float2half_rn(a[h] * down);
+        const __nv_bfloat16 b16 = __float2bfloat16_rn(a[h]);
+        const float sc = value ? __half2float(r16) * up : __bfloat162float(b16);
+        const bool quick = sc > 0x1p-100f && sc < 0x1p100f && (!value || __half2float(r16) >= 0x1p-14f);
+        const float inv = __frcp_rn(sc);
+        const uint32_t lo = codes4({x[h][0], x[h][1], x[h][2], x[h][3]}, sc, inv, quick);
+        const uint32_t hi = codes4({x[h][4], x[h][5], x[h][6], x[h][7]}, sc, inv, quick);
+        if (value) {
+          *reinterpret_cast<uint16_t *>(page + G::kVCodes + v_chunk(t, J, 2 * part) + 2 * j) = (uint16_t)lo;
+          *reinterpret_cast<uint16_t *>(page + G::kVCodes + v_chunk(t, J, 2 * part + 1) + 2 * j) = (uint16_t)hi;
+          if (part == 0)
+            *reinterpret_cast<__half *>(page + G::kVScales + (((t >> 1) * (D / 32) + 4 * J + j) * 2 + (t & 1)) * 2) = r16;
+        } else {
+          *reinterpret_cast<uint32_t *>(page + t * (D / 2) + J * 64 + (4 * part + j) * 4) = __byte_perm(lo, hi, 0x5410);
+          if (part == 0) *reinterpret_cast<__nv_bfloat16 *>(page + G::kKScales + (t * (D / 32) + 4 * J + j) * 2) = b16;
+        }
+      }
+      if (value && u == 0) *reinterpret_cast<__nv_bfloat16 *>(page + G::kVExps + 2 * t) = __float2bfloat16_rn((float)e);
+    }
+  }
+}
+
+// The same where a part of the head rotates: a warp a row, four dims a lane.
+template <int FMT, int D>
+FPX_INLINE void append_rows_partly(const AppendParams &p, int b, int l, int pos, uint8_t *gran, int r0, int lane) {
+  const int last = min(r0 + kStoreRows, 2 * p.Hkv), t = pos & (kGranule - 1);
+  Turn<D> turn{};
+  if (r0 < p.Hkv) turn = load_turn<D>(p.rope + (int64_t)pos * p.rotary, p.rotary, lane);
+  HeadRow<D> rows[kStoreRows];
+#pragma unroll
+  for (int i = 0; i < kStoreRows; ++i) {
+    const int r = r0 + i;
+    if (r >= last) break;
+    rows[i] = load_row<D>(r >= p.Hkv ? p.v + b * p.v_sb + l * p.v_sl + (r - p.Hkv) * p.v_sh
+                                     : p.k + b * p.k_sb + l * p.k_sl + r * p.k_sh, lane);
+  }
+  __syncwarp();  // k_out may be k: a lane stores only after every lane has loaded
+#pragma unroll
+  for (int i = 0; i < kStoreRows; ++i) {
     const int r = r0 + i;
     if (r >= last) break;
     float x[D / 128][4];
@@ -294,46 +416,58 @@ FPX_INLINE void append_rows(const AppendParams &p, int b, int l, int pos, int r0
     if (value)
       unpack_row<D>(rows[i], x);
     else
-      rotate_row<D>(rows[i], turn, rotary, lane, x);
+      rotate_row<D>(rows[i], turn, p.rotary, lane, x);
     if (!value && p.k_out) store_row<D>(p.k_out + b * p.ko_sb + l * p.ko_sl + kvh * p.ko_sh, x, lane);
-    uint8_t *gran = granule_of(p.pv, b, pos, kvh, Granule<FMT, D>::kBytes);
     if (!gran) continue;
-    const int t = pos & (kGranule - 1);
+    uint8_t *page = gran + (int64_t)kvh * p.pv.head_bytes;
     if (FMT == FPX_PAGES_INT4) {
       if (value)
-        write_int4<D, true>(gran, t, x, lane);
+        write_int4<D, true>(page, t, x, lane);
       else
-        write_int4<D, false>(gran, t, x, lane);
+        write_int4<D, false>(page, t, x, lane);
     } else {
       if (value)
-        write_bf16<D, true>(gran, t, x, lane);
+        write_bf16<D, true>(page, t, x, lane);
       else
-        write_bf16<D, false>(gran, t, x, lane);
+        write_bf16<D, false>(page, t, x, lane);
     }
   }
 }
 
-// A warp a token: blocks of the grid's second dim below query_chunks take kQueryHeads query heads each, the others
-// kStoreHeads rows for the pages.
+// A warp a token: blocks of the grid's second dim below query_chunks take query_heads(D) query heads each, the others
+// kStoreRows rows for the pages.
 template <int FMT, int D>
 __global__ void __launch_bounds__(128) paged_append_kernel(const __grid_constant__ AppendParams p, int query_chunks) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int lane = threadIdx.x & 31;
-  const int64_t token = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-  if (token >= (int64_t)p.B * p.L) return;
-  const int b = (int)(token / p.L), l = (int)(token % p.L);
+  const uint32_t token = blockIdx.x * 4 + (threadIdx.x >> 5);
+  if (token >= (uint32_t)p.B * (uint32_t)p.L) return;
+  const int b = (int)(token / (uint32_t)p.L), l = (int)(token - (uint32_t)b * p.L);
   int start, count;
   p.pv.rows(b, p.L, start, count);
-  const int64_t pos = (int64_t)start + l;
-  const bool row = l < count, past = pos > 0x7ffffffe || (p.rope && pos >= p.rope_len);
+  const int64_t pos64 = (int64_t)start + l;
+  const bool row = l < count, past = pos64 > 0x7ffffffe || (p.rope && pos64 >= p.rope_len);
   if (row && past) p.pv.fail();
   const bool live = row && !past;
   if (!live && !p.zero_padding) return;
-  if ((int)blockIdx.y < query_chunks)
-    append_queries<D>(p, b, l, (int)pos, blockIdx.y * kQueryHeads, live, lane);
+  const int pos = (int)pos64;
+  if ((int)blockIdx.y < query_chunks) {
+    append_queries<D>(p, b, l, pos, blockIdx.y * query_heads(D), live, lane);
+    return;
+  }
+  const int r0 = (blockIdx.y - query_chunks) * kStoreRows;
+  if (!live) {
+    const float zero[D / 128][4] = {};
+    for (int r = r0; r < min(r0 + kStoreRows, p.Hkv) && p.k_out; ++r)
+      store_row<D>(p.k_out + b * p.ko_sb + l * p.ko_sl + r * p.ko_sh, zero, lane);
+    return;
+  }
+  uint8_t *gran = granule_of(p.pv, b, pos, 0, Granule<FMT, D>::kBytes);
+  if (!p.rope || p.rotary == D)
+    append_rows<FMT, D>(p, b, l, pos, gran, r0, lane);
   else
-    append_rows<FMT, D>(p, b, l, (int)pos, (blockIdx.y - query_chunks) * kStoreHeads, live, lane);
+    append_rows_partly<FMT, D>(p, b, l, pos, gran, r0, lane);
 }
 
 struct GatherParams {
@@ -341,7 +475,7 @@ struct GatherParams {
   __nv_bfloat16 *k, *v;
   int64_t k_sb, k_sl, k_sh, v_sb, v_sl, v_sh;
   int B, L, Hkv;
-  bool zero_padding;
+  bool zero_padding, wide;
 };
 
 // Rows of one granule that a warp writes: row of token t is first + t. live: bit t: it comes from the page; zero: it
@@ -350,9 +484,15 @@ struct GatherRows {
   __nv_bfloat16 *k, *v;  // of row `first`, which may lie before the output's first
   int64_t k_sl, v_sl;
   uint32_t live, zero;
+  bool wide;  // the output's rows are 16-byte aligned
 };
-FPX_INLINE void gather_store8(__nv_bfloat16 *dst, const float *x) {  // two or four pairs of neighbours
-  *reinterpret_cast<uint2 *>(dst) = make_uint2(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]));
+FPX_INLINE void gather_store(const GatherRows &o, __nv_bfloat16 *dst, uint4 v) {  // eight dims
+  if (o.wide) {
+    *reinterpret_cast<uint4 *>(dst) = v;
+  } else {
+    *reinterpret_cast<uint2 *>(dst) = make_uint2(v.x, v.y);
+    *reinterpret_cast<uint2 *>(dst + 4) = make_uint2(v.z, v.w);
+  }
 }
 
 // int4: a lane reads 16 bytes of codes: of keys, its parts of four groups of one token (eight dims each), of values, four dims of four groups
@@ -383,8 +523,7 @@ FPX_INLINE void gather_int4(const GatherRows &o, const uint8_t *gran, int lane) 
         float x[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) x[i] = (float)((int)((words[j] >> (4 * i)) & 15u) - 8) * s;
-        gather_store8(dst + 32 * j, x);
-        gather_store8(dst + 32 * j + 4, x + 4);
+        gather_store(o, dst + 32 * j, make_uint4(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7])));
       }
     }
   const int vg = lane & 7;
@@ -419,27 +558,33 @@ FPX_INLINE void gather_int4(const GatherRows &o, const uint8_t *gran, int lane) 
           float x[4];
 #pragma unroll
           for (int i = 0; i < 4; ++i) x[i] = live ? (float)((int)((words[j >> 1] >> (16 * (j & 1) + 4 * i)) & 15u) - 8) * s : 0.f;
-          gather_store8(dst + 32 * j, x);
+          *reinterpret_cast<uint2 *>(dst + 32 * j) = make_uint2(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]));
         }
       }
     }
 }
 
-// bf16: 16-byte chunks, unswizzled; the output's rows may be 8-byte aligned only.
+// bf16: 16-byte chunks, unswizzled.
 template <int D>
 FPX_INLINE void gather_bf16(const GatherRows &o, const uint8_t *gran, int lane) {
   using G = Granule<FPX_PAGES_BF16, D>;
   constexpr int kChunks = D / 8;  // of K, and of V
-#pragma unroll 4
-  for (int i = lane; i < kGranule * 2 * kChunks; i += 32) {
-    const int token = i / (2 * kChunks), c = i % kChunks;
-    const bool value = (i / kChunks) & 1, live = (o.live >> token) & 1;
-    if (!live && !((o.zero >> token) & 1)) continue;
-    uint4 w = make_uint4(0, 0, 0, 0);
-    if (live) w = *reinterpret_cast<const uint4 *>(gran + token * G::kRow + (value ? 2 * D : 0) + ((c ^ (token & 7)) << 4));
-    __nv_bfloat16 *dst = (value ? o.v + token * o.v_sl : o.k + token * o.k_sl) + 8 * c;
-    *reinterpret_cast<uint2 *>(dst) = make_uint2(w.x, w.y);
-    *reinterpret_cast<uint2 *>(dst + 4) = make_uint2(w.z, w.w);
+  constexpr int kAhead = 8;  // loads in flight
+  for (int i0 = lane; i0 < kGranule * 2 * kChunks; i0 += 32 * kAhead) {
+    uint4 w[kAhead];
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      const int i = i0 + 32 * k, token = i / (2 * kChunks), c = i % kChunks;
+      w[k] = make_uint4(0, 0, 0, 0);
+      if ((o.live >> token) & 1)
+        w[k] = *reinterpret_cast<const uint4 *>(gran + token * G::kRow + ((i / kChunks) & 1 ? 2 * D : 0) + ((c ^ (token & 7)) << 4));
+    }
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      const int i = i0 + 32 * k, token = i / (2 * kChunks), c = i % kChunks;
+      if (((o.live | o.zero) >> token) & 1)
+        gather_store(o, ((i / kChunks) & 1 ? o.v + token * o.v_sl : o.k + token * o.k_sl) + 8 * c, w[k]);
+    }
   }
 }
 
@@ -474,6 +619,7 @@ __global__ void __launch_bounds__(128) paged_gather_kernel(const __grid_constant
       live = 0;
     }
   }
+  o.wide = p.wide;
   o.live = live;
   o.zero = zero;
   o.k_sl = p.k_sl;
@@ -569,8 +715,8 @@ extern "C" int fpx_paged_append(int format, const void *q, int64_t q_sb, int64_t
   p.rope = rope; p.rope_len = rope_len; p.rotary = rotary;
   p.B = B; p.L = L; p.H = H; p.Hkv = Hkv; p.zero_padding = zero_padding != 0;
   const int64_t blocks = ((int64_t)B * L + 3) / 4;
-  const int query_chunks = (H + kQueryHeads - 1) / kQueryHeads, chunks = query_chunks + (2 * Hkv + kStoreHeads - 1) / kStoreHeads;
-  if (blocks > 0x7fffffff || chunks > 65535) return FPX_ERR_SHAPE;
+  const int query_chunks = (H + query_heads(d) - 1) / query_heads(d), chunks = query_chunks + (2 * Hkv + kStoreRows - 1) / kStoreRows;
+  if ((int64_t)B * L > 0x7ffffff0 || chunks > 65535) return FPX_ERR_SHAPE;
   const auto kernel = format == FPX_PAGES_INT4
                           ? (d == 256 ? paged_append_kernel<FPX_PAGES_INT4, 256> : paged_append_kernel<FPX_PAGES_INT4, 128>)
                           : (d == 256 ? paged_append_kernel<FPX_PAGES_BF16, 256> : paged_append_kernel<FPX_PAGES_BF16, 128>);
@@ -592,6 +738,7 @@ extern "C" int fpx_paged_gather(int format, const void *pool, int pages, int pag
   p.k = static_cast<__nv_bfloat16 *>(k); p.k_sb = ks.b; p.k_sl = ks.l; p.k_sh = ks.h;
   p.v = static_cast<__nv_bfloat16 *>(v); p.v_sb = vs.b; p.v_sl = vs.l; p.v_sh = vs.h;
   p.B = B; p.L = L; p.Hkv = Hkv; p.zero_padding = zero_padding != 0;
+  p.wide = !((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15) && ks.multiples_of(8) && vs.multiples_of(8);
   const int granules = L / kGranule + 2;  // that L rows can touch
   const int64_t blocks = ((int64_t)B * granules + 3) / 4;
   if (blocks > 0x7fffffff || Hkv > 65535) return FPX_ERR_SHAPE;
