@@ -16,7 +16,7 @@ struct AppendParams {
   const float *rope;  // [rope_len][rotary]: cosines, then sines; null: no rotation
   int rope_len, rotary;
   int B, L, H, Hkv;   // H = 0: keys and values alone
-  bool zero_padding;
+  bool zero_padding, q_wide, kv_wide;  // wide: q and q_out, or k, v and k_out, are 16-byte aligned rows
 };
 
 // A warp's share of a head row: lane holds dims 128 J + 4 lane .. + 3, as two packed words.
@@ -213,10 +213,10 @@ constexpr int kPasses = 8;                                     // of a warp over
 constexpr int query_heads(int d) { return kPasses * 32 / (d / 8); }
 constexpr int kStoreRows = 8;                                  // rows of [k heads | v heads] of a warp
 
-// Queries: D / 8 lanes a head row. A lane holds four dims and the four that they rotate with (or eight that do not
+// Queries of which a part rotates (or nothing): D / 8 lanes a head row. A lane holds four dims and the four that they rotate with (or eight that do not
 // rotate), so a rotation stays in the lane; the token's cosines and sines are loaded once for all of the warp's heads.
 template <int D>
-FPX_INLINE void append_queries(const AppendParams &p, int b, int l, int pos, int h0, bool live, int lane) {
+FPX_INLINE void append_queries_partly(const AppendParams &p, int b, int l, int pos, int h0, bool live, int lane) {
   constexpr int kLanes = D / 8, kRows = 32 / kLanes;
   const int u = lane % kLanes, sub = lane / kLanes, rotary = p.rope ? p.rotary : 0;
   const bool turns = 8 * u < rotary;
@@ -270,6 +270,88 @@ FPX_INLINE void append_queries(const AppendParams &p, int b, int l, int pos, int
   }
 }
 
+// Eight neighbouring dims; head rows are 8-byte aligned at least.
+FPX_INLINE uint4 load8(const __nv_bfloat16 *src, bool wide) {
+  if (wide) return *reinterpret_cast<const uint4 *>(src);
+  const uint2 lo = *reinterpret_cast<const uint2 *>(src), hi = *reinterpret_cast<const uint2 *>(src + 4);
+  return make_uint4(lo.x, lo.y, hi.x, hi.y);
+}
+FPX_INLINE void store8(__nv_bfloat16 *dst, uint4 v, bool wide) {
+  if (wide) {
+    *reinterpret_cast<uint4 *>(dst) = v;
+  } else {
+    *reinterpret_cast<uint2 *>(dst) = make_uint2(v.x, v.y);
+    *reinterpret_cast<uint2 *>(dst + 4) = make_uint2(v.z, v.w);
+  }
+}
+FPX_INLINE void unpack8(uint4 w, float (&x)[8]) {
+  const uint32_t v[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    x[2 * e] = __uint_as_float(v[e] << 16);
+    x[2 * e + 1] = __uint_as_float(v[e] & 0xffff0000u);
+  }
+}
+FPX_INLINE uint4 pack8(const float (&x)[8]) {
+  return make_uint4(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7]));
+}
+// Cosines and sines of dims 8 u .. + 7, where the whole head rotates; x and its partners half a head away, as
+// rotate_row: each product and each sum rounded (no fused multiply-add).
+template <int D>
+struct WholeTurn {
+  float c[8], s[8];
+  FPX_INLINE void load(const float *rope, int pos, int u) {
+    const float4 *row = reinterpret_cast<const float4 *>(rope + (int64_t)pos * D + 8 * u);
+    const float4 v[4] = {row[0], row[1], row[D / 8], row[D / 8 + 1]};
+    c[0] = v[0].x; c[1] = v[0].y; c[2] = v[0].z; c[3] = v[0].w; c[4] = v[1].x; c[5] = v[1].y; c[6] = v[1].z; c[7] = v[1].w;
+    s[0] = v[2].x; s[1] = v[2].y; s[2] = v[2].z; s[3] = v[2].w; s[4] = v[3].x; s[5] = v[3].y; s[6] = v[3].z; s[7] = v[3].w;
+  }
+  FPX_INLINE void turn(float (&x)[2][8]) const {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float a = x[0][e], z = x[1][e];
+      x[0][e] = __fsub_rn(__fmul_rn(a, c[e]), __fmul_rn(z, s[e]));
+      x[1][e] = __fadd_rn(__fmul_rn(z, c[e]), __fmul_rn(a, s[e]));
+    }
+  }
+};
+
+// Queries that rotate as a whole: D / 16 lanes a head row, the token's cosines and sines loaded once for the warp's heads.
+template <int D>
+FPX_INLINE void append_queries(const AppendParams &p, int b, int l, int pos, int h0, bool live, int lane) {
+  constexpr int kLanes = D / 16, kRows = 32 / kLanes, kTimes = query_heads(D) / kRows;
+  const int u = lane % kLanes, sub = lane / kLanes;
+  const __nv_bfloat16 *src = p.q + b * p.q_sb + l * p.q_sl + 8 * u;
+  __nv_bfloat16 *dst = p.q_out + b * p.qo_sb + l * p.qo_sl + 8 * u;
+  uint4 w[kTimes][2];
+#pragma unroll
+  for (int i = 0; i < kTimes; ++i) {
+    const int h = h0 + kRows * i + sub;
+    w[i][0] = w[i][1] = make_uint4(0, 0, 0, 0);
+    if (!live || h >= p.H) continue;
+    w[i][0] = load8(src + h * p.q_sh, p.q_wide);
+    w[i][1] = load8(src + h * p.q_sh + D / 2, p.q_wide);
+  }
+  WholeTurn<D> turn;
+  if (live) turn.load(p.rope, pos, u);
+  __syncwarp();  // q_out may be q: a lane stores only after every lane has loaded
+#pragma unroll
+  for (int i = 0; i < kTimes; ++i) {
+    const int h = h0 + kRows * i + sub;
+    if (h >= p.H) continue;
+    if (live) {
+      float x[2][8];
+      unpack8(w[i][0], x[0]);
+      unpack8(w[i][1], x[1]);
+      turn.turn(x);
+      w[i][0] = pack8(x[0]);
+      w[i][1] = pack8(x[1]);
+    }
+    store8(dst + h * p.qo_sh, w[i][0], p.q_wide);
+    store8(dst + h * p.qo_sh + D / 2, w[i][1], p.q_wide);
+  }
+}
+
 // Keys and values into their pages, where the whole head or nothing of it rotates: D / 16 lanes a row. A lane holds
 // dims 8 u .. + 7 and 8 u + d / 2 .. + 7, which rotate with each other; four lanes hold a group of 32.
 template <int FMT, int D>
@@ -284,20 +366,11 @@ FPX_INLINE void append_rows(const AppendParams &p, int b, int l, int pos, uint8_
     if (r >= last) continue;
     const __nv_bfloat16 *src = r < p.Hkv ? p.k + b * p.k_sb + l * p.k_sl + r * p.k_sh
                                          : p.v + b * p.v_sb + l * p.v_sl + (r - p.Hkv) * p.v_sh;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {  // head rows are 8-byte aligned
-      const uint2 lo = *reinterpret_cast<const uint2 *>(src + 8 * u + h * (D / 2));
-      const uint2 hi = *reinterpret_cast<const uint2 *>(src + 8 * u + h * (D / 2) + 4);
-      w[i][h] = make_uint4(lo.x, lo.y, hi.x, hi.y);
-    }
+    w[i][0] = load8(src + 8 * u, p.kv_wide);
+    w[i][1] = load8(src + 8 * u + D / 2, p.kv_wide);
   }
-  float c[8], s[8];
-  if (p.rope && r0 < p.Hkv) {
-    const float4 *row = reinterpret_cast<const float4 *>(p.rope + (int64_t)pos * D + 8 * u);
-    const float4 v[4] = {row[0], row[1], row[D / 8], row[D / 8 + 1]};
-    c[0] = v[0].x; c[1] = v[0].y; c[2] = v[0].z; c[3] = v[0].w; c[4] = v[1].x; c[5] = v[1].y; c[6] = v[1].z; c[7] = v[1].w;
-    s[0] = v[2].x; s[1] = v[2].y; s[2] = v[2].z; s[3] = v[2].w; s[4] = v[3].x; s[5] = v[3].y; s[6] = v[3].z; s[7] = v[3].w;
-  }
+  WholeTurn<D> turn;
+  if (p.rope && r0 < p.Hkv) turn.load(p.rope, pos, u);
   __syncwarp();  // k_out may be k: a lane stores only after every lane has loaded
 #pragma unroll
   for (int i = 0; i < kStoreRows / kRows; ++i) {
@@ -306,37 +379,16 @@ FPX_INLINE void append_rows(const AppendParams &p, int b, int l, int pos, uint8_
     const bool value = r >= p.Hkv, mine = r < last;
     const int kvh = value ? r - p.Hkv : r;
     float x[2][8];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const uint32_t v[4] = {w[i][h].x, w[i][h].y, w[i][h].z, w[i][h].w};
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        x[h][2 * e] = __uint_as_float(v[e] << 16);
-        x[h][2 * e + 1] = __uint_as_float(v[e] & 0xffff0000u);
-      }
-    }
-    if (!value && mine) {
-      if (p.rope) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {  // as rotate_row
-          const float a = x[0][e], z = x[1][e];
-          x[0][e] = __fsub_rn(__fmul_rn(a, c[e]), __fmul_rn(z, s[e]));
-          x[1][e] = __fadd_rn(__fmul_rn(z, c[e]), __fmul_rn(a, s[e]));
-        }
-      }
-    }
+    unpack8(w[i][0], x[0]);
+    unpack8(w[i][1], x[1]);
+    if (!value && p.rope) turn.turn(x);
     if (FMT == FPX_PAGES_BF16 || (!value && p.k_out)) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-        w[i][h] = make_uint4(pack_bf16(x[h][0], x[h][1]), pack_bf16(x[h][2], x[h][3]), pack_bf16(x[h][4], x[h][5]),
-                             pack_bf16(x[h][6], x[h][7]));
+      w[i][0] = pack8(x[0]);
+      w[i][1] = pack8(x[1]);
       if (!value && p.k_out && mine) {
         __nv_bfloat16 *dst = p.k_out + b * p.ko_sb + l * p.ko_sl + kvh * p.ko_sh + 8 * u;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          *reinterpret_cast<uint2 *>(dst + h * (D / 2)) = make_uint2(w[i][h].x, w[i][h].y);
-          *reinterpret_cast<uint2 *>(dst + h * (D / 2) + 4) = make_uint2(w[i][h].z, w[i][h].w);
-        }
+        store8(dst, w[i][0], p.kv_wide);
+        store8(dst + D / 2, w[i][1], p.kv_wide);
       }
     }
     uint8_t *page = gran + (int64_t)kvh * p.pv.head_bytes;
@@ -453,7 +505,10 @@ __global__ void __launch_bounds__(128) paged_append_kernel(const __grid_constant
   if (!live && !p.zero_padding) return;
   const int pos = (int)pos64;
   if ((int)blockIdx.y < query_chunks) {
-    append_queries<D>(p, b, l, pos, blockIdx.y * query_heads(D), live, lane);
+    if (p.rope && p.rotary == D)
+      append_queries<D>(p, b, l, pos, blockIdx.y * query_heads(D), live, lane);
+    else
+      append_queries_partly<D>(p, b, l, pos, blockIdx.y * query_heads(D), live, lane);
     return;
   }
   const int r0 = (blockIdx.y - query_chunks) * kStoreRows;
@@ -680,6 +735,9 @@ extern "C" size_t fpx_paged_page_bytes(int format, int Hkv, int d, int page_size
   return 0;
 }
 
+static bool row_aligned16(const void *p, const RowStrides &s) {
+  return !p || (!(reinterpret_cast<uintptr_t>(p) & 15) && s.multiples_of(8));
+}
 static bool row_aligned(const void *p, const RowStrides &s) {  // 8-byte pieces of a head row
   return !(reinterpret_cast<uintptr_t>(p) & 7) && s.multiples_of(4);
 }
@@ -714,6 +772,8 @@ extern "C" int fpx_paged_append(int format, const void *q, int64_t q_sb, int64_t
   p.k_out = static_cast<__nv_bfloat16 *>(k_out); p.ko_sb = ko.b; p.ko_sl = ko.l; p.ko_sh = ko.h;
   p.rope = rope; p.rope_len = rope_len; p.rotary = rotary;
   p.B = B; p.L = L; p.H = H; p.Hkv = Hkv; p.zero_padding = zero_padding != 0;
+  p.q_wide = row_aligned16(q, qs) && row_aligned16(q_out, qo);
+  p.kv_wide = row_aligned16(k, ks) && row_aligned16(v, vs) && row_aligned16(k_out, ko);
   const int64_t blocks = ((int64_t)B * L + 3) / 4;
   const int query_chunks = (H + query_heads(d) - 1) / query_heads(d), chunks = query_chunks + (2 * Hkv + kStoreRows - 1) / kStoreRows;
   if ((int64_t)B * L > 0x7ffffff0 || chunks > 65535) return FPX_ERR_SHAPE;
@@ -738,7 +798,7 @@ extern "C" int fpx_paged_gather(int format, const void *pool, int pages, int pag
   p.k = static_cast<__nv_bfloat16 *>(k); p.k_sb = ks.b; p.k_sl = ks.l; p.k_sh = ks.h;
   p.v = static_cast<__nv_bfloat16 *>(v); p.v_sb = vs.b; p.v_sl = vs.l; p.v_sh = vs.h;
   p.B = B; p.L = L; p.Hkv = Hkv; p.zero_padding = zero_padding != 0;
-  p.wide = !((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15) && ks.multiples_of(8) && vs.multiples_of(8);
+  p.wide = row_aligned16(k, ks) && row_aligned16(v, vs);
   const int granules = L / kGranule + 2;  // that L rows can touch
   const int64_t blocks = ((int64_t)B * granules + 3) / 4;
   if (blocks > 0x7fffffff || Hkv > 65535) return FPX_ERR_SHAPE;
