@@ -31,6 +31,7 @@
 namespace fpx {
 
 constexpr int kGranule = 16;  // tokens
+constexpr int kSms = 148;
 
 template <int FMT, int D>
 struct Granule;

@@ -874,8 +874,6 @@ __global__ void __launch_bounds__(kMergeThreads) paged_merge_kernel(const __grid
 
 // ---- host -----------------------------------------------------------------------------------
 
-constexpr int kSms = 148;
-
 template <int FMT, int D, int NT>
 struct Shape;  // granules of a step, warps of a CTA, stages of a warp's ring, CTAs of an SM
 template <> struct Shape<FPX_PAGES_INT4, 128, 1> { static constexpr int kGranules = 2, kWarps = 4, kStages = 3, kOcc = 3; };
