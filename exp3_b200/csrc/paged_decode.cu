@@ -25,6 +25,7 @@
 // finished there; the pieces of the others are merged in CTA order by the second launch, so
 // results do not depend on timing.
 #include <algorithm>
+#include <atomic>
 
 #include "paged.cuh"
 #include "tc.cuh"
@@ -921,8 +922,16 @@ static int launch(PagedDecodeParams &p, const Layout &w, cudaStream_t stream) {
   using Smem = PagedSmem<FMT, D, NT, S::kGranules, S::kWarps, S::kStages>;
   static_assert(sizeof(Smem) <= 227 * 1024, "shared memory of one CTA");
   const auto kernel = paged_decode_kernel<FMT, D, NT, S::kGranules, S::kWarps, S::kStages, S::kOcc>;
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(Smem)) != cudaSuccess)
-    return FPX_ERR_CUDA;
+  // The kernel's shared-memory limit is a setting of the device: once for each.
+  static std::atomic<uint64_t> set{0};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return FPX_ERR_CUDA;
+  const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+  if (!(set.load(std::memory_order_relaxed) & bit) || !bit) {
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(Smem)) != cudaSuccess)
+      return FPX_ERR_CUDA;
+    set.fetch_or(bit, std::memory_order_relaxed);
+  }
   p.min_steps = S::kWarps;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(w.ctas);

@@ -25,7 +25,7 @@ from typing import Optional
 
 import torch
 
-from ._capi import FpxError, call, lib
+from ._capi import STATUS, FpxError, lib
 
 FORMATS = {"bf16": 0, "int4": 1}
 MAX_ROWS = 64  # query rows of a sequence in one paged_decode_attention
@@ -60,22 +60,23 @@ def rope_table(positions: int, rotary: int = 128, theta: float = 1e6, device="cu
     return torch.cat((angle.cos(), angle.sin()), 1).float()
 
 
+_BF16, _U8, _I32, _F32 = torch.bfloat16, torch.uint8, torch.int32, torch.float32
+_ROW_DIMS = {(_BF16, 256): (0, 128), (_BF16, 512): (0, 256), (_U8, 146): (1, 128), (_U8, 290): (1, 256)}
+
+
 def _pool(pool: torch.Tensor):
     """(format id, head dim) of a pool tensor."""
     if pool.dim() != 4:
         raise FpxError("a pool is [pages, Hkv, page_size, row]")
-    row = pool.shape[3]
-    if pool.dtype is torch.bfloat16:
-        form, dim = 0, row // 2
-    elif pool.dtype is torch.uint8:
-        form, dim = 1, (row - 2) * 8 // 9
-    else:
-        raise TypeError("a pool is bfloat16, or uint8 in the 4-bit form")
-    if dim not in (128, 256) or row != (2 * dim if form == 0 else 9 * dim // 8 + 2):
+    dtype, row = pool.dtype, pool.shape[3]
+    known = _ROW_DIMS.get((dtype, row))
+    if known is None:
+        if dtype is not _BF16 and dtype is not _U8:
+            raise TypeError("a pool is bfloat16, or uint8 in the 4-bit form")
         raise FpxError(f"a pool's rows of {row} elements are of no compiled head dim")
     if not pool.is_contiguous():
         raise FpxError("a pool must be contiguous")
-    return form, dim
+    return known
 
 
 def _where(pool, page_table, starts, counts, batch, kv_heads, head_dim):
@@ -84,21 +85,26 @@ def _where(pool, page_table, starts, counts, batch, kv_heads, head_dim):
     pages, pool_heads, page_size, _ = pool.shape
     if dim != head_dim or pool_heads != kv_heads:
         raise FpxError(f"the pool holds {pool_heads} KV heads of {dim}, the call {kv_heads} of {head_dim}")
-    if page_table.dtype is not torch.int32 or starts.dtype is not torch.int32:
+    if page_table.dtype is not _I32 or starts.dtype is not _I32:
         raise TypeError("page_table, starts and counts must be int32")
-    if page_table.dim() != 2 or page_table.shape[0] != batch or (page_table.shape[1] > 1 and page_table.stride(1) != 1):
+    table_shape = page_table.shape
+    if len(table_shape) != 2 or table_shape[0] != batch:
         raise FpxError("page_table must be [B, max_pages] with contiguous rows")
-    if starts.shape != (batch,) or not starts.is_contiguous():
+    max_pages = table_shape[1]
+    stride, inner = page_table.stride()
+    if inner != 1 and max_pages > 1:
+        raise FpxError("page_table must be [B, max_pages] with contiguous rows")
+    if batch == 1:
+        stride = max_pages
+    if starts.dim() != 1 or starts.shape[0] != batch or not starts.is_contiguous():
         raise FpxError("starts and counts must be [B], contiguous")
     count_ptr = None
     if counts is not None:
-        if counts.dtype is not torch.int32:
+        if counts.dtype is not _I32:
             raise TypeError("page_table, starts and counts must be int32")
-        if counts.shape != (batch,) or not counts.is_contiguous():
+        if counts.dim() != 1 or counts.shape[0] != batch or not counts.is_contiguous():
             raise FpxError("starts and counts must be [B], contiguous")
         count_ptr = counts.data_ptr()
-    max_pages = page_table.shape[1]
-    stride = page_table.stride(0) if batch > 1 else max_pages
     return form, (pool.data_ptr(), pages, page_size, page_table.data_ptr(), stride, max_pages, starts.data_ptr(),
                   count_ptr)
 
@@ -114,20 +120,28 @@ def _device(first, *tensors):
     return dev
 
 
+@functools.lru_cache(maxsize=None)
+def _function(name):
+    return getattr(lib(), name)
+
+
 def _call(dev, name, *args):
     """The C call on dev's current stream, with dev as the current device (its default stream has no
     device of its own to be bound to)."""
-    stream = torch._C._cuda_getCurrentRawStream(dev.index)
-    if dev.index == torch.cuda.current_device():
-        call(name, *args, stream)
+    index = dev.index
+    stream = torch._C._cuda_getCurrentRawStream(index)
+    if index == torch._C._cuda_getDevice():
+        rc = _function(name)(*args, stream)
     else:
         with torch.cuda.device(dev):
-            call(name, *args, stream)
+            rc = _function(name)(*args, stream)
+    if rc != 0:
+        raise FpxError(f"{name} failed with status {rc} ({STATUS.get(rc, 'unknown')})")
 
 
 def _rows(t, shape, name):
     """(address, strides) of a bf16 tensor [B, L, heads, d] of the given shape."""
-    if t.dtype is not torch.bfloat16:
+    if t.dtype is not _BF16:
         raise TypeError("q, k, v and their outputs must be bfloat16")
     if t.shape != shape:
         raise FpxError(f"{name} must be {tuple(shape)}, is {tuple(t.shape)}")
@@ -167,7 +181,7 @@ def paged_append(k, v, pool, page_table, starts, counts=None, q=None, rope=None,
     rope_len = rotary = zero = heads = 0
     rope_ptr = None
     if rope is not None:
-        if rope.dtype is not torch.float32 or rope.dim() != 2 or not rope.is_contiguous():
+        if rope.dtype is not _F32 or rope.dim() != 2 or not rope.is_contiguous():
             raise FpxError("rope must be a contiguous fp32 [positions, rotary] table")
         rope_len, rotary = rope.shape
         rope_ptr = rope.data_ptr()
@@ -198,13 +212,13 @@ def paged_gather(pool, page_table, starts, counts, length: int, k_out=None, v_ou
     _, dim = _pool(pool)
     batch, kv_heads = starts.shape[0], pool.shape[1]
     form, where = _where(pool, page_table, starts, counts, batch, kv_heads, dim)
-    shape = (batch, length, kv_heads, dim)
+    shape = torch.Size((batch, length, kv_heads, dim))
     if (k_out is None) != (v_out is None):
         raise FpxError("give both of k_out and v_out, or neither")
     zero = int(k_out is None)
     if zero:
-        k_out = torch.empty(shape, dtype=torch.bfloat16, device=dev)
-        v_out = torch.empty(shape, dtype=torch.bfloat16, device=dev)
+        k_out = torch.empty(shape, dtype=_BF16, device=dev)
+        v_out = torch.empty_like(k_out)
     k_rows, v_rows = _output(k_out, shape, "k_out"), _output(v_out, shape, "v_out")
     if batch and length:
         _call(dev, "fpx_paged_gather", form, *where, batch, length, kv_heads, dim, *k_rows, *v_rows, zero)
@@ -236,7 +250,7 @@ def paged_decode_attention(q, pool, page_table, starts, scale: float, counts=Non
     if out is None:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
     o_rows = _output(out, shape, "out")
-    if lse is not None and (lse.dtype is not torch.float32 or not lse.is_contiguous() or lse.shape != shape[:3]):
+    if lse is not None and (lse.dtype is not _F32 or not lse.is_contiguous() or lse.shape != shape[:3]):
         raise FpxError("lse must be a contiguous fp32 [B, Lq, H]")
     if batch and rows:
         if ws is None:
