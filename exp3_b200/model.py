@@ -30,6 +30,10 @@ that, and its down all-reduce overlaps the following chunks (and the next layer'
 Only the last chunk's o_proj all-reduce of each layer is left exposed.
 
 The embedding and LM head are replicated; only the last token's logits are computed.
+
+The ``*_paged`` methods keep the cache in pages (``exp3_b200.paged``) instead of one dense tensor:
+several sequences of any lengths decode together, in bf16 or 4-bit pages, and a prompt that
+continues a cached one prefills its new rows only.
 """
 
 from __future__ import annotations
@@ -40,7 +44,7 @@ from dataclasses import dataclass
 import torch
 
 from . import decode as _decode
-from . import ops
+from . import ops, paged
 from ._capi import FpxError, call, lib, ptr, stream, strides3
 
 
@@ -188,6 +192,7 @@ class Qwen2Model:
         # Row chunks of the tensor-parallel prefill pipeline (1 = one pass per layer, no overlap).
         self.prefill_chunks = 4 if tp_size > 1 else 1
         self.replay_events = None  # (start, end, replays) of the last decode_graph
+        self._rope_table = None    # cosines and sines of the paged calls
 
     # ---------------------------------------------------------------- pieces
     def _rmsnorm(self, x, weight, residual=None):
@@ -455,6 +460,152 @@ class Qwen2Model:
             token = self.decode_step(token)
             out.append(token)
         return torch.stack(out)
+
+    # ---------------------------------------------------------------- paged cache
+    def new_cache(self, pages: int, page_size: int = 64, format: str = "int4", sequences: int = 1,
+                  max_tokens: int | None = None) -> paged.PagedKVCache:
+        """A paged cache for this rank's KV heads."""
+        return paged.PagedKVCache(self.cfg.num_hidden_layers, pages, len(self.kv), self.cfg.head_dim, page_size, format,
+                                  sequences, max_tokens, self.device)
+
+    def _table(self, cache):
+        if self._rope_table is None or self._rope_table.shape[0] < cache.max_tokens:
+            self._rope_table = paged.rope_table(cache.max_tokens, self.cfg.head_dim, self.cfg.rope_theta, self.device)
+        return self._rope_table
+
+    def _paged_rest(self, i, h, attn):
+        """The layer behind its attention: (residual stream, MLP output before its addition)."""
+        lw = self.layers[i]
+        o = self._all_reduce(attn @ lw.w_o.t())
+        x2 = self._rmsnorm(o, lw.ln2, residual=h)
+        return h, self._all_reduce(self._silu_mul(x2 @ lw.w_gu.t()) @ lw.w_down.t())
+
+    def _qkv(self, i, x, batch):
+        """Views [batch, rows, heads, d] of the layer's fused projection of x [batch * rows, hidden]."""
+        hq, hkv, d = len(self.qh), len(self.kv), self.cfg.head_dim
+        qkv = torch.addmm(self.layers[i].b_qkv, x, self.layers[i].w_qkv.t()).view(batch, -1, (hq + 2 * hkv) * d)
+        part = lambda a, n: qkv[..., a * d:(a + n) * d].unflatten(-1, (n, d))  # noqa: E731
+        return part(0, hq), part(hq, hkv), part(hq + hkv, hkv)
+
+    def _logits(self, rows, residual):
+        """fp32 logits of each row over the whole vocabulary."""
+        logits = (self._rmsnorm(rows, self.norm, residual=residual) @ self.lm_head.t()).float()
+        if self.vocab_sharded:
+            parts = torch.empty(self.tp_size, *logits.shape, dtype=logits.dtype, device=logits.device)
+            torch.distributed.all_gather_into_tensor(parts, logits, group=self.group)
+            logits = parts.transpose(0, 1).flatten(1)
+        return logits
+
+    @torch.inference_mode()
+    def prefill_paged(self, input_ids: torch.Tensor, cache: paged.PagedKVCache, sequence: int = 0, reuse: int = 0):
+        """One forward over a prompt into a slot of ``cache``; returns the last token's fp32 logits.
+
+        ``reuse`` tokens of the prompt are in the slot already (an earlier turn): whole 128-token tiles of
+        them are read back from the pages, and only the rows behind are computed and stored."""
+        if input_ids.dim() != 1 or input_ids.shape[0] == 0:
+            raise ValueError("input_ids must be 1-D and hold a token")
+        length = input_ids.shape[0]
+        if reuse < 0 or reuse > max(0, cache.lengths[sequence]):
+            raise ValueError(f"the slot holds {max(0, cache.lengths[sequence])} tokens, {reuse} cannot be reused")
+        prefix = min(reuse, length - 1) // ops.BLOCK_SIZE * ops.BLOCK_SIZE
+        cache.reserve(sequence, length)
+        cfg, a = self.cfg, self.attn
+        hq, hkv, d, dev = len(self.qh), len(self.kv), cfg.head_dim, self.device
+        at = lambda n: torch.tensor([n], dtype=torch.int32, device=dev)  # noqa: E731
+        pages, start = cache.page_table[sequence:sequence + 1], at(prefix)
+        table = self._table(cache)
+        if prefix:  # dense K / V of the whole prompt, and queries of which only the new rows are read
+            origin, counts = at(0), at(prefix)
+            k_all, v_all = (torch.empty(1, length, hkv, d, dtype=torch.bfloat16, device=dev) for _ in range(2))
+            q_all = torch.empty(1, length, hq, d, dtype=torch.bfloat16, device=dev)
+        h = torch.nn.functional.embedding(input_ids[prefix:], self.embed)
+        x = self._rmsnorm(h, self.layers[0].ln1)
+        for i in range(cfg.num_hidden_layers):
+            if i > 0:
+                x = self._rmsnorm(down, self.layers[i].ln1, residual=h)  # h += down
+            q, k, v = self._qkv(i, x, 1)
+            pool = cache.pools[i]
+            if prefix:
+                paged.paged_gather(pool, pages, origin, counts, prefix, k_all[:, :prefix], v_all[:, :prefix])
+                paged.paged_append(k, v, pool, pages, start, q=q, rope=table, q_out=q_all[:, prefix:], k_out=k_all[:, prefix:])
+                v_all[:, prefix:] = v
+                tiles = (prefix // ops.BLOCK_SIZE, -(-length // ops.BLOCK_SIZE))
+                attn = ops.prefill_attention(q_all, k_all, v_all, a.method, a.alpha, self.scale, a.sink, a.window,
+                                             a.last_full, tile_range=tiles)[:, prefix:]
+            else:
+                paged.paged_append(k, v, pool, pages, start, q=q, rope=table, q_out=q, k_out=k)
+                attn = ops.prefill_attention(q, k, v, a.method, a.alpha, self.scale, a.sink, a.window, a.last_full)
+            h, down = self._paged_rest(i, h, attn.reshape(length - prefix, hq * d))
+        cache.set_length(sequence, length)
+        return self._logits(down[-1:].contiguous(), h[-1:].contiguous())[0]
+
+    def _paged_step(self, tokens, cache, table):
+        """One token of every active slot: fp32 logits [sequences, vocab]; moves ``cache.starts``."""
+        n = cache.sequences
+        h = torch.nn.functional.embedding(tokens, self.embed)
+        x = self._rmsnorm(h, self.layers[0].ln1)
+        for i in range(self.cfg.num_hidden_layers):
+            if i > 0:
+                x = self._rmsnorm(down, self.layers[i].ln1, residual=h)
+            q, k, v = self._qkv(i, x, n)
+            where = (cache.pools[i], cache.page_table, cache.starts)
+            paged.paged_append(k, v, *where, q=q, rope=table, q_out=q)
+            attn = paged.paged_decode_attention(q, *where, self.scale)
+            h, down = self._paged_rest(i, h, attn.view(n, -1))
+        logits = self._logits(down, h)
+        cache.starts.add_((cache.starts >= 0).to(torch.int32))
+        return logits
+
+    def _paged_room(self, cache, steps):
+        for sequence, length in enumerate(cache.lengths):
+            if length >= 0:
+                cache.reserve(sequence, length + steps)
+
+    @torch.inference_mode()
+    def decode_paged(self, tokens: torch.Tensor, cache: paged.PagedKVCache):
+        """One dense greedy decode step of every active slot of ``cache``: tokens [sequences] (those of
+        inactive slots are ignored) -> fp32 logits [sequences, vocab]."""
+        if tokens.shape != (cache.sequences,):
+            raise ValueError(f"tokens must be [{cache.sequences}], one for each slot")
+        self._paged_room(cache, 1)
+        self._decode_comm()
+        logits = self._paged_step(tokens, cache, self._table(cache))
+        cache.advance()
+        return logits
+
+    @torch.inference_mode()
+    def decode_paged_graph(self, first_tokens: torch.Tensor, steps: int, cache: paged.PagedKVCache):
+        """``steps`` greedy tokens of every active slot, the first of them given: [steps, sequences] int64. The same
+        computation as ``decode_paged``, each step but the first one replay of a CUDA graph."""
+        if first_tokens.shape != (cache.sequences,):
+            raise ValueError(f"first_tokens must be [{cache.sequences}], one for each slot")
+        out = torch.empty(steps, cache.sequences, dtype=torch.int64, device=self.device)
+        out[0] = first_tokens
+        if steps == 1:
+            return out
+        self._paged_room(cache, steps - 1)
+        self._decode_comm()
+        table, token = self._table(cache), first_tokens.clone()
+
+        def one_step():
+            token.copy_(self._paged_step(token, cache, table).argmax(-1))
+
+        side = torch.cuda.Stream(device=self.device)  # the eager first step warms the allocator up
+        side.wait_stream(torch.cuda.current_stream(self.device))
+        with torch.cuda.stream(side):
+            one_step()
+        torch.cuda.current_stream(self.device).wait_stream(side)
+        out[1] = token
+        if steps > 2:
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                one_step()
+            for i in range(2, steps):
+                graph.replay()
+                out[i] = token
+            del graph  # a graph holding NCCL calls must go before the process group
+        cache.advance(steps - 1)
+        return out
 
     def close_comm(self):
         """Unmaps the peer all-reduce buffers (every rank calls it; no kernel of theirs may be

@@ -266,6 +266,63 @@ def paged_decode_workspace_bytes(pool, batch: int, rows: int, heads: int) -> int
     return _workspace_bytes(form, batch, rows, heads, pool.shape[1], dim)
 
 
+class PagedKVCache:
+    """The pools of a model's layers, the page table that they share, and which pages are free.
+
+    ``sequences`` slots of up to ``max_tokens`` tokens share ``pages`` pages. ``starts`` (device) is the
+    position of a slot's next token, negative for an inactive slot; ``lengths`` is the same on the host. Pages are
+    handed out by ``reserve`` and taken back by ``release``, on the host, before the calls that use them."""
+
+    def __init__(self, layers: int, pages: int, kv_heads: int, head_dim: int = 128, page_size: int = 64,
+                 format: str = "int4", sequences: int = 1, max_tokens: int | None = None, device="cuda"):
+        if layers <= 0 or sequences <= 0:
+            raise ValueError("a cache needs layers and sequences")
+        self.pools = new_pool(pages, kv_heads, head_dim, page_size, format, device, layers)
+        self.page_size, self.format, self.sequences = page_size, format, sequences
+        self.max_tokens = pages * page_size if max_tokens is None else max_tokens
+        self.page_table = torch.full((sequences, -(-self.max_tokens // page_size)), -1, dtype=torch.int32, device=device)
+        self.starts = torch.full((sequences,), -1, dtype=torch.int32, device=device)
+        self.lengths = [-1] * sequences
+        self._free = list(range(pages - 1, -1, -1))
+        self._held: list[list[int]] = [[] for _ in range(sequences)]
+
+    @property
+    def free_pages(self) -> int:
+        return len(self._free)
+
+    def reserve(self, sequence: int, tokens: int) -> None:
+        """Pages for ``tokens`` tokens of a slot in all (those that it holds count)."""
+        if tokens > self.max_tokens:
+            raise FpxError(f"{tokens} tokens: a slot holds {self.max_tokens}")
+        held = self._held[sequence]
+        more = -(-tokens // self.page_size) - len(held)
+        if more <= 0:
+            return
+        if more > len(self._free):
+            raise FpxError(f"{more} pages are needed, {len(self._free)} are free")
+        new = [self._free.pop() for _ in range(more)]
+        self.page_table[sequence, len(held):len(held) + more] = torch.tensor(new, dtype=torch.int32).to(self.page_table.device)
+        held.extend(new)
+
+    def release(self, sequence: int) -> None:
+        """Takes a slot's pages back and makes it inactive. Its calls must be in the stream already."""
+        self._free.extend(reversed(self._held[sequence]))
+        self._held[sequence] = []
+        self.page_table[sequence] = -1
+        self.set_length(sequence, -1)
+
+    def set_length(self, sequence: int, tokens: int) -> None:
+        """The slot's next token stands at position ``tokens`` (negative: inactive)."""
+        if tokens > len(self._held[sequence]) * self.page_size:
+            raise FpxError(f"the slot's {len(self._held[sequence])} pages hold fewer than {tokens} tokens")
+        self.lengths[sequence] = tokens
+        self.starts[sequence] = tokens
+
+    def advance(self, tokens: int = 1) -> None:
+        """Host side of a step that appended ``tokens`` tokens to every active slot and moved ``starts`` itself."""
+        self.lengths = [n + tokens if n >= 0 else n for n in self.lengths]
+
+
 # The same calls as PyTorch custom ops, for torch.compile and fake tensors.
 
 
@@ -305,5 +362,5 @@ def _(q, pool, page_table, starts, counts, scale):
     return q.new_empty(q.shape)
 
 
-__all__ = ["FORMATS", "new_pool", "rope_table", "row_elements", "paged_append", "paged_gather",
+__all__ = ["FORMATS", "PagedKVCache", "new_pool", "rope_table", "row_elements", "paged_append", "paged_gather",
            "paged_decode_attention", "paged_decode_workspace_bytes", "FpxError"]

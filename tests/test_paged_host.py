@@ -144,3 +144,33 @@ def test_rope_table_is_right_at_far_positions():
         import math
         angle = p * 1e6 ** (-2 * i / 128)
         assert abs(float(table[p, i]) - math.cos(angle)) < 1e-6 and abs(float(table[p, 64 + i]) - math.sin(angle)) < 1e-6
+
+
+def test_cache_pages_on_the_host():
+    """Pages are handed out once, taken back whole, and refused beyond the pool or a slot's size."""
+    cache = paged.PagedKVCache(2, pages=10, kv_heads=2, page_size=16, sequences=3, max_tokens=96, device="cpu")
+    assert cache.pools.shape == (2, 10, 2, 16, 146) and cache.page_table.shape == (3, 6)
+    cache.reserve(0, 33)
+    cache.reserve(0, 40)
+    cache.reserve(2, 96)
+    assert cache.free_pages == 1
+    used = [p for row in cache.page_table.tolist() for p in row if p >= 0]
+    assert len(used) == len(set(used)) == 9
+    with pytest.raises(_capi.FpxError):
+        cache.reserve(1, 17)
+    assert cache.free_pages == 1 and cache.page_table[1].tolist() == [-1] * 6
+    with pytest.raises(_capi.FpxError):
+        cache.reserve(2, 97)
+    with pytest.raises(_capi.FpxError):
+        cache.set_length(0, 49)
+    cache.set_length(0, 48)
+    cache.set_length(2, 0)
+    cache.advance(2)
+    assert cache.lengths == [50, -1, 2] and cache.starts.tolist() == [48, -1, 0]
+    cache.release(0)
+    assert cache.free_pages == 4 and cache.lengths[0] == -1 and cache.starts.tolist() == [-1, -1, 0]
+    cache.reserve(1, 64)
+    assert cache.free_pages == 0
+    for bad in (dict(layers=0), dict(sequences=0)):
+        with pytest.raises(ValueError):
+            paged.PagedKVCache(**{**dict(layers=1, pages=2, kv_heads=1, device="cpu"), **bad})
