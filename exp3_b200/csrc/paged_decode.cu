@@ -880,8 +880,9 @@ struct Shape;  // granules of a step, warps of a CTA, stages of a warp's ring, C
 template <> struct Shape<FPX_PAGES_INT4, 128, 1> { static constexpr int kGranules = 2, kWarps = 4, kStages = 3, kOcc = 3; };
 template <> struct Shape<FPX_PAGES_INT4, 128, 2> { static constexpr int kGranules = 2, kWarps = 4, kStages = 4, kOcc = 2; };
 template <> struct Shape<FPX_PAGES_INT4, 256, 1> { static constexpr int kGranules = 2, kWarps = 4, kStages = 2, kOcc = 2; };
-template <> struct Shape<FPX_PAGES_BF16, 128, 1> { static constexpr int kGranules = 1, kWarps = 4, kStages = 2, kOcc = 3; };
-template <> struct Shape<FPX_PAGES_BF16, 128, 2> { static constexpr int kGranules = 1, kWarps = 4, kStages = 2, kOcc = 3; };
+template <> struct Shape<FPX_PAGES_BF16, 256, 2> { static constexpr int kGranules = 1, kWarps = 4, kStages = 3, kOcc = 1; };
+template <> struct Shape<FPX_PAGES_BF16, 128, 1> { static constexpr int kGranules = 1, kWarps = 4, kStages = 3, kOcc = 2; };
+template <> struct Shape<FPX_PAGES_BF16, 128, 2> { static constexpr int kGranules = 1, kWarps = 4, kStages = 3, kOcc = 2; };
 template <> struct Shape<FPX_PAGES_BF16, 256, 1> { static constexpr int kGranules = 1, kWarps = 4, kStages = 3, kOcc = 1; };
 
 struct Layout {
@@ -896,19 +897,20 @@ constexpr int grid_ctas() {
   return kSms * Shape<FMT, D, NT>::kOcc;
 }
 
-// Column tiles: two where one would leave rows over, except at head dim 256 (registers).
+// Column tiles of a row block: two where one would leave rows over (16 rows at d = 128: 25.5 us in one block of two
+// tiles, 35 in two of one), but one for int4 at d = 256, whose registers two do not fit (16 rows: 59 us, 40 in two blocks).
 static Layout layout_of(int format, int B, int Lq, int H, int Hkv, int d) {
   Layout w{};
   const int64_t rows = (int64_t)Lq * (H / Hkv);
-  w.nt = d == 128 && rows > 8 ? 2 : 1;
+  w.nt = rows > 8 && !(format == FPX_PAGES_INT4 && d == 256) ? 2 : 1;
   w.rows = 8 * w.nt;
   w.blocks = (int)((rows + w.rows - 1) / w.rows);
   if (format == FPX_PAGES_INT4)
     w.ctas = d == 256 ? grid_ctas<FPX_PAGES_INT4, 256, 1>()
-                      : w.nt == 1 ? grid_ctas<FPX_PAGES_INT4, 128, 1>() : grid_ctas<FPX_PAGES_INT4, 128, 2>();
+                      : (w.nt == 1 ? grid_ctas<FPX_PAGES_INT4, 128, 1>() : grid_ctas<FPX_PAGES_INT4, 128, 2>());
   else
-    w.ctas = d == 256 ? grid_ctas<FPX_PAGES_BF16, 256, 1>()
-                      : w.nt == 1 ? grid_ctas<FPX_PAGES_BF16, 128, 1>() : grid_ctas<FPX_PAGES_BF16, 128, 2>();
+    w.ctas = d == 256 ? (w.nt == 1 ? grid_ctas<FPX_PAGES_BF16, 256, 1>() : grid_ctas<FPX_PAGES_BF16, 256, 2>())
+                      : (w.nt == 1 ? grid_ctas<FPX_PAGES_BF16, 128, 1>() : grid_ctas<FPX_PAGES_BF16, 128, 2>());
   w.units = (int64_t)B * w.blocks * Hkv;
   w.prefix = up256(((size_t)B * w.blocks + 1) * sizeof(int));
   w.ml = up256((size_t)(w.ctas + w.units) * w.rows * 2 * sizeof(float));
@@ -1005,6 +1007,6 @@ extern "C" int fpx_paged_decode_attention(int format, const void *q, int64_t q_s
     if (d == 256) return launch<FPX_PAGES_INT4, 256, 1>(p, w, stream);
     return w.nt == 1 ? launch<FPX_PAGES_INT4, 128, 1>(p, w, stream) : launch<FPX_PAGES_INT4, 128, 2>(p, w, stream);
   }
-  if (d == 256) return launch<FPX_PAGES_BF16, 256, 1>(p, w, stream);
+  if (d == 256) return w.nt == 1 ? launch<FPX_PAGES_BF16, 256, 1>(p, w, stream) : launch<FPX_PAGES_BF16, 256, 2>(p, w, stream);
   return w.nt == 1 ? launch<FPX_PAGES_BF16, 128, 1>(p, w, stream) : launch<FPX_PAGES_BF16, 128, 2>(p, w, stream);
 }
