@@ -20,14 +20,17 @@ names nothing (a page outside the pool, a position past the table) is skipped, a
 
 from __future__ import annotations
 
+import ctypes
 import functools
+from pathlib import Path
 from typing import Optional
 
 import torch
 
-from ._capi import STATUS, FpxError, lib
+from ._capi import FpxError, lib
 
 FORMATS = {"bf16": 0, "int4": 1}
+BINDING_PATH = Path(__file__).resolve().parent / "_paged.so"
 MAX_ROWS = 64  # query rows of a sequence in one paged_decode_attention
 
 
@@ -60,105 +63,17 @@ def rope_table(positions: int, rotary: int = 128, theta: float = 1e6, device="cu
     return torch.cat((angle.cos(), angle.sin()), 1).float()
 
 
-_BF16, _U8, _I32, _F32 = torch.bfloat16, torch.uint8, torch.int32, torch.float32
-_ROW_DIMS = {(_BF16, 256): (0, 128), (_BF16, 512): (0, 256), (_U8, 146): (1, 128), (_U8, 290): (1, 256)}
-
-
-def _pool(pool: torch.Tensor):
-    """(format id, head dim) of a pool tensor."""
-    if pool.dim() != 4:
-        raise FpxError("a pool is [pages, Hkv, page_size, row]")
-    dtype, row = pool.dtype, pool.shape[3]
-    known = _ROW_DIMS.get((dtype, row))
-    if known is None:
-        if dtype is not _BF16 and dtype is not _U8:
-            raise TypeError("a pool is bfloat16, or uint8 in the 4-bit form")
-        raise FpxError(f"a pool's rows of {row} elements are of no compiled head dim")
-    if not pool.is_contiguous():
-        raise FpxError("a pool must be contiguous")
-    return known
-
-
-def _where(pool, page_table, starts, counts, batch, kv_heads, head_dim):
-    """Checks the tensors that say where rows lie; (format, arguments of the C calls)."""
-    form, dim = _pool(pool)
-    pages, pool_heads, page_size, _ = pool.shape
-    if dim != head_dim or pool_heads != kv_heads:
-        raise FpxError(f"the pool holds {pool_heads} KV heads of {dim}, the call {kv_heads} of {head_dim}")
-    if page_table.dtype is not _I32 or starts.dtype is not _I32:
-        raise TypeError("page_table, starts and counts must be int32")
-    table_shape = page_table.shape
-    if len(table_shape) != 2 or table_shape[0] != batch:
-        raise FpxError("page_table must be [B, max_pages] with contiguous rows")
-    max_pages = table_shape[1]
-    stride, inner = page_table.stride()
-    if inner != 1 and max_pages > 1:
-        raise FpxError("page_table must be [B, max_pages] with contiguous rows")
-    if batch == 1:
-        stride = max_pages
-    if starts.dim() != 1 or starts.shape[0] != batch or not starts.is_contiguous():
-        raise FpxError("starts and counts must be [B], contiguous")
-    count_ptr = None
-    if counts is not None:
-        if counts.dtype is not _I32:
-            raise TypeError("page_table, starts and counts must be int32")
-        if counts.dim() != 1 or counts.shape[0] != batch or not counts.is_contiguous():
-            raise FpxError("starts and counts must be [B], contiguous")
-        count_ptr = counts.data_ptr()
-    return form, (pool.data_ptr(), pages, page_size, page_table.data_ptr(), stride, max_pages, starts.data_ptr(),
-                  count_ptr)
-
-
-def _device(first, *tensors):
-    """The tensors' common CUDA device."""
-    dev = first.device
-    if dev.type != "cuda":
-        raise FpxError("fpx ops run on CUDA tensors only (there is no CPU path)")
-    for t in tensors:
-        if t is not None and t.device != dev:
-            raise FpxError("all tensors of a call must be on one CUDA device")
-    return dev
-
-
 @functools.lru_cache(maxsize=None)
-def _function(name):
-    return getattr(lib(), name)
+def _binding():
+    """The module that checks a call's tensors and makes the C call on their device's current stream."""
+    if not BINDING_PATH.exists():
+        raise FpxError(f"{BINDING_PATH} is missing: build it with `python -m exp3_b200.build`")
+    from . import _paged
 
-
-def _call(dev, name, *args):
-    """The C call on dev's current stream, with dev as the current device (its default stream has no
-    device of its own to be bound to)."""
-    index = dev.index
-    stream = torch._C._cuda_getCurrentRawStream(index)
-    if index == torch._C._cuda_getDevice():
-        rc = _function(name)(*args, stream)
-    else:
-        with torch.cuda.device(dev):
-            rc = _function(name)(*args, stream)
-    if rc != 0:
-        raise FpxError(f"{name} failed with status {rc} ({STATUS.get(rc, 'unknown')})")
-
-
-def _rows(t, shape, name):
-    """(address, strides) of a bf16 tensor [B, L, heads, d] of the given shape."""
-    if t.dtype is not _BF16:
-        raise TypeError("q, k, v and their outputs must be bfloat16")
-    if t.shape != shape:
-        raise FpxError(f"{name} must be {tuple(shape)}, is {tuple(t.shape)}")
-    sb, sl, sh, sd = t.stride()
-    if sd != 1:
-        raise FpxError("the last dimension must be contiguous")
-    return t.data_ptr(), sb, sl, sh
-
-
-def _output(t, shape, name):
-    rows = _rows(t, shape, name)
-    if 0 in rows[1:] and any(s == 0 and n > 1 for s, n in zip(rows[1:], shape)):
-        raise FpxError(f"{name} must not be an expanded tensor")
-    return rows
-
-
-_NONE = (None, 0, 0, 0)
+    names = ("fpx_paged_append", "fpx_paged_gather", "fpx_paged_decode_attention", "fpx_paged_decode_workspace_bytes",
+             "fpx_status_string")
+    _paged.bind(*(ctypes.cast(getattr(lib(), name), ctypes.c_void_p).value for name in names), FpxError)
+    return _paged
 
 
 def paged_append(k, v, pool, page_table, starts, counts=None, q=None, rope=None, q_out=None, k_out=None):
@@ -171,63 +86,13 @@ def paged_append(k, v, pool, page_table, starts, counts=None, q=None, rope=None,
     padding rows are left as they are.
     Rotation is in fp32 and rounds once, to bf16 or to the 4-bit codes. Sequences of one call must not
     write the same page."""
-    dev = _device(k, v, pool, page_table, starts, counts, q, rope, q_out, k_out)
-    shape = k.shape
-    if len(shape) != 4:
-        raise FpxError("k and v must be [B, L, Hkv, d]")
-    batch, length, kv_heads, dim = shape
-    k_rows, v_rows = _rows(k, shape, "k"), _rows(v, shape, "v")
-    form, where = _where(pool, page_table, starts, counts, batch, kv_heads, dim)
-    rope_len = rotary = zero = heads = 0
-    rope_ptr = None
-    if rope is not None:
-        if rope.dtype is not _F32 or rope.dim() != 2 or not rope.is_contiguous():
-            raise FpxError("rope must be a contiguous fp32 [positions, rotary] table")
-        rope_len, rotary = rope.shape
-        rope_ptr = rope.data_ptr()
-    q_rows = qo_rows = ko_rows = _NONE
-    if q is None:
-        if q_out is not None:
-            raise FpxError("q_out without q")
-    else:
-        if q.dim() != 4:
-            raise FpxError("q must be [B, L, H, d]")
-        heads = q.shape[2]
-        q_rows = _rows(q, (batch, length, heads, dim), "q")
-        if q_out is None:
-            zero, q_out = 1, torch.empty_like(q, memory_format=torch.contiguous_format)
-        qo_rows = _output(q_out, q.shape, "q_out")
-    if k_out is not None:
-        ko_rows = _output(k_out, shape, "k_out")
-    if batch and length:
-        _call(dev, "fpx_paged_append", form, *q_rows, *k_rows, *v_rows, batch, length, heads, kv_heads, dim, rope_ptr,
-              rope_len, rotary, *where, *qo_rows, *ko_rows, zero)
-    return q_out
+    return _binding().paged_append(k, v, pool, page_table, starts, counts, q, rope, q_out, k_out)
 
 
 def paged_gather(pool, page_table, starts, counts, length: int, k_out=None, v_out=None):
     """Rows back as bf16: (k, v) [B, length, Hkv, d], for a prefill over a cached prefix. Rows behind
     ``counts`` (None: every row counts) are left as they are in given outputs, and zero in new ones."""
-    dev = _device(pool, page_table, starts, counts, k_out, v_out)
-    _, dim = _pool(pool)
-    batch, kv_heads = starts.shape[0], pool.shape[1]
-    form, where = _where(pool, page_table, starts, counts, batch, kv_heads, dim)
-    shape = torch.Size((batch, length, kv_heads, dim))
-    if (k_out is None) != (v_out is None):
-        raise FpxError("give both of k_out and v_out, or neither")
-    zero = int(k_out is None)
-    if zero:
-        k_out = torch.empty(shape, dtype=_BF16, device=dev)
-        v_out = torch.empty_like(k_out)
-    k_rows, v_rows = _output(k_out, shape, "k_out"), _output(v_out, shape, "v_out")
-    if batch and length:
-        _call(dev, "fpx_paged_gather", form, *where, batch, length, kv_heads, dim, *k_rows, *v_rows, zero)
-    return k_out, v_out
-
-
-@functools.lru_cache(maxsize=256)
-def _workspace_bytes(form, batch, rows, heads, kv_heads, dim) -> int:
-    return int(lib().fpx_paged_decode_workspace_bytes(form, batch, rows, heads, kv_heads, dim))
+    return _binding().paged_gather(pool, page_table, starts, counts, length, k_out, v_out)
 
 
 def paged_decode_attention(q, pool, page_table, starts, scale: float, counts=None, out=None, lse=None, ws=None):
@@ -239,31 +104,18 @@ def paged_decode_attention(q, pool, page_table, starts, scale: float, counts=Non
     prefix with ``paged_gather`` and runs ``prefill_attention``. ``ws`` is a uint8 workspace of
     ``paged_decode_workspace_bytes``; without it each call takes its own from torch's allocator, so calls on
     several streams or in several graphs share nothing."""
-    dev = _device(q, pool, page_table, starts, counts, out, lse, ws)
-    shape = q.shape
-    if len(shape) != 4:
-        raise FpxError("q must be [B, Lq, H, d]")
-    batch, rows, heads, dim = shape
-    q_rows = _rows(q, shape, "q")
-    kv_heads = pool.shape[1] if pool.dim() == 4 else 0
-    form, where = _where(pool, page_table, starts, counts, batch, kv_heads, dim)
-    if out is None:
-        out = torch.empty_like(q, memory_format=torch.contiguous_format)
-    o_rows = _output(out, shape, "out")
-    if lse is not None and (lse.dtype is not _F32 or not lse.is_contiguous() or lse.shape != shape[:3]):
-        raise FpxError("lse must be a contiguous fp32 [B, Lq, H]")
-    if batch and rows:
-        if ws is None:
-            ws = torch.empty(_workspace_bytes(form, batch, rows, heads, kv_heads, dim), dtype=torch.uint8, device=dev)
-        _call(dev, "fpx_paged_decode_attention", form, *q_rows, batch, rows, heads, kv_heads, dim, scale, *where,
-              *o_rows, None if lse is None else lse.data_ptr(), ws.data_ptr(), ws.numel())
-    return out
+    return _binding().paged_decode_attention(q, pool, page_table, starts, scale, counts, out, lse, ws)
+
+
+def _head_dim(pool) -> int:
+    return {256: 128, 512: 256, 146: 128, 290: 256}.get(pool.shape[-1], 0)
 
 
 def paged_decode_workspace_bytes(pool, batch: int, rows: int, heads: int) -> int:
     """Bytes of ``paged_decode_attention``'s workspace, whatever the sequences' lengths."""
-    form, dim = _pool(pool)
-    return _workspace_bytes(form, batch, rows, heads, pool.shape[1], dim)
+    none = torch.empty(0, dtype=torch.int32)
+    form = _binding().check_where(pool, none[None, :0][:0], none, None, 0, pool.shape[1], _head_dim(pool))
+    return int(lib().fpx_paged_decode_workspace_bytes(form, batch, rows, heads, pool.shape[1], _head_dim(pool)))
 
 
 class PagedKVCache:
@@ -347,7 +199,7 @@ def _gather_op(pool: torch.Tensor, page_table: torch.Tensor, starts: torch.Tenso
 
 @_gather_op.register_fake
 def _(pool, page_table, starts, counts, length):
-    shape = (starts.shape[0], length, pool.shape[1], _pool(pool)[1])
+    shape = (starts.shape[0], length, pool.shape[1], _head_dim(pool))
     return pool.new_empty(shape, dtype=torch.bfloat16), pool.new_empty(shape, dtype=torch.bfloat16)
 
 

@@ -110,8 +110,9 @@ def test_python_refusals():
         paged.paged_gather(pool, table, starts, None, 4)
     with pytest.raises(_capi.FpxError):
         paged.paged_decode_attention(k[:, :1], pool, table, starts, 0.1)
-    fit = paged._where
-    assert fit(pool, table, starts, None, 1, 2, 128)[0] == 1
+    fit = paged._binding().check_where
+    assert fit(pool, table, starts, None, 1, 2, 128) == 1
+    assert paged.paged_decode_workspace_bytes(pool, 3, 2, 6) == _capi.lib().fpx_paged_decode_workspace_bytes(1, 3, 2, 6, 2, 128)
     for args in ((pool, table, starts, None, 1, 3, 128), (pool, table, starts, None, 1, 2, 256), (pool, table, starts, None, 2, 2, 128),
                  (pool[..., :-1], table, starts, None, 1, 2, 128), (pool.transpose(0, 1), table, starts, None, 1, 4, 128),
                  (pool[0], table, starts, None, 1, 2, 128), (pool, table, starts[None], None, 1, 2, 128),
