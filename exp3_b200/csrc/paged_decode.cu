@@ -42,6 +42,7 @@ struct PagedDecodeParams {
   int B, Lq, H, Hkv, group, blocks;  // blocks: row blocks of 8 NT (query row, head of the group) pairs
   float scale_log2;
   int ctas, min_steps;
+  bool whole;      // a CTA a unit, no merge
   int *prefix;     // [B * blocks + 1] steps of all heads before an item (b, row block)
   float *part_o;   // [ctas + units][8 NT][d]
   float *part_ml;  // [ctas + units][8 NT][2]
@@ -457,75 +458,85 @@ __global__ void __launch_bounds__(32 * W, OCC) paged_decode_kernel(const __grid_
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
-  // This CTA's run of steps, and the item that it starts in.
-  const int chunk = (items + kThreads - 1) / kThreads;
-  const int i0 = min(items, tid * chunk), i1 = min(items, i0 + chunk);
-  auto steps_in = [&](int i) {
-    const int b = i / p.blocks;
-    int start, count;
-    p.pv.rows(b, p.Lq, start, count);
-    return padded(steps_of<GS>(item_keys<NT>(p, start, count, i - b * p.blocks))) * p.Hkv;
-  };
-  int mine = 0;
-  for (int i = i0; i < i1; ++i) mine += steps_in(i);
-  int before = mine;
+  int lo = 0, hi = 0, item = 0, base = 0;
+  if (p.whole) {
+    item = blockIdx.x / p.Hkv;
+    __syncthreads();  // the barriers
+  } else {
+    // This CTA's run of steps, and the item that it starts in.
+    const int chunk = (items + kThreads - 1) / kThreads;
+    const int i0 = min(items, tid * chunk), i1 = min(items, i0 + chunk);
+    auto steps_in = [&](int i) {
+      const int b = i / p.blocks;
+      int start, count;
+      p.pv.rows(b, p.Lq, start, count);
+      return padded(steps_of<GS>(item_keys<NT>(p, start, count, i - b * p.blocks))) * p.Hkv;
+    };
+    int mine = 0;
+    for (int i = i0; i < i1; ++i) mine += steps_in(i);
+    int before = mine;
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int x = __shfl_up_sync(0xffffffffu, before, o);
-    if (lane >= o) before += x;
-  }
-  if (lane == 31) sh.scan[warp] = before;
-  before -= mine;
-  __syncthreads();
-  int total = 0;
-#pragma unroll
-  for (int w = 0; w < W; ++w) {
-    if (w < warp) before += sh.scan[w];
-    total += sh.scan[w];
-  }
-  if (blockIdx.x == 0) {  // for the merge
-    int at = before;
-    for (int i = i0; i < i1; ++i) {
-      p.prefix[i] = at;
-      at += chunk == 1 ? mine : steps_in(i);
+    for (int o = 1; o < 32; o <<= 1) {
+      const int x = __shfl_up_sync(0xffffffffu, before, o);
+      if (lane >= o) before += x;
     }
-    if (tid == 0) p.prefix[items] = total;
-  }
-  const int per = max(p.min_steps, (total + p.ctas - 1) / p.ctas);
-  int lo = (int)min((int64_t)blockIdx.x * per, (int64_t)total);
-  const int hi = min(total, lo + per);
-  if (lo >= hi) return;
-  if (before <= lo && lo < before + mine) {
-    int at = before;
-    for (int i = i0; i < i1; ++i) {
-      const int n = chunk == 1 ? mine : steps_in(i);
-      if (lo < at + n) {
-        sh.item = i;
-        sh.base = at;
-        break;
+    if (lane == 31) sh.scan[warp] = before;
+    before -= mine;
+    __syncthreads();
+    int total = 0;
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      if (w < warp) before += sh.scan[w];
+      total += sh.scan[w];
+    }
+    if (blockIdx.x == 0) {  // for the merge
+      int at = before;
+      for (int i = i0; i < i1; ++i) {
+        p.prefix[i] = at;
+        at += chunk == 1 ? mine : steps_in(i);
       }
-      at += n;
+      if (tid == 0) p.prefix[items] = total;
     }
+    const int per = max(p.min_steps, (total + p.ctas - 1) / p.ctas);
+    lo = (int)min((int64_t)blockIdx.x * per, (int64_t)total);
+    hi = min(total, lo + per);
+    if (lo >= hi) return;
+    if (before <= lo && lo < before + mine) {
+      int at = before;
+      for (int i = i0; i < i1; ++i) {
+        const int n = chunk == 1 ? mine : steps_in(i);
+        if (lo < at + n) {
+          sh.item = i;
+          sh.base = at;
+          break;
+        }
+        at += n;
+      }
+    }
+    __syncthreads();
+    item = sh.item;
+    base = sh.base;
   }
-  __syncthreads();
 
   const Lane<FMT, D> at(lane);
   uint8_t *const ring_bytes = sh.ring(warp);
   const uint32_t ring = smem_u32(ring_bytes);
 
   // The part of a unit that this CTA works on: steps g0 .. g1 - 1 of n_steps. lo is its place in the partition.
-  int item = sh.item, base = sh.base;
   int b, rb, kvh, start, rows, seen, n_steps, g0, g1;
+  auto read_item = [&]() {
+    b = item / p.blocks;
+    rb = item - b * p.blocks;
+    int count;
+    p.pv.rows(b, p.Lq, start, count);
+    rows = count * p.group;
+    seen = item_keys<NT>(p, start, count, rb);
+    n_steps = steps_of<GS>(seen);
+  };
   auto find = [&]() {  // the next part from lo on; false: none is left
     while (lo < hi) {
       for (;;) {
-        b = item / p.blocks;
-        rb = item - b * p.blocks;
-        int count;
-        p.pv.rows(b, p.Lq, start, count);
-        rows = count * p.group;
-        seen = item_keys<NT>(p, start, count, rb);
-        n_steps = steps_of<GS>(seen);
+        read_item();
         if (lo - base < padded(n_steps) * p.Hkv) break;
         base += padded(n_steps) * p.Hkv;
         ++item;
@@ -600,7 +611,22 @@ __global__ void __launch_bounds__(32 * W, OCC) paged_decode_kernel(const __grid_
     sent = 0;
     if (todo > 0 && !stopped) issue();
   };
-  if (!find()) return;
+  if (p.whole) {
+    read_item();
+    kvh = blockIdx.x - item * p.Hkv;
+    g0 = 0;
+    g1 = n_steps;
+    // rows that see nothing: padding, and inactive sequences
+    for (int i = max(0, rows - rb * kRows) * (D / 4) + tid; i < min(kRows, p.Lq * p.group - rb * kRows) * (D / 4); i += kThreads) {
+      const int r = rb * kRows + i / (D / 4), row = r / p.group, h = kvh * p.group + r % p.group, d = 4 * (i % (D / 4));
+      __nv_bfloat16 *out = p.out + b * p.o_sb + row * p.o_sl + h * p.o_sh + d;
+      out[0] = out[1] = out[2] = out[3] = __float2bfloat16_rn(0.f);
+      if (p.lse && d == 0) p.lse[((int64_t)b * p.Lq + row) * p.H + h] = -INFINITY;
+    }
+    if (n_steps == 0) return;
+  } else if (!find()) {
+    return;
+  }
   begin();
   for (;;) {
     const int row0 = rb * kRows;
@@ -792,45 +818,56 @@ __global__ void __launch_bounds__(32 * W, OCC) paged_decode_kernel(const __grid_
   }
 }
 
-// Merges the pieces of one (unit, row): D / 4 threads a piece, kPieces of them at a time, kAhead
-// loads in flight before the weights are known. Rows that see nothing (padding, inactive
-// sequences) become zero here.
-template <int D, int NT, int kMergeThreads>
-__global__ void __launch_bounds__(kMergeThreads) paged_merge_kernel(const __grid_constant__ PagedDecodeParams p) {
-  constexpr int kPieces = kMergeThreads / (D / 4), kRows = 8 * NT, kAhead = kMergeThreads == 512 ? 10 : 4;
-  const int r = blockIdx.y, kvh = blockIdx.x % p.Hkv, item = blockIdx.x / p.Hkv;
-  const int b = item / p.blocks, rr = (item % p.blocks) * kRows + r;
-  const int row = rr / p.group, h = kvh * p.group + rr % p.group;
-  const int tid = threadIdx.x, piece = tid / (D / 4), d = 4 * (tid % (D / 4));
-  __shared__ float red[kMergeThreads / 32];
+// What the merge launches know of a unit: its pieces lie in slots slot .. slot + pieces - 1 (one piece: its CTA has
+// finished it; none: no row of it sees anything).
+struct Pieces {
+  int b, rb, kvh, rows, pieces;
+  int64_t slot;
+  FPX_INLINE Pieces(const PagedDecodeParams &p, int unit) {
+    const int item = unit / p.Hkv;
+    kvh = unit - item * p.Hkv;
+    b = item / p.blocks;
+    rb = item - b * p.blocks;
+    const int base = p.prefix[item], next = p.prefix[item + 1], total = p.prefix[p.B * p.blocks];
+    int start, count;
+    p.pv.rows(b, p.Lq, start, count);
+    rows = count * p.group;
+    const int n = (next - base) / p.Hkv;  // padding, then steps
+    const int per = max(p.min_steps, (total + p.ctas - 1) / p.ctas);
+    const int first = base + kvh * n, c0 = (first + kPad) / per, c1 = (first + n - 1) / per;
+    pieces = n ? c1 - c0 + 1 : 0;
+    slot = c0 + (int64_t)item * p.Hkv + kvh;
+  }
+};
+
+// Merges the pieces of one (unit, row), where rows are few and pieces many: D / 4 threads a piece, kPieces of them at a
+// time, kAhead loads in flight before the weights are known. Rows that see nothing (padding, inactive sequences)
+// become zero here.
+template <int D, int NT>
+__global__ void __launch_bounds__(512) paged_merge_pieces_kernel(const __grid_constant__ PagedDecodeParams p) {
+  constexpr int kThreads = 512, kPieces = kThreads / (D / 4), kRows = 8 * NT, kAhead = 10;
+  const int r = blockIdx.y, tid = threadIdx.x, piece = tid / (D / 4), d = 4 * (tid % (D / 4));
+  __shared__ float red[kThreads / 32];
   __shared__ __align__(16) float part[kPieces][D];
-  __shared__ float weight[kMergeThreads];
+  __shared__ float weight[kThreads];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const Pieces u(p, blockIdx.x);
+  const int rr = u.rb * kRows + r, row = rr / p.group, h = u.kvh * p.group + rr % p.group;
   if (rr >= p.Lq * p.group) return;
-  const int base = p.prefix[item], next = p.prefix[item + 1], total = p.prefix[p.B * p.blocks];
-  int start, count;
-  p.pv.rows(b, p.Lq, start, count);
-  const int n = (next - base) / p.Hkv;
-  __nv_bfloat16 *out = p.out + b * p.o_sb + row * p.o_sl + h * p.o_sh;
-  float *lse = p.lse ? p.lse + ((int64_t)b * p.Lq + row) * p.H + h : nullptr;
-  if (row >= count || n == 0) {
-    for (int i = tid; i < D; i += kMergeThreads) out[i] = __float2bfloat16_rn(0.f);
+  __nv_bfloat16 *out = p.out + u.b * p.o_sb + row * p.o_sl + h * p.o_sh;
+  float *lse = p.lse ? p.lse + ((int64_t)u.b * p.Lq + row) * p.H + h : nullptr;
+  if (rr >= u.rows || u.pieces == 0) {
+    for (int i = tid; i < D; i += kThreads) out[i] = __float2bfloat16_rn(0.f);
     if (lse && tid == 0) *lse = -INFINITY;
     return;
   }
-  const int per = max(p.min_steps, (total + p.ctas - 1) / p.ctas);
-  const int first = base + kvh * n;  // padding, then steps
-  const int c0 = (first + kPad) / per, c1 = (first + n - 1) / per;
-  if (c0 == c1) return;  // finished by its CTA
-  const int64_t slot0 = c0 + (int64_t)item * p.Hkv + kvh;
-  const int pieces = c1 - c0 + 1;
-  const float *ml = p.part_ml + 2 * (slot0 * kRows + r), *po = p.part_o + (slot0 * kRows + r) * D + d;
+  if (u.pieces == 1) return;
+  const float *ml = p.part_ml + 2 * (u.slot * kRows + r), *po = p.part_o + (u.slot * kRows + r) * D + d;
   float m = kLowest, l = 0.f;
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-  // kMergeThreads pieces at a time (there are no more unless a later GPU has more CTAs)
-  for (int i0 = 0; i0 < pieces; i0 += kMergeThreads) {
-    const int here = min(pieces - i0, kMergeThreads);
+  for (int i0 = 0; i0 < u.pieces; i0 += kThreads) {
+    const int here = min(u.pieces - i0, kThreads);
     float2 mine = make_float2(kLowest, 0.f);
     if (tid < here) mine = *reinterpret_cast<const float2 *>(ml + 2 * (int64_t)(i0 + tid) * kRows);
     float4 x[kAhead];
@@ -839,7 +876,7 @@ __global__ void __launch_bounds__(kMergeThreads) paged_merge_kernel(const __grid
       const int i = piece + k * kPieces;
       x[k] = i < here ? *reinterpret_cast<const float4 *>(po + (int64_t)(i0 + i) * kRows * D) : make_float4(0.f, 0.f, 0.f, 0.f);
     }
-    const float top = fmaxf(m, block_max<kMergeThreads>(mine.x, red));  // NaN stays out of m, and in l
+    const float top = fmaxf(m, block_max<kThreads>(mine.x, red));  // NaN stays out of m, and in l
     const float keep = tc::ex2(m - top);
     m = top;
     const float s = tid < here ? tc::ex2(mine.x - m) : 0.f;
@@ -862,15 +899,55 @@ __global__ void __launch_bounds__(kMergeThreads) paged_merge_kernel(const __grid
     __syncthreads();
   }
   *reinterpret_cast<float4 *>(&part[piece][d]) = o;
-  l = block_sum<kMergeThreads>(l, red);  // its barriers publish part
+  l = block_sum<kThreads>(l, red);  // its barriers publish part
   const float inv = l == 0.f ? 0.f : 1.f / l;
-  for (int i = tid; i < D; i += kMergeThreads) {
+  for (int i = tid; i < D; i += kThreads) {
     float x = 0.f;
 #pragma unroll
     for (int k = 0; k < kPieces; ++k) x += part[k][i];
     out[i] = __float2bfloat16_rn(x * inv);
   }
   if (lse && tid == 0) *lse = l == 0.f ? -INFINITY : m * kLn2 + logf(l);
+}
+
+// The same where units are many and pieces few: a block a unit, a warp a row, D / 32 dims a lane.
+template <int D, int NT>
+__global__ void __launch_bounds__(256 * NT) paged_merge_rows_kernel(const __grid_constant__ PagedDecodeParams p) {
+  constexpr int kRows = 8 * NT;
+  const int r = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const Pieces u(p, blockIdx.x);
+  const int rr = u.rb * kRows + r, row = rr / p.group, h = u.kvh * p.group + rr % p.group;
+  const bool sees = rr < u.rows && u.pieces > 0;
+  if (rr >= p.Lq * p.group || (sees && u.pieces == 1)) return;
+  float m = kLowest, l = 0.f;
+  float4 o[D / 128] = {};
+  if (sees) {
+    const float *ml = p.part_ml + 2 * (u.slot * kRows + r), *po = p.part_o + (u.slot * kRows + r) * D + 4 * lane;
+    for (int i = lane; i < u.pieces; i += 32) m = fmaxf(m, ml[2 * (int64_t)i * kRows]);
+    m = warp_max(m);
+#pragma unroll 4
+    for (int i = 0; i < u.pieces; ++i) {
+      const float2 mine = *reinterpret_cast<const float2 *>(ml + 2 * (int64_t)i * kRows);
+      const float s = tc::ex2(mine.x - m);
+      l = fmaf(mine.y, s, l);
+#pragma unroll
+      for (int J = 0; J < D / 128; ++J) {
+        const float4 x = *reinterpret_cast<const float4 *>(po + (int64_t)i * kRows * D + 128 * J);
+        o[J].x = fmaf(x.x, s, o[J].x); o[J].y = fmaf(x.y, s, o[J].y); o[J].z = fmaf(x.z, s, o[J].z); o[J].w = fmaf(x.w, s, o[J].w);
+      }
+    }
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  __nv_bfloat16 *out = p.out + u.b * p.o_sb + row * p.o_sl + h * p.o_sh + 4 * lane;
+#pragma unroll
+  for (int J = 0; J < D / 128; ++J) {
+    const float x[4] = {o[J].x * inv, o[J].y * inv, o[J].z * inv, o[J].w * inv};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) out[128 * J + e] = __float2bfloat16_rn(x[e]);
+  }
+  if (p.lse && lane == 0) p.lse[((int64_t)u.b * p.Lq + row) * p.H + h] = l == 0.f ? -INFINITY : m * kLn2 + logf(l);
 }
 
 // ---- host -----------------------------------------------------------------------------------
@@ -918,6 +995,8 @@ static Layout layout_of(int format, int B, int Lq, int H, int Hkv, int d) {
   return w;
 }
 
+constexpr int kWholeTokens = 512, kWholeUnits = 32;
+
 template <int FMT, int D, int NT>
 static int launch(PagedDecodeParams &p, const Layout &w, cudaStream_t stream) {
   using S = Shape<FMT, D, NT>;
@@ -935,8 +1014,16 @@ static int launch(PagedDecodeParams &p, const Layout &w, cudaStream_t stream) {
     set.fetch_or(bit, std::memory_order_relaxed);
   }
   p.min_steps = S::kWarps;
+  // Short tables: a CTA a unit and one launch. Otherwise no more CTAs than the table could keep busy. Four KV heads,
+  // int4, us in one launch / in two: 1 sequence of 256 tokens 5.6 / 8.2, 512 7.4 / 8.4, 1024 10.8 / 8.4; 37 sequences 6.7 /
+  // 11.1, 8.4 / 16.2, 11.8 / 14.0; bf16: 5.5 / 7.5, 7.4 / 7.7, 11.0 / 7.5 and 5.8 / 9.6, 9.7 / 13.3, 15.7 / 19.4.
+  const int64_t longest = ((int64_t)p.pv.max_pages << p.pv.page_shift) / S::kGranules + 1;  // steps
+  const int64_t tokens = ((int64_t)p.pv.max_pages << p.pv.page_shift) * kGranule;
+  p.whole = tokens <= (w.units >= kWholeUnits ? 2 * kWholeTokens : kWholeTokens);
+  const int64_t busy = w.units * (longest + kPad) / p.min_steps + 1;
+  p.ctas = (int)(p.whole ? w.units : std::min<int64_t>(w.ctas, busy));
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(w.ctas);
+  cfg.gridDim = dim3(p.ctas);
   cfg.blockDim = dim3(32 * S::kWarps);
   cfg.dynamicSmemBytes = sizeof(Smem);
   cfg.stream = stream;
@@ -946,13 +1033,15 @@ static int launch(PagedDecodeParams &p, const Layout &w, cudaStream_t stream) {
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
   if (cudaLaunchKernelEx(&cfg, kernel, p) != cudaSuccess) return FPX_ERR_CUDA;
-  cfg.gridDim = dim3((unsigned)w.units, w.rows);
+  if (p.whole) return FPX_OK;
   cfg.dynamicSmemBytes = 0;
-  // Few rows have many pieces each, many rows few: 512 threads read a row's pieces at once (one sequence of
-  // 131072 tokens: merge 7.0 -> 2.5 us against 256), 128 leave room for more rows (batch of 32: 20 -> 10 us).
-  const bool wide = w.units * w.rows <= 2 * kSms;
-  cfg.blockDim = dim3(wide ? 512 : 128);
-  const auto merge = wide ? paged_merge_kernel<D, NT, 512> : paged_merge_kernel<D, NT, 128>;
+  // Few rows have many pieces each, many rows few: a block a row reads them all at once (one sequence of 131072
+  // tokens: 7.0 us with a loop over them, 2.5 with this), a warp a row leaves room for more rows (32 sequences of up
+  // to 32768: 20 us with a block a row, 5 with this).
+  const bool many = w.units * w.rows > 2 * kSms;
+  cfg.gridDim = many ? dim3((unsigned)w.units) : dim3((unsigned)w.units, w.rows);
+  cfg.blockDim = dim3(many ? 256 * NT : 512);
+  const auto merge = many ? paged_merge_rows_kernel<D, NT> : paged_merge_pieces_kernel<D, NT>;
   if (cudaLaunchKernelEx(&cfg, merge, p) != cudaSuccess) return FPX_ERR_CUDA;
   return FPX_OK;
 }
@@ -995,7 +1084,6 @@ extern "C" int fpx_paged_decode_attention(int format, const void *q, int64_t q_s
   p.lse = lse;
   p.B = B; p.Lq = Lq; p.H = H; p.Hkv = Hkv; p.group = H / Hkv; p.blocks = w.blocks;
   p.scale_log2 = (float)scale * kLog2e;
-  p.ctas = w.ctas;
   // 32-bit counts of steps: what the table could name in all
   if ((int64_t)B * w.blocks * Hkv * (((int64_t)max_pages << p.pv.page_shift) + kPad) > 0x7fffffff - (1 << 24))
     return FPX_ERR_UNSUPPORTED;

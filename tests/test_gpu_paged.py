@@ -230,10 +230,19 @@ def test_ragged_batch_with_padding_and_inactive_sequences(form, page):
 
 
 @pytest.mark.parametrize("form", ["int4", "bf16"])
-def test_many_sequences_share_the_launch(form):
-    """More units than CTAs, most of one granule."""
+@pytest.mark.parametrize("longest", [40, 1500])
+def test_many_sequences_share_the_launch(form, longest):
+    """More units than CTAs, most of one granule; with a long table, whose work is split, and a short one."""
     lengths = [1 + (37 * i) % 40 for i in range(333)]
+    lengths[200] = longest
     attend(form, lengths, 1, 8, 4, 128, 16, seed=9)
+
+
+@pytest.mark.parametrize("form", ["int4", "bf16"])
+@pytest.mark.parametrize("dim,heads", [(128, 4), (128, 24), (256, 10)])
+def test_padding_and_inactive_sequences_of_short_tables(form, dim, heads):
+    counts, starts = [3, 2, 0, 1, 3, 2, 1], [97, 0, 100, 0, -1, 22, 32]
+    attend(form, [100, 2, 100, 1, 77, 24, 33], 3, heads, 2, dim, 16, seed=dim, counts=counts, starts=starts)
 
 
 @pytest.mark.parametrize("form,dim,heads,kv_heads", [("int4", 128, 7, 1), ("int4", 256, 16, 4), ("bf16", 128, 5, 1), ("int4", 128, 16, 1)])
