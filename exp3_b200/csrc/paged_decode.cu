@@ -925,19 +925,44 @@ __global__ void __launch_bounds__(256 * NT) paged_merge_rows_kernel(const __grid
   float4 o[D / 128] = {};
   if (sees) {
     const float *ml = p.part_ml + 2 * (u.slot * kRows + r), *po = p.part_o + (u.slot * kRows + r) * D + 4 * lane;
-    for (int i = lane; i < u.pieces; i += 32) m = fmaxf(m, ml[2 * (int64_t)i * kRows]);
-    m = warp_max(m);
-#pragma unroll 4
-    for (int i = 0; i < u.pieces; ++i) {
-      const float2 mine = *reinterpret_cast<const float2 *>(ml + 2 * (int64_t)i * kRows);
-      const float s = tc::ex2(mine.x - m);
-      l = fmaf(mine.y, s, l);
+    constexpr int kAhead = 8;  // pieces whose loads do not wait for the weights
+    for (int i0 = 0; i0 < u.pieces; i0 += 32) {
+      const int here = min(u.pieces - i0, 32);
+      float2 mine = make_float2(kLowest, 0.f);
+      if (lane < here) mine = *reinterpret_cast<const float2 *>(ml + 2 * (int64_t)(i0 + lane) * kRows);
+      float4 x[kAhead][D / 128];
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k)
+#pragma unroll
+        for (int J = 0; J < D / 128; ++J)
+          x[k][J] = k < here ? *reinterpret_cast<const float4 *>(po + (int64_t)(i0 + k) * kRows * D + 128 * J)
+                             : make_float4(0.f, 0.f, 0.f, 0.f);
+      const float top = fmaxf(m, warp_max(mine.x)), keep = tc::ex2(m - top);
+      m = top;
+      const float s = lane < here ? tc::ex2(mine.x - m) : 0.f;
+      l = fmaf(l, keep, mine.y * s);
 #pragma unroll
       for (int J = 0; J < D / 128; ++J) {
-        const float4 x = *reinterpret_cast<const float4 *>(po + (int64_t)i * kRows * D + 128 * J);
-        o[J].x = fmaf(x.x, s, o[J].x); o[J].y = fmaf(x.y, s, o[J].y); o[J].z = fmaf(x.z, s, o[J].z); o[J].w = fmaf(x.w, s, o[J].w);
+        o[J].x *= keep; o[J].y *= keep; o[J].z *= keep; o[J].w *= keep;
+      }
+      auto add = [&](float w, const float4 (&v)[D / 128]) {
+#pragma unroll
+        for (int J = 0; J < D / 128; ++J) {
+          o[J].x = fmaf(v[J].x, w, o[J].x); o[J].y = fmaf(v[J].y, w, o[J].y);
+          o[J].z = fmaf(v[J].z, w, o[J].z); o[J].w = fmaf(v[J].w, w, o[J].w);
+        }
+      };
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) add(__shfl_sync(0xffffffffu, s, k), x[k]);
+#pragma unroll 4
+      for (int i = kAhead; i < here; ++i) {
+        float4 v[D / 128];
+#pragma unroll
+        for (int J = 0; J < D / 128; ++J) v[J] = *reinterpret_cast<const float4 *>(po + (int64_t)(i0 + i) * kRows * D + 128 * J);
+        add(__shfl_sync(0xffffffffu, s, i), v);
       }
     }
+    l = warp_sum(l);
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
   __nv_bfloat16 *out = p.out + u.b * p.o_sb + row * p.o_sl + h * p.o_sh + 4 * lane;
