@@ -552,6 +552,20 @@ FPX_INLINE void gather_store(const GatherRows &o, __nv_bfloat16 *dst, uint4 v) {
   }
 }
 
+// bf16(n - 8) s of a word of eight codes, correctly rounded (both factors are bf16): codes become 128 + n by an
+// and-or of two of them, four dims apart, 136 is taken off exactly, and the products are put back in order.
+FPX_INLINE uint4 scaled8(uint32_t w, __nv_bfloat162 s) {
+  uint32_t p[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t u = ((w >> (4 * i)) & 0x000f000fu) | 0x43004300u;
+    const __nv_bfloat162 x = __hmul2(__hsub2(*reinterpret_cast<const __nv_bfloat162 *>(&u), __floats2bfloat162_rn(136.f, 136.f)), s);
+    p[i] = *reinterpret_cast<const uint32_t *>(&x);
+  }
+  return make_uint4(__byte_perm(p[0], p[1], 0x5410), __byte_perm(p[2], p[3], 0x5410), __byte_perm(p[0], p[1], 0x7632),
+                    __byte_perm(p[2], p[3], 0x7632));
+}
+
 // int4: a lane reads 16 bytes of codes: of keys, its parts of four groups of one token (eight dims each), of values, four dims of four groups
 // of a token pair. Quads and eights of lanes write 64 contiguous bytes.
 template <int D>
@@ -576,11 +590,8 @@ FPX_INLINE void gather_int4(const GatherRows &o, const uint8_t *gran, int lane) 
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const uint32_t u = j < 2 ? sc.x : sc.y;
-        const float s = __uint_as_float(j & 1 ? u & 0xffff0000u : u << 16);
-        float x[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = (float)((int)((words[j] >> (4 * i)) & 15u) - 8) * s;
-        gather_store(o, dst + 32 * j, make_uint4(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7])));
+        const uint32_t s = __byte_perm(u, u, j & 1 ? 0x3232 : 0x1010);
+        gather_store(o, dst + 32 * j, scaled8(words[j], *reinterpret_cast<const __nv_bfloat162 *>(&s)));
       }
     }
   const int vg = lane & 7;
@@ -614,7 +625,8 @@ FPX_INLINE void gather_int4(const GatherRows &o, const uint8_t *gran, int lane) 
           const float s = live ? __half2float(odd ? __high2half(r2) : __low2half(r2)) * up : 0.f;
           float x[4];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) x[i] = live ? (float)((int)((words[j >> 1] >> (16 * (j & 1) + 4 * i)) & 15u) - 8) * s : 0.f;
+          for (int i = 0; i < 4; ++i)  // 2^23 + n in the float's bits
+            x[i] = live ? (__uint_as_float(((words[j >> 1] >> (16 * (j & 1) + 4 * i)) & 15u) | 0x4b000000u) - 8388616.f) * s : 0.f;
           *reinterpret_cast<uint2 *>(dst + 32 * j) = make_uint2(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]));
         }
       }
