@@ -298,6 +298,54 @@ def test_nan_and_infinity_stay_where_they_are(form):
     assert early[1].isfinite().all()
 
 
+@pytest.mark.parametrize("form", ["int4", "bf16"])
+def test_huge_queries_pick_one_key(form):
+    """Logits far apart: the output is the value of the largest, up to the largest bf16 queries. bf16 pages sum q k in
+    fp32 before the scale: 128 products of 2^124 and 1 have a sum of about 2^124 128^0.5 2^2 > 2^128, which fp32 does not
+    hold, so there the sizes end before (int4 brings the query to 2^15 first)."""
+    g = torch.Generator().manual_seed(26)
+    k, v = randn(g, 1, 300, 1, 128), randn(g, 1, 300, 1, 128)
+    q = randn(g, 1, 1, 4, 128)
+    cache = Cache(form, [300], 1, 128, 64)
+    paged.paged_append(k.to(DEV), v.to(DEV), cache.pool, cache.table, ints([0]))
+    kc, vc = cached_values(form, k[0].float(), v[0])
+    best = torch.einsum("hd,td->ht", q[0, 0].double(), kc[:, 0].double()).argmax(-1)
+    for size in (2.0 ** 40, 2.0 ** 100, 2.0 ** 115) + ((2.0 ** 124,) if form == "int4" else ()):
+        out = paged.paged_decode_attention((q * size).to(DEV), cache.pool, cache.table, ints([299]), 1.0 if size < 1e30 else 2.0 ** -20)
+        assert torch.equal(out[0, 0].cpu(), vc[best, 0].to(torch.bfloat16)), size
+
+
+def test_shared_pages_and_output_in_place():
+    """Two sequences with a common prefix in the same pages; the output may be the queries' tensor."""
+    g = torch.Generator().manual_seed(27)
+    k, v = randn(g, 1, 1300, 2, 128).to(DEV), randn(g, 1, 1300, 2, 128).to(DEV)
+    q = randn(g, 2, 2, 8, 128).to(DEV)
+    cache = Cache("int4", [1300], 2, 128, 64)
+    paged.paged_append(k, v, cache.pool, cache.table, ints([0]))
+    both = cache.table.expand(2, -1).contiguous()
+    starts = ints([1298, 640])
+    want = [paged.paged_decode_attention(q[b:b + 1], cache.pool, cache.table, starts[b:b + 1], 0.1) for b in range(2)]
+    assert paged.paged_decode_attention(q, cache.pool, both, starts, 0.1, out=q) is q
+    for b in range(2):
+        torch.testing.assert_close(q[b], want[b][0], rtol=2.0 ** -7, atol=1e-6)  # another split of the keys
+
+
+def test_unseen_rows_of_a_granule_hold_anything():
+    """NaN and infinities stored behind a row's position, in its own granule, do not reach it."""
+    g = torch.Generator().manual_seed(28)
+    k, v, q = randn(g, 1, 64, 1, 128), randn(g, 1, 64, 1, 128), randn(g, 1, 4, 4, 128).to(DEV)
+    for form in ("int4", "bf16"):
+        outs = []
+        for dirty in (False, True):
+            kd, vd = k.clone(), v.clone()
+            if dirty:
+                kd[0, 41:], vd[0, 41:] = math.nan, math.inf
+            cache = Cache(form, [64], 1, 128, 16)
+            paged.paged_append(kd.to(DEV), vd.to(DEV), cache.pool, cache.table, ints([0]))
+            outs.append(paged.paged_decode_attention(q, cache.pool, cache.table, ints([37]), 0.1))
+        assert outs[0].isfinite().all() and torch.equal(*outs)
+
+
 def test_pool_beyond_four_gigabytes():
     """Pages whose byte offsets pass 32 bits."""
     g = torch.Generator().manual_seed(6)
