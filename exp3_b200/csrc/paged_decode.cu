@@ -713,8 +713,9 @@ __global__ void __launch_bounds__(32 * W, OCC) paged_decode_kernel(const __grid_
     if (todo > 0 && !stopped && arrived(get)) {
 #pragma unroll
       for (int h = 0; h < GS; ++h) scores<FMT, D, NT>(y[h], f, ring + get * kBytes + h * G::kBytes, at, lane);
-      for (int i = 0; i + 1 < todo; ++i) {
+      for (int i = 0;; ++i) {
         weigh(i);
+        if (i + 1 == todo) break;
         const int after = get + 1 == ST ? 0 : get + 1;
         if (!arrived(after)) break;
         const uint32_t stage = ring + get * kBytes, next = ring + after * kBytes;
@@ -730,7 +731,6 @@ __global__ void __launch_bounds__(32 * W, OCC) paged_decode_kernel(const __grid_
         }
       }
       if (!stopped) {
-        weigh(todo - 1);
 #pragma unroll
         for (int h = 0; h < GS; ++h) values<FMT, D, NT>(c, pw[h], ring + get * kBytes + h * G::kBytes, at, lane);
         get = get + 1 == ST ? 0 : get + 1;
