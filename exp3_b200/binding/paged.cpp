@@ -7,7 +7,7 @@
 #include <Python.h>
 
 #include <ATen/core/Tensor.h>
-#include <ATen/ops/empty.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -138,7 +138,7 @@ void on_stream(const Device &dev, const char *name, F f) {
   if (rc) refuse(std::string(name) + " failed with status " + std::to_string(rc) + " (" + g_status(rc) + ")");
 }
 at::Tensor empty(at::IntArrayRef shape, const Device &dev, at::ScalarType type) {
-  return at::empty(shape, at::TensorOptions().dtype(type).device(dev.value));
+  return at::detail::empty_cuda(shape, type, dev.value, c10::nullopt);
 }
 
 // paged_decode_attention(q, pool, page_table, starts, scale, counts, out, lse, ws)

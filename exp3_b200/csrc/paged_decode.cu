@@ -43,7 +43,7 @@ struct PagedDecodeParams {
   float scale_log2;
   int ctas, min_steps;
   bool whole;      // a CTA a unit, no merge
-  int *prefix;     // [B * blocks + 1] steps of all heads before an item (b, row block)
+  int *prefix;     // [B * blocks + 1] steps of all heads before an item (b, row block), with more than 32 items
   float *part_o;   // [ctas + units][8 NT][d]
   float *part_ml;  // [ctas + units][8 NT][2]
 };
@@ -71,6 +71,28 @@ FPX_INLINE int steps_of(int keys) { return (keys + GS * kGranule - 1) / (GS * kG
 // (queries, first copies, merge) in steps.
 constexpr int kPad = 4;
 FPX_INLINE int padded(int steps) { return steps ? steps + kPad : 0; }
+
+// What item i (sequence, row block) counts in the partition, all heads together.
+template <int NT, int GS>
+FPX_INLINE int item_steps(const PagedDecodeParams &p, int i) {
+  const int b = i / p.blocks;
+  int start, count;
+  p.pv.rows(b, p.Lq, start, count);
+  return padded(steps_of<GS>(item_keys<NT>(p, start, count, i - b * p.blocks))) * p.Hkv;
+}
+// Up to 32 items: lane i's steps before its item and of it, and all of them. Every warp does it for itself.
+template <int NT, int GS>
+FPX_INLINE void lane_items(const PagedDecodeParams &p, int items, int lane, int &before, int &mine, int &total) {
+  mine = lane < items ? item_steps<NT, GS>(p, lane) : 0;
+  before = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int x = __shfl_up_sync(0xffffffffu, before, o);
+    if (lane >= o) before += x;
+  }
+  total = __shfl_sync(0xffffffffu, before, 31);
+  before -= mine;
+}
 
 FPX_INLINE uint32_t and_or(uint32_t a, uint32_t b, uint32_t c) {
   uint32_t d;
@@ -459,22 +481,27 @@ __global__ void __launch_bounds__(32 * W, OCC) paged_decode_kernel(const __grid_
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
+  // This CTA's run of steps, and the item that it starts in.
   int lo = 0, hi = 0, item = 0, base = 0;
+  auto run = [&](int total) {
+    const int per = max(p.min_steps, (total + p.ctas - 1) / p.ctas);
+    lo = (int)min((int64_t)blockIdx.x * per, (int64_t)total);
+    hi = min(total, lo + per);
+    return lo < hi;
+  };
   if (p.whole) {
     item = blockIdx.x / p.Hkv;
-    __syncthreads();  // the barriers
+  } else if (items <= 32) {
+    int before, mine, total;
+    lane_items<NT, GS>(p, items, lane, before, mine, total);
+    if (!run(total)) return;
+    item = __ffs(__ballot_sync(0xffffffffu, before <= lo && lo < before + mine)) - 1;
+    base = __shfl_sync(0xffffffffu, before, item);
   } else {
-    // This CTA's run of steps, and the item that it starts in.
     const int chunk = (items + kThreads - 1) / kThreads;
     const int i0 = min(items, tid * chunk), i1 = min(items, i0 + chunk);
-    auto steps_in = [&](int i) {
-      const int b = i / p.blocks;
-      int start, count;
-      p.pv.rows(b, p.Lq, start, count);
-      return padded(steps_of<GS>(item_keys<NT>(p, start, count, i - b * p.blocks))) * p.Hkv;
-    };
     int mine = 0;
-    for (int i = i0; i < i1; ++i) mine += steps_in(i);
+    for (int i = i0; i < i1; ++i) mine += item_steps<NT, GS>(p, i);
     int before = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -494,18 +521,15 @@ __global__ void __launch_bounds__(32 * W, OCC) paged_decode_kernel(const __grid_
       int at = before;
       for (int i = i0; i < i1; ++i) {
         p.prefix[i] = at;
-        at += chunk == 1 ? mine : steps_in(i);
+        at += chunk == 1 ? mine : item_steps<NT, GS>(p, i);
       }
       if (tid == 0) p.prefix[items] = total;
     }
-    const int per = max(p.min_steps, (total + p.ctas - 1) / p.ctas);
-    lo = (int)min((int64_t)blockIdx.x * per, (int64_t)total);
-    hi = min(total, lo + per);
-    if (lo >= hi) return;
+    if (!run(total)) return;
     if (before <= lo && lo < before + mine) {
       int at = before;
       for (int i = i0; i < i1; ++i) {
-        const int n = chunk == 1 ? mine : steps_in(i);
+        const int n = chunk == 1 ? mine : item_steps<NT, GS>(p, i);
         if (lo < at + n) {
           sh.item = i;
           sh.base = at;
@@ -518,6 +542,7 @@ __global__ void __launch_bounds__(32 * W, OCC) paged_decode_kernel(const __grid_
     item = sh.item;
     base = sh.base;
   }
+  __syncthreads();  // the ring's barriers are set
 
   const Lane<FMT, D> at(lane);
   uint8_t *const ring_bytes = sh.ring(warp);
@@ -821,21 +846,36 @@ __global__ void __launch_bounds__(32 * W, OCC) paged_decode_kernel(const __grid_
 
 // What the merge launches know of a unit: its pieces lie in slots slot .. slot + pieces - 1 (one piece: its CTA has
 // finished it; none: no row of it sees anything).
+//
+// With up to 32 items they work it out from the lengths, before they wait for the main launch (whose CTAs have all waited for
+// what came before them by then, so the lengths are there); otherwise from the sums that it left, after.
 struct Pieces {
   int b, rb, kvh, rows, pieces;
   int64_t slot;
-  FPX_INLINE Pieces(const PagedDecodeParams &p, int unit) {
-    const int item = unit / p.Hkv;
+  template <int NT, int GS>
+  FPX_INLINE void find(const PagedDecodeParams &p, int unit, int lane) {
+    const int items = p.B * p.blocks, item = unit / p.Hkv;
     kvh = unit - item * p.Hkv;
     b = item / p.blocks;
     rb = item - b * p.blocks;
-    const int base = p.prefix[item], next = p.prefix[item + 1], total = p.prefix[p.B * p.blocks];
+    int base, n, total;
+    if (items <= 32) {
+      int before, mine;
+      lane_items<NT, GS>(p, items, lane, before, mine, total);
+      base = __shfl_sync(0xffffffffu, before, item);
+      n = __shfl_sync(0xffffffffu, mine, item) / p.Hkv;
+      asm volatile("griddepcontrol.wait;" ::: "memory");
+    } else {
+      asm volatile("griddepcontrol.wait;" ::: "memory");
+      base = p.prefix[item];
+      n = (p.prefix[item + 1] - base) / p.Hkv;
+      total = p.prefix[items];
+    }
     int start, count;
     p.pv.rows(b, p.Lq, start, count);
     rows = count * p.group;
-    const int n = (next - base) / p.Hkv;  // padding, then steps
     const int per = max(p.min_steps, (total + p.ctas - 1) / p.ctas);
-    const int first = base + kvh * n, c0 = (first + kPad) / per, c1 = (first + n - 1) / per;
+    const int first = base + kvh * n, c0 = (first + kPad) / per, c1 = (first + n - 1) / per;  // padding, then steps
     pieces = n ? c1 - c0 + 1 : 0;
     slot = c0 + (int64_t)item * p.Hkv + kvh;
   }
@@ -844,16 +884,16 @@ struct Pieces {
 // Merges the pieces of one (unit, row), where rows are few and pieces many: D / 4 threads a piece, kPieces of them at a
 // time, kAhead loads in flight before the weights are known. Rows that see nothing (padding, inactive sequences)
 // become zero here.
-template <int D, int NT>
+template <int D, int NT, int GS>
 __global__ void __launch_bounds__(512) paged_merge_pieces_kernel(const __grid_constant__ PagedDecodeParams p) {
   constexpr int kThreads = 512, kPieces = kThreads / (D / 4), kRows = 8 * NT, kAhead = 10;
   const int r = blockIdx.y, tid = threadIdx.x, piece = tid / (D / 4), d = 4 * (tid % (D / 4));
   __shared__ float red[kThreads / 32];
   __shared__ __align__(16) float part[kPieces][D];
   __shared__ float weight[kThreads];
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  Pieces u;
+  u.find<NT, GS>(p, blockIdx.x, tid & 31);
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const Pieces u(p, blockIdx.x);
   const int rr = u.rb * kRows + r, row = rr / p.group, h = u.kvh * p.group + rr % p.group;
   if (rr >= p.Lq * p.group) return;
   __nv_bfloat16 *out = p.out + u.b * p.o_sb + row * p.o_sl + h * p.o_sh;
@@ -912,13 +952,13 @@ __global__ void __launch_bounds__(512) paged_merge_pieces_kernel(const __grid_co
 }
 
 // The same where units are many and pieces few: a block a unit, a warp a row, D / 32 dims a lane.
-template <int D, int NT>
+template <int D, int NT, int GS>
 __global__ void __launch_bounds__(256 * NT) paged_merge_rows_kernel(const __grid_constant__ PagedDecodeParams p) {
   constexpr int kRows = 8 * NT;
   const int r = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  Pieces u;
+  u.find<NT, GS>(p, blockIdx.x, lane);
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const Pieces u(p, blockIdx.x);
   const int rr = u.rb * kRows + r, row = rr / p.group, h = u.kvh * p.group + rr % p.group;
   const bool sees = rr < u.rows && u.pieces > 0;
   if (rr >= p.Lq * p.group || (sees && u.pieces == 1)) return;
@@ -1067,7 +1107,7 @@ static int launch(PagedDecodeParams &p, const Layout &w, cudaStream_t stream) {
   const bool many = w.units * w.rows > 2 * kSms;
   cfg.gridDim = many ? dim3((unsigned)w.units) : dim3((unsigned)w.units, w.rows);
   cfg.blockDim = dim3(many ? 256 * NT : 512);
-  const auto merge = many ? paged_merge_rows_kernel<D, NT> : paged_merge_pieces_kernel<D, NT>;
+  const auto merge = many ? paged_merge_rows_kernel<D, NT, S::kGranules> : paged_merge_pieces_kernel<D, NT, S::kGranules>;
   if (cudaLaunchKernelEx(&cfg, merge, p) != cudaSuccess) return FPX_ERR_CUDA;
   return FPX_OK;
 }
