@@ -165,14 +165,19 @@ PyObject *decode(PyObject *const *a) {
     refuse("lse must be a contiguous fp32 [B, Lq, H]");
   if (B && L) {
     at::Tensor scratch;
-    if (!ws) {
-      scratch = empty({(int64_t)g_workspace(w.format, to_int(B), to_int(L), to_int(H), w.heads, w.dim)}, dev, at::kByte);
-      ws = &scratch;
-    }
     on_stream(dev, "fpx_paged_decode_attention", [&](fpx_stream_t stream) {
-      return g_decode(w.format, qr.data, qr.b, qr.l, qr.h, to_int(B), to_int(L), to_int(H), w.heads, w.dim, scale, w.pool, w.pages,
-                      w.page_size, w.table, w.stride, w.max_pages, w.starts, w.counts, o.data, o.b, o.l, o.h,
-                      lse ? static_cast<float *>(lse->data_ptr()) : nullptr, ws->data_ptr(), (size_t)ws->nbytes(), stream);
+      const auto call = [&](const at::Tensor *space) {
+        return g_decode(w.format, qr.data, qr.b, qr.l, qr.h, to_int(B), to_int(L), to_int(H), w.heads, w.dim, scale, w.pool, w.pages,
+                        w.page_size, w.table, w.stride, w.max_pages, w.starts, w.counts, o.data, o.b, o.l, o.h,
+                        lse ? static_cast<float *>(lse->data_ptr()) : nullptr, space ? space->data_ptr() : nullptr,
+                        space ? (size_t)space->nbytes() : 0, stream);
+      };
+      int rc = call(ws);  // short tables need no workspace: without one the call says so before it does anything
+      if (rc == FPX_ERR_WORKSPACE && !ws) {
+        scratch = empty({(int64_t)g_workspace(w.format, to_int(B), to_int(L), to_int(H), w.heads, w.dim)}, dev, at::kByte);
+        rc = call(&scratch);
+      }
+      return rc;
     });
   }
   return made.defined() ? THPVariable_Wrap(made) : Py_NewRef(a[6]);

@@ -1061,7 +1061,13 @@ static Layout layout_of(int format, int B, int Lq, int H, int Hkv, int d) {
   return w;
 }
 
-constexpr int kWholeTokens = 512, kWholeUnits = 32;
+// Short tables: a CTA a unit, one launch and no workspace. Four KV heads, us in one launch / in two, int4: 1 sequence of 256
+// tokens 5.6 / 8.2, 512 7.4 / 8.4, 1024 10.8 / 8.4; 37 sequences 6.7 / 11.1, 8.4 / 16.2, 11.8 / 14.0; bf16: 5.5 / 7.5, 7.4 /
+// 7.7, 11.0 / 7.5 and 5.8 / 9.6, 9.7 / 13.3, 15.7 / 19.4.
+static bool whole_units(const PageView &pv, int64_t units) {
+  const int64_t tokens = ((int64_t)pv.max_pages << pv.page_shift) * kGranule;
+  return tokens <= (units >= 32 ? 1024 : 512);
+}
 
 template <int FMT, int D, int NT>
 static int launch(PagedDecodeParams &p, const Layout &w, cudaStream_t stream) {
@@ -1080,12 +1086,8 @@ static int launch(PagedDecodeParams &p, const Layout &w, cudaStream_t stream) {
     set.fetch_or(bit, std::memory_order_relaxed);
   }
   p.min_steps = S::kWarps;
-  // Short tables: a CTA a unit and one launch. Otherwise no more CTAs than the table could keep busy. Four KV heads,
-  // int4, us in one launch / in two: 1 sequence of 256 tokens 5.6 / 8.2, 512 7.4 / 8.4, 1024 10.8 / 8.4; 37 sequences 6.7 /
-  // 11.1, 8.4 / 16.2, 11.8 / 14.0; bf16: 5.5 / 7.5, 7.4 / 7.7, 11.0 / 7.5 and 5.8 / 9.6, 9.7 / 13.3, 15.7 / 19.4.
+  // No more CTAs than the table could keep busy.
   const int64_t longest = ((int64_t)p.pv.max_pages << p.pv.page_shift) / S::kGranules + 1;  // steps
-  const int64_t tokens = ((int64_t)p.pv.max_pages << p.pv.page_shift) * kGranule;
-  p.whole = tokens <= (w.units >= kWholeUnits ? 2 * kWholeTokens : kWholeTokens);
   const int64_t busy = w.units * (longest + kPad) / p.min_steps + 1;
   p.ctas = (int)(p.whole ? w.units : std::min<int64_t>(w.ctas, busy));
   cudaLaunchConfig_t cfg{};
@@ -1144,7 +1146,9 @@ extern "C" int fpx_paged_decode_attention(int format, const void *q, int64_t q_s
   const RowStrides qs(q_sb, q_sl, q_sh, B, Lq, H);
   if ((reinterpret_cast<uintptr_t>(q) & 15) || !qs.multiples_of(8)) return FPX_ERR_SHAPE;
   const Layout w = layout_of(format, B, Lq, H, Hkv, d);
-  if (!workspace || workspace_bytes < w.bytes || (reinterpret_cast<uintptr_t>(workspace) & 15)) return FPX_ERR_WORKSPACE;
+  p.whole = whole_units(p.pv, w.units);
+  if (!p.whole && (!workspace || workspace_bytes < w.bytes || (reinterpret_cast<uintptr_t>(workspace) & 15)))
+    return FPX_ERR_WORKSPACE;
   p.q = static_cast<const __nv_bfloat16 *>(q); p.q_sb = qs.b; p.q_sl = qs.l; p.q_sh = qs.h;
   p.out = static_cast<__nv_bfloat16 *>(out); p.o_sb = o_sb; p.o_sl = o_sl; p.o_sh = o_sh;
   p.lse = lse;

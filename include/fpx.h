@@ -354,7 +354,8 @@ int fpx_paged_gather(int format, const void *pool, int pages, int page_size, con
  * row sees positions 0 .. its own, which fpx_paged_append has stored. Lq <= 64, H / Hkv <= 16,
  * B * Lq * H <= 2^24. out bf16 with element strides, lse fp32 [B, Lq, H] natural log or NULL;
  * padding rows give 0 and -inf. Bytes of workspace do not depend on the sequences' lengths; it
- * needs no initial value, and two calls that may overlap need two. */
+ * needs no initial value, and two calls that may overlap need two. Tables of up to 512 tokens
+ * (max_pages * page_size) need none: NULL. */
 size_t fpx_paged_decode_workspace_bytes(int format, int B, int Lq, int H, int Hkv, int d);
 int fpx_paged_decode_attention(int format, const void *q, int64_t q_sb, int64_t q_sl, int64_t q_sh, int B, int Lq,
                                int H, int Hkv, int d, double scale, const void *pool, int pages, int page_size,
