@@ -526,5 +526,5 @@ extern "C" int fpx_device_error(int *code, int reset) {
     const int zero = 0;
     if (cudaMemcpyToSymbol(fpx::g_device_error, &zero, sizeof(int)) != cudaSuccess) return FPX_ERR_CUDA;
   }
-  return FPX_OK;
+  return *code ? FPX_OK : fpx::read_bad_index(code, reset);  // a bad index beside it is kept for the next call
 }

@@ -63,7 +63,8 @@ struct PageView {
   int64_t table_stride;
   int max_pages;
   const int32_t *starts, *counts;  // [B]; counts may be null: every row counts
-  int *error;                      // fpx_device_error's word, or null
+  int *bad_index;                  // set where one of these names nothing; apart from the word of waits that gave up, whose
+                                   // value other kernels take as a reason not to run. Null: not reported
 
   FPX_INLINE int capacity() const { return (int)min((int64_t)max_pages << (page_shift + 4), (int64_t)0x7fffffff); }
   // Rows of sequence b that are no padding.
@@ -78,7 +79,7 @@ struct PageView {
     count = start < 0 ? 0 : max(0, min(c, L));
   }
   FPX_INLINE void fail() const {
-    if (error) atomicMax(error, FPX_DEVICE_BAD_INDEX);
+    if (bad_index) *bad_index = FPX_DEVICE_BAD_INDEX;
   }
 };
 

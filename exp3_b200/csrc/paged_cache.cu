@@ -1,6 +1,7 @@
 // Writing and reading back the paged KV cache: append (rotary embedding on the way, 4-bit
 // quantisation for int4 pages) and gather. Page layout: paged.cuh.
 #include <algorithm>
+#include <atomic>
 
 #include "paged.cuh"
 #include "tc.cuh"
@@ -716,6 +717,29 @@ static int launch_dependent(K kernel, dim3 grid, cudaStream_t stream, A... args)
   return cudaLaunchKernelEx(&cfg, kernel, args...) == cudaSuccess ? FPX_OK : FPX_ERR_CUDA;
 }
 
+static __device__ int g_bad_index;
+
+// Its address on the current device, looked up once for each.
+static int *bad_index_word() {
+  static std::atomic<int *> cache[64];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return nullptr;
+  int *word = cache[dev].load(std::memory_order_relaxed);
+  if (!word) {
+    void *ptr = nullptr;
+    if (cudaGetSymbolAddress(&ptr, g_bad_index) != cudaSuccess) return nullptr;
+    cache[dev].store(word = static_cast<int *>(ptr), std::memory_order_relaxed);
+  }
+  return word;
+}
+
+int read_bad_index(int *code, int reset) {
+  if (cudaMemcpyFromSymbol(code, g_bad_index, sizeof(int)) != cudaSuccess) return FPX_ERR_CUDA;
+  const int zero = 0;
+  if (reset && cudaMemcpyToSymbol(g_bad_index, &zero, sizeof(int)) != cudaSuccess) return FPX_ERR_CUDA;
+  return FPX_OK;
+}
+
 int make_page_view(PageView *view, int format, const void *pool, int pages, int page_size, const int32_t *table,
                    int64_t table_stride, int max_pages, const int32_t *starts, const int32_t *counts, int Hkv, int d) {
   if (format != FPX_PAGES_BF16 && format != FPX_PAGES_INT4) return FPX_ERR_INVALID;
@@ -734,7 +758,7 @@ int make_page_view(PageView *view, int format, const void *pool, int pages, int 
   view->max_pages = max_pages;
   view->starts = starts;
   view->counts = counts;
-  view->error = device_error_word();
+  view->bad_index = bad_index_word();
   return FPX_OK;
 }
 

@@ -34,6 +34,7 @@ namespace fpx {
 
 struct PagedDecodeParams {
   PageView pv;
+  int *error;  // the word of waits that gave up, or null
   const __nv_bfloat16 *q;
   int64_t q_sb, q_sl, q_sh;
   __nv_bfloat16 *out;
@@ -626,7 +627,7 @@ __global__ void __launch_bounds__(32 * W, OCC) paged_decode_kernel(const __grid_
   auto arrived = [&](int stage) {  // the copy that was put there last
     if (!tc::mbar_wait_warp(&sh.full[warp][stage], (phase >> stage) & 1, &sh.abort)) {
       stopped = true;  // it did not arrive: report it and let the launch end
-      if (lane == 0 && p.pv.error) atomicMax(p.pv.error, FPX_DEVICE_WAIT);
+      if (lane == 0 && p.error) atomicMax(p.error, FPX_DEVICE_WAIT);
       return false;
     }
     phase ^= 1u << stage;
@@ -1152,6 +1153,7 @@ extern "C" int fpx_paged_decode_attention(int format, const void *q, int64_t q_s
   p.q = static_cast<const __nv_bfloat16 *>(q); p.q_sb = qs.b; p.q_sl = qs.l; p.q_sh = qs.h;
   p.out = static_cast<__nv_bfloat16 *>(out); p.o_sb = o_sb; p.o_sl = o_sl; p.o_sh = o_sh;
   p.lse = lse;
+  p.error = device_error_word();
   p.B = B; p.Lq = Lq; p.H = H; p.Hkv = Hkv; p.group = H / Hkv; p.blocks = w.blocks;
   p.scale_log2 = (float)scale * kLog2e;
   // 32-bit counts of steps: what the table could name in all

@@ -279,5 +279,7 @@ bool encode_4d(CUtensorMap *map, const void *base, int64_t d, int64_t heads, int
 // Device address of the library's error word (fpx_device_error) on the current device, for
 // kernels in other translation units; null if the runtime cannot resolve it.
 int *device_error_word();
+// The other word that fpx_device_error reads: FPX_DEVICE_BAD_INDEX or 0 (paged_cache.cu). An fpx_status.
+int read_bad_index(int *code, int reset);
 
 }  // namespace fpx

@@ -91,9 +91,9 @@ int fpx_version(void);
  * bf16 high + low halves, two passes (default), 1 = fp32 CUDA cores (cross-check). */
 int fpx_set_option(int key, int value);
 
-/* Reads (and with reset != 0 clears) the device error word: an fpx_device_code, the highest that
- * was set (a bounded wait inside a kernel gave up, or an index in device memory named nothing);
- * synchronous. No reference counterpart. */
+/* Reads (and with reset != 0 clears) the device error: an fpx_device_code (a bounded wait inside a
+ * kernel gave up, or an index in device memory named nothing). Where both happened the first call
+ * reports and clears the wait, the next one the index; synchronous. No reference counterpart. */
 int fpx_device_error(int *code, int reset);
 
 /* ---- routing ------------------------------------------------------------------------ */

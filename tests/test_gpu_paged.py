@@ -404,6 +404,19 @@ def test_positions_past_the_table_write_nothing():
     assert (out[0, 10:] == 0).all()
 
 
+def test_a_bad_index_does_not_stop_other_kernels():
+    """The report of a missing page leaves the prefill kernels, which stop after a wait that gave up, at work."""
+    from exp3_b200 import ops
+    g = torch.Generator().manual_seed(29)
+    q, k = randn(g, 1, 300, 4, 128).to(DEV), randn(g, 1, 300, 2, 128).to(DEV)
+    want = ops.prefill_attention(q, k, k, "fp_v1_rescue", 0.08, 0.088)
+    cache = Cache("int4", [40], 2, 128, 16)
+    paged.paged_append(k[:, :40], k[:, :40], cache.pool, torch.full_like(cache.table, -1), ints([0]))
+    got = ops.prefill_attention(q, k, k, "fp_v1_rescue", 0.08, 0.088, out=torch.zeros_like(q))
+    assert torch.equal(got, want)
+    assert _capi.device_error() == 2
+
+
 def test_results_do_not_depend_on_timing():
     cache, q, out, lse, starts, counts, _ = attend("int4", [5000, 3000, 20], 1, 28, 4, 128, 64, seed=14)
     for _ in range(5):
