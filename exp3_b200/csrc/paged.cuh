@@ -66,7 +66,8 @@ struct PageView {
   int *bad_index;                  // set where one of these names nothing; apart from the word of waits that gave up, whose
                                    // value other kernels take as a reason not to run. Null: not reported
 
-  FPX_INLINE int capacity() const { return (int)min((int64_t)max_pages << (page_shift + 4), (int64_t)0x7fffffff); }
+  // Positions that the table holds; a tile's end stays below 2^31.
+  FPX_INLINE int capacity() const { return (int)min((int64_t)max_pages << (page_shift + 4), (int64_t)0x7fffff80); }
   // Rows of sequence b that are no padding.
   FPX_INLINE int count(int b, int L) const {
     if (starts[b] < 0) return 0;

@@ -24,82 +24,10 @@
 // ring of bulk copies (no barrier between warps inside a unit). A unit inside one CTA is
 // finished there; the pieces of the others are merged in CTA order by the second launch, so
 // results do not depend on timing.
-#include <algorithm>
-#include <atomic>
-
-#include "paged.cuh"
-#include "tc.cuh"
+#include "paged_decode.cuh"
 
 namespace fpx {
 
-struct PagedDecodeParams {
-  PageView pv;
-  int *error;  // the word of waits that gave up, or null
-  const __nv_bfloat16 *q;
-  int64_t q_sb, q_sl, q_sh;
-  __nv_bfloat16 *out;
-  int64_t o_sb, o_sl, o_sh;
-  float *lse;  // [B][Lq][H] or null
-  int B, Lq, H, Hkv, group, blocks;  // blocks: row blocks of 8 NT (query row, head of the group) pairs
-  float scale_log2;
-  int ctas, min_steps;
-  bool whole;      // a CTA a unit, no merge
-  int *prefix;     // [B * blocks + 1] steps of all heads before an item (b, row block), with more than 32 items
-  float *part_o;   // [ctas + units][8 NT][d]
-  float *part_ml;  // [ctas + units][8 NT][2]
-};
-
-constexpr float kRaise = 8.f;      // the running reference follows when a logit passes it by this (log2)
-constexpr float kLowest = -3e38f;  // reference before any logit: below all of them, and finite
-
-// Keys that row block rb of sequence b needs: all up to its last row's position.
-template <int NT>
-FPX_INLINE int item_keys(const PagedDecodeParams &p, int start, int count, int rb) {
-  const int first = rb * 8 * NT;
-  if (first >= count * p.group) return 0;
-  const int last = min(count * p.group, first + 8 * NT) - 1;
-  const int64_t keys = (int64_t)start + last / p.group + 1;
-  if (keys > p.pv.capacity()) {
-    p.pv.fail();
-    return p.pv.capacity();
-  }
-  return (int)keys;
-}
-// A step is the GS granules of one ring stage.
-template <int GS>
-FPX_INLINE int steps_of(int keys) { return (keys + GS * kGranule - 1) / (GS * kGranule); }
-// What a unit counts in the partition: its steps and, in front of them, what beginning a unit costs a CTA
-// (queries, first copies, merge) in steps.
-constexpr int kPad = 4;
-FPX_INLINE int padded(int steps) { return steps ? steps + kPad : 0; }
-
-// What item i (sequence, row block) counts in the partition, all heads together.
-template <int NT, int GS>
-FPX_INLINE int item_steps(const PagedDecodeParams &p, int i) {
-  const int b = i / p.blocks;
-  int start, count;
-  p.pv.rows(b, p.Lq, start, count);
-  return padded(steps_of<GS>(item_keys<NT>(p, start, count, i - b * p.blocks))) * p.Hkv;
-}
-// Up to 32 items: lane i's steps before its item and of it, and all of them. Every warp does it for itself.
-template <int NT, int GS>
-FPX_INLINE void lane_items(const PagedDecodeParams &p, int items, int lane, int &before, int &mine, int &total) {
-  mine = lane < items ? item_steps<NT, GS>(p, lane) : 0;
-  before = mine;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int x = __shfl_up_sync(0xffffffffu, before, o);
-    if (lane >= o) before += x;
-  }
-  total = __shfl_sync(0xffffffffu, before, 31);
-  before -= mine;
-}
-
-FPX_INLINE uint32_t and_or(uint32_t a, uint32_t b, uint32_t c) {
-  uint32_t d;
-  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
-  return d;
-}
 FPX_INLINE uint32_t transpose8(uint32_t a) {  // 8 x 8 16-bit matrix, one row of pairs a quad
   uint32_t d;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
@@ -121,50 +49,6 @@ FPX_INLINE void mma_f16_first(float (&d)[4], const uint32_t (&a)[4], uint32_t b0
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
 }
-FPX_INLINE uint32_t hmul2u(uint32_t a, uint32_t b) {
-  __half2 r = __hmul2(*reinterpret_cast<__half2 *>(&a), *reinterpret_cast<__half2 *>(&b));
-  return *reinterpret_cast<uint32_t *>(&r);
-}
-FPX_INLINE uint32_t hsub2u(uint32_t a, uint32_t b) {
-  __half2 r = __hsub2(*reinterpret_cast<__half2 *>(&a), *reinterpret_cast<__half2 *>(&b));
-  return *reinterpret_cast<uint32_t *>(&r);
-}
-FPX_INLINE uint32_t hfma2u(uint32_t a, uint32_t b, uint32_t c) {
-  __half2 r = __hfma2(*reinterpret_cast<__half2 *>(&a), *reinterpret_cast<__half2 *>(&b), *reinterpret_cast<__half2 *>(&c));
-  return *reinterpret_cast<uint32_t *>(&r);
-}
-FPX_INLINE uint32_t pack_f16(float lo, float hi) {
-  __half2 v = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<uint32_t *>(&v);
-}
-FPX_INLINE float ex2_neg(float x) {  // 2^-x
-  float y;
-  asm("{\n\t.reg .f32 t;\n\tneg.f32 t, %1;\n\tex2.approx.ftz.f32 %0, t;\n\t}\n" : "=f"(y) : "f"(x));
-  return y;
-}
-// Loads from a shared-memory address (the granules arrive by bulk copies: ordered by the barrier's wait).
-FPX_INLINE uint4 lds128(uint32_t a) {
-  uint4 v;
-  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
-  return v;
-}
-FPX_INLINE uint2 lds64(uint32_t a) {
-  uint2 v;
-  asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a) : "memory");
-  return v;
-}
-FPX_INLINE uint32_t lds16(uint32_t a) {
-  uint32_t v;
-  asm volatile("ld.shared.u16 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
-  return v;
-}
-FPX_INLINE void bulk_load(void *dst, const void *src, uint32_t bytes, uint64_t *bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
-                   smem_u32(dst)),
-               "l"(src), "r"(bytes), "r"(smem_u32(bar))
-               : "memory");
-}
-
 // Shared memory of a CTA. The merge of its warps has memory of its own where that leaves as many CTAs
 // on an SM (int4 pages): the next unit's first copies are then under way while a unit is merged.
 template <int FMT, int D, int NT, int GS, int W, int ST>
@@ -177,8 +61,8 @@ struct PagedSmem {
   static constexpr int kRing = W * ST * GS * Granule<FMT, D>::kBytes;
   alignas(128) uint8_t memory[kApart ? kRing + sizeof(Merge) : kRing > sizeof(Merge) ? kRing : sizeof(Merge)];
   uint64_t full[W][ST];
-  int scan[W];
-  int item, base, abort;
+  Scan<W> scan;
+  int abort;
   FPX_INLINE uint8_t *ring(int warp) { return memory + warp * (kRing / W); }
   FPX_INLINE Merge &merge() { return *reinterpret_cast<Merge *>(memory + (kApart ? kRing : 0)); }
 };
@@ -475,109 +359,22 @@ __global__ void __launch_bounds__(32 * W, OCC) paged_decode_kernel(const __grid_
   extern __shared__ __align__(128) uint8_t smem_raw[];
   Smem &sh = *reinterpret_cast<Smem *>(smem_raw);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-  const int items = p.B * p.blocks;
   if (lane < ST) tc::mbar_init(&sh.full[warp][lane], 1);
   if (tid == 0) sh.abort = 0;
   tc::fence_barrier_init();
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
-  // This CTA's run of steps, and the item that it starts in.
-  int lo = 0, hi = 0, item = 0, base = 0;
-  auto run = [&](int total) {
-    const int per = max(p.min_steps, (total + p.ctas - 1) / p.ctas);
-    lo = (int)min((int64_t)blockIdx.x * per, (int64_t)total);
-    hi = min(total, lo + per);
-    return lo < hi;
-  };
-  if (p.whole) {
-    item = blockIdx.x / p.Hkv;
-  } else if (items <= 32) {
-    int before, mine, total;
-    lane_items<NT, GS>(p, items, lane, before, mine, total);
-    if (!run(total)) return;
-    item = __ffs(__ballot_sync(0xffffffffu, before <= lo && lo < before + mine)) - 1;
-    base = __shfl_sync(0xffffffffu, before, item);
-  } else {
-    const int chunk = (items + kThreads - 1) / kThreads;
-    const int i0 = min(items, tid * chunk), i1 = min(items, i0 + chunk);
-    int mine = 0;
-    for (int i = i0; i < i1; ++i) mine += item_steps<NT, GS>(p, i);
-    int before = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int x = __shfl_up_sync(0xffffffffu, before, o);
-      if (lane >= o) before += x;
-    }
-    if (lane == 31) sh.scan[warp] = before;
-    before -= mine;
-    __syncthreads();
-    int total = 0;
-#pragma unroll
-    for (int w = 0; w < W; ++w) {
-      if (w < warp) before += sh.scan[w];
-      total += sh.scan[w];
-    }
-    if (blockIdx.x == 0) {  // for the merge
-      int at = before;
-      for (int i = i0; i < i1; ++i) {
-        p.prefix[i] = at;
-        at += chunk == 1 ? mine : item_steps<NT, GS>(p, i);
-      }
-      if (tid == 0) p.prefix[items] = total;
-    }
-    if (!run(total)) return;
-    if (before <= lo && lo < before + mine) {
-      int at = before;
-      for (int i = i0; i < i1; ++i) {
-        const int n = chunk == 1 ? mine : item_steps<NT, GS>(p, i);
-        if (lo < at + n) {
-          sh.item = i;
-          sh.base = at;
-          break;
-        }
-        at += n;
-      }
-    }
-    __syncthreads();
-    item = sh.item;
-    base = sh.base;
-  }
+  Walk<NT, GS> u;
+  if (!u.begin(p, sh.scan, tid)) return;
   __syncthreads();  // the ring's barriers are set
 
   const Lane<FMT, D> at(lane);
   uint8_t *const ring_bytes = sh.ring(warp);
   const uint32_t ring = smem_u32(ring_bytes);
 
-  // The part of a unit that this CTA works on: steps g0 .. g1 - 1 of n_steps. lo is its place in the partition.
-  int b, rb, kvh, start, rows, seen, n_steps, g0, g1;
-  auto read_item = [&]() {
-    b = item / p.blocks;
-    rb = item - b * p.blocks;
-    int count;
-    p.pv.rows(b, p.Lq, start, count);
-    rows = count * p.group;
-    seen = item_keys<NT>(p, start, count, rb);
-    n_steps = steps_of<GS>(seen);
-  };
-  auto find = [&]() {  // the next part from lo on; false: none is left
-    while (lo < hi) {
-      for (;;) {
-        read_item();
-        if (lo - base < padded(n_steps) * p.Hkv) break;
-        base += padded(n_steps) * p.Hkv;
-        ++item;
-      }
-      kvh = (lo - base) / (n_steps + kPad);
-      const int first = base + kvh * (n_steps + kPad) + kPad;  // the unit's first step
-      g0 = max(0, lo - first);
-      g1 = min(n_steps, hi - first);
-      lo = first + max(g1, 0);  // hi, or the unit's end
-      if (g1 > g0) return true;
-    }
-    return false;
-  };
-
+  int &b = u.b, &rb = u.rb, &kvh = u.kvh, &start = u.start, &rows = u.rows, &seen = u.seen, &n_steps = u.n_steps, &g0 = u.g0,
+      &g1 = u.g1, &item = u.item;
   // Ring: step g0 + warp + W i of the part goes into the next stage. A lane works out where one of the
   // next 32 steps lies (16 where each granule has a page of its own).
   const bool paired = GS == 2 && p.pv.page_shift == 0;
@@ -639,10 +436,7 @@ __global__ void __launch_bounds__(32 * W, OCC) paged_decode_kernel(const __grid_
     if (todo > 0 && !stopped) issue();
   };
   if (p.whole) {
-    read_item();
-    kvh = blockIdx.x - item * p.Hkv;
-    g0 = 0;
-    g1 = n_steps;
+    u.whole(p);
     // rows that see nothing: padding, and inactive sequences
     for (int i = max(0, rows - rb * kRows) * (D / 4) + tid; i < min(kRows, p.Lq * p.group - rb * kRows) * (D / 4); i += kThreads) {
       const int r = rb * kRows + i / (D / 4), row = r / p.group, h = kvh * p.group + r % p.group, d = 4 * (i % (D / 4));
@@ -651,7 +445,7 @@ __global__ void __launch_bounds__(32 * W, OCC) paged_decode_kernel(const __grid_
       if (p.lse && d == 0) p.lse[((int64_t)b * p.Lq + row) * p.H + h] = -INFINITY;
     }
     if (n_steps == 0) return;
-  } else if (!find()) {
+  } else if (!u.find(p)) {
     return;
   }
   begin();
@@ -781,7 +575,7 @@ __global__ void __launch_bounds__(32 * W, OCC) paged_decode_kernel(const __grid_
     const bool whole = g0 == 0 && g1 == n_steps;
     const int64_t slot = blockIdx.x + (int64_t)item * p.Hkv + kvh;
     const int mb = b, mkvh = kvh, mrows = rows;
-    const bool more = find();
+    const bool more = u.find(p);
     if (Smem::kApart) {
       if (more) begin();
     } else {
@@ -845,178 +639,6 @@ __global__ void __launch_bounds__(32 * W, OCC) paged_decode_kernel(const __grid_
   }
 }
 
-// What the merge launches know of a unit: its pieces lie in slots slot .. slot + pieces - 1 (one piece: its CTA has
-// finished it; none: no row of it sees anything).
-//
-// With up to 32 items they work it out from the lengths, before they wait for the main launch (whose CTAs have all waited for
-// what came before them by then, so the lengths are there); otherwise from the sums that it left, after.
-struct Pieces {
-  int b, rb, kvh, rows, pieces;
-  int64_t slot;
-  template <int NT, int GS>
-  FPX_INLINE void find(const PagedDecodeParams &p, int unit, int lane) {
-    const int items = p.B * p.blocks, item = unit / p.Hkv;
-    kvh = unit - item * p.Hkv;
-    b = item / p.blocks;
-    rb = item - b * p.blocks;
-    int base, n, total;
-    if (items <= 32) {
-      int before, mine;
-      lane_items<NT, GS>(p, items, lane, before, mine, total);
-      base = __shfl_sync(0xffffffffu, before, item);
-      n = __shfl_sync(0xffffffffu, mine, item) / p.Hkv;
-      asm volatile("griddepcontrol.wait;" ::: "memory");
-    } else {
-      asm volatile("griddepcontrol.wait;" ::: "memory");
-      base = p.prefix[item];
-      n = (p.prefix[item + 1] - base) / p.Hkv;
-      total = p.prefix[items];
-    }
-    int start, count;
-    p.pv.rows(b, p.Lq, start, count);
-    rows = count * p.group;
-    const int per = max(p.min_steps, (total + p.ctas - 1) / p.ctas);
-    const int first = base + kvh * n, c0 = (first + kPad) / per, c1 = (first + n - 1) / per;  // padding, then steps
-    pieces = n ? c1 - c0 + 1 : 0;
-    slot = c0 + (int64_t)item * p.Hkv + kvh;
-  }
-};
-
-// Merges the pieces of one (unit, row), where rows are few and pieces many: D / 4 threads a piece, kPieces of them at a
-// time, kAhead loads in flight before the weights are known. Rows that see nothing (padding, inactive sequences)
-// become zero here.
-template <int D, int NT, int GS>
-__global__ void __launch_bounds__(512) paged_merge_pieces_kernel(const __grid_constant__ PagedDecodeParams p) {
-  constexpr int kThreads = 512, kPieces = kThreads / (D / 4), kRows = 8 * NT, kAhead = 10;
-  const int r = blockIdx.y, tid = threadIdx.x, piece = tid / (D / 4), d = 4 * (tid % (D / 4));
-  __shared__ float red[kThreads / 32];
-  __shared__ __align__(16) float part[kPieces][D];
-  __shared__ float weight[kThreads];
-  Pieces u;
-  u.find<NT, GS>(p, blockIdx.x, tid & 31);
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const int rr = u.rb * kRows + r, row = rr / p.group, h = u.kvh * p.group + rr % p.group;
-  if (rr >= p.Lq * p.group) return;
-  __nv_bfloat16 *out = p.out + u.b * p.o_sb + row * p.o_sl + h * p.o_sh;
-  float *lse = p.lse ? p.lse + ((int64_t)u.b * p.Lq + row) * p.H + h : nullptr;
-  if (rr >= u.rows || u.pieces == 0) {
-    for (int i = tid; i < D; i += kThreads) out[i] = __float2bfloat16_rn(0.f);
-    if (lse && tid == 0) *lse = -INFINITY;
-    return;
-  }
-  if (u.pieces == 1) return;
-  const float *ml = p.part_ml + 2 * (u.slot * kRows + r), *po = p.part_o + (u.slot * kRows + r) * D + d;
-  float m = kLowest, l = 0.f;
-  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int i0 = 0; i0 < u.pieces; i0 += kThreads) {
-    const int here = min(u.pieces - i0, kThreads);
-    float2 mine = make_float2(kLowest, 0.f);
-    if (tid < here) mine = *reinterpret_cast<const float2 *>(ml + 2 * (int64_t)(i0 + tid) * kRows);
-    float4 x[kAhead];
-#pragma unroll
-    for (int k = 0; k < kAhead; ++k) {
-      const int i = piece + k * kPieces;
-      x[k] = i < here ? *reinterpret_cast<const float4 *>(po + (int64_t)(i0 + i) * kRows * D) : make_float4(0.f, 0.f, 0.f, 0.f);
-    }
-    const float top = fmaxf(m, block_max<kThreads>(mine.x, red));  // NaN stays out of m, and in l
-    const float keep = tc::ex2(m - top);
-    m = top;
-    const float s = tid < here ? tc::ex2(mine.x - m) : 0.f;
-    weight[tid] = s;
-    l = fmaf(l, keep, mine.y * s);
-    o.x *= keep; o.y *= keep; o.z *= keep; o.w *= keep;
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < kAhead; ++k) {
-      const int i = piece + k * kPieces;
-      const float w = i < here ? weight[i] : 0.f;
-      o.x = fmaf(x[k].x, w, o.x); o.y = fmaf(x[k].y, w, o.y); o.z = fmaf(x[k].z, w, o.z); o.w = fmaf(x[k].w, w, o.w);
-    }
-#pragma unroll 4
-    for (int i = piece + kAhead * kPieces; i < here; i += kPieces) {
-      const float4 v = *reinterpret_cast<const float4 *>(po + (int64_t)(i0 + i) * kRows * D);
-      const float w = weight[i];
-      o.x = fmaf(v.x, w, o.x); o.y = fmaf(v.y, w, o.y); o.z = fmaf(v.z, w, o.z); o.w = fmaf(v.w, w, o.w);
-    }
-    __syncthreads();
-  }
-  *reinterpret_cast<float4 *>(&part[piece][d]) = o;
-  l = block_sum<kThreads>(l, red);  // its barriers publish part
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  for (int i = tid; i < D; i += kThreads) {
-    float x = 0.f;
-#pragma unroll
-    for (int k = 0; k < kPieces; ++k) x += part[k][i];
-    out[i] = __float2bfloat16_rn(x * inv);
-  }
-  if (lse && tid == 0) *lse = l == 0.f ? -INFINITY : m * kLn2 + logf(l);
-}
-
-// The same where units are many and pieces few: a block a unit, a warp a row, D / 32 dims a lane.
-template <int D, int NT, int GS>
-__global__ void __launch_bounds__(256 * NT) paged_merge_rows_kernel(const __grid_constant__ PagedDecodeParams p) {
-  constexpr int kRows = 8 * NT;
-  const int r = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  Pieces u;
-  u.find<NT, GS>(p, blockIdx.x, lane);
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const int rr = u.rb * kRows + r, row = rr / p.group, h = u.kvh * p.group + rr % p.group;
-  const bool sees = rr < u.rows && u.pieces > 0;
-  if (rr >= p.Lq * p.group || (sees && u.pieces == 1)) return;
-  float m = kLowest, l = 0.f;
-  float4 o[D / 128] = {};
-  if (sees) {
-    const float *ml = p.part_ml + 2 * (u.slot * kRows + r), *po = p.part_o + (u.slot * kRows + r) * D + 4 * lane;
-    constexpr int kAhead = 8;  // pieces whose loads do not wait for the weights
-    for (int i0 = 0; i0 < u.pieces; i0 += 32) {
-      const int here = min(u.pieces - i0, 32);
-      float2 mine = make_float2(kLowest, 0.f);
-      if (lane < here) mine = *reinterpret_cast<const float2 *>(ml + 2 * (int64_t)(i0 + lane) * kRows);
-      float4 x[kAhead][D / 128];
-#pragma unroll
-      for (int k = 0; k < kAhead; ++k)
-#pragma unroll
-        for (int J = 0; J < D / 128; ++J)
-          x[k][J] = k < here ? *reinterpret_cast<const float4 *>(po + (int64_t)(i0 + k) * kRows * D + 128 * J)
-                             : make_float4(0.f, 0.f, 0.f, 0.f);
-      const float top = fmaxf(m, warp_max(mine.x)), keep = tc::ex2(m - top);
-      m = top;
-      const float s = lane < here ? tc::ex2(mine.x - m) : 0.f;
-      l = fmaf(l, keep, mine.y * s);
-#pragma unroll
-      for (int J = 0; J < D / 128; ++J) {
-        o[J].x *= keep; o[J].y *= keep; o[J].z *= keep; o[J].w *= keep;
-      }
-      auto add = [&](float w, const float4 (&v)[D / 128]) {
-#pragma unroll
-        for (int J = 0; J < D / 128; ++J) {
-          o[J].x = fmaf(v[J].x, w, o[J].x); o[J].y = fmaf(v[J].y, w, o[J].y);
-          o[J].z = fmaf(v[J].z, w, o[J].z); o[J].w = fmaf(v[J].w, w, o[J].w);
-        }
-      };
-#pragma unroll
-      for (int k = 0; k < kAhead; ++k) add(__shfl_sync(0xffffffffu, s, k), x[k]);
-#pragma unroll 4
-      for (int i = kAhead; i < here; ++i) {
-        float4 v[D / 128];
-#pragma unroll
-        for (int J = 0; J < D / 128; ++J) v[J] = *reinterpret_cast<const float4 *>(po + (int64_t)(i0 + i) * kRows * D + 128 * J);
-        add(__shfl_sync(0xffffffffu, s, i), v);
-      }
-    }
-    l = warp_sum(l);
-  }
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  __nv_bfloat16 *out = p.out + u.b * p.o_sb + row * p.o_sl + h * p.o_sh + 4 * lane;
-#pragma unroll
-  for (int J = 0; J < D / 128; ++J) {
-    const float x[4] = {o[J].x * inv, o[J].y * inv, o[J].z * inv, o[J].w * inv};
-#pragma unroll
-    for (int e = 0; e < 4; ++e) out[128 * J + e] = __float2bfloat16_rn(x[e]);
-  }
-  if (p.lse && lane == 0) p.lse[((int64_t)u.b * p.Lq + row) * p.H + h] = l == 0.f ? -INFINITY : m * kLn2 + logf(l);
-}
-
 // ---- host -----------------------------------------------------------------------------------
 
 template <int FMT, int D, int NT>
@@ -1029,11 +651,6 @@ template <> struct Shape<FPX_PAGES_BF16, 128, 1> { static constexpr int kGranule
 template <> struct Shape<FPX_PAGES_BF16, 128, 2> { static constexpr int kGranules = 1, kWarps = 4, kStages = 3, kOcc = 2; };
 template <> struct Shape<FPX_PAGES_BF16, 256, 1> { static constexpr int kGranules = 1, kWarps = 4, kStages = 3, kOcc = 1; };
 
-struct Layout {
-  int nt, blocks, ctas, rows;
-  size_t prefix, ml, bytes;
-  int64_t units;
-};
 static size_t up256(size_t x) { return (x + 255) & ~size_t(255); }
 
 template <int FMT, int D, int NT>
@@ -1043,13 +660,16 @@ constexpr int grid_ctas() {
 
 // Column tiles of a row block: two where one would leave rows over (16 rows at d = 128: 25.5 us in one block of two
 // tiles, 35 in two of one), but one for int4 at d = 256, whose registers two do not fit (16 rows: 59 us, 40 in two blocks).
-static Layout layout_of(int format, int B, int Lq, int H, int Hkv, int d) {
-  Layout w{};
+static DecodeLayout layout_of(int format, int B, int Lq, int H, int Hkv, int d) {
+  DecodeLayout w{};
   const int64_t rows = (int64_t)Lq * (H / Hkv);
-  w.nt = rows > 8 && !(format == FPX_PAGES_INT4 && d == 256) ? 2 : 1;
+  const bool tc = format == FPX_PAGES_INT4 && rows > 16;
+  w.nt = tc ? (rows > 32 ? 8 : 4) : rows > 8 && !(format == FPX_PAGES_INT4 && d == 256) ? 2 : 1;
   w.rows = 8 * w.nt;
   w.blocks = (int)((rows + w.rows - 1) / w.rows);
-  if (format == FPX_PAGES_INT4)
+  if (tc)
+    w.ctas = kSms;
+  else if (format == FPX_PAGES_INT4)
     w.ctas = d == 256 ? grid_ctas<FPX_PAGES_INT4, 256, 1>()
                       : (w.nt == 1 ? grid_ctas<FPX_PAGES_INT4, 128, 1>() : grid_ctas<FPX_PAGES_INT4, 128, 2>());
   else
@@ -1071,48 +691,13 @@ static bool whole_units(const PageView &pv, int64_t units) {
 }
 
 template <int FMT, int D, int NT>
-static int launch(PagedDecodeParams &p, const Layout &w, cudaStream_t stream) {
+static int launch(PagedDecodeParams &p, const DecodeLayout &w, cudaStream_t stream) {
   using S = Shape<FMT, D, NT>;
   using Smem = PagedSmem<FMT, D, NT, S::kGranules, S::kWarps, S::kStages>;
   static_assert(sizeof(Smem) <= 227 * 1024, "shared memory of one CTA");
-  const auto kernel = paged_decode_kernel<FMT, D, NT, S::kGranules, S::kWarps, S::kStages, S::kOcc>;
-  // The kernel's shared-memory limit is a setting of the device: once for each.
   static std::atomic<uint64_t> set{0};
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess) return FPX_ERR_CUDA;
-  const uint64_t bit = dev < 64 ? 1ull << dev : 0;
-  if (!(set.load(std::memory_order_relaxed) & bit) || !bit) {
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(Smem)) != cudaSuccess)
-      return FPX_ERR_CUDA;
-    set.fetch_or(bit, std::memory_order_relaxed);
-  }
-  p.min_steps = S::kWarps;
-  // No more CTAs than the table could keep busy.
-  const int64_t longest = ((int64_t)p.pv.max_pages << p.pv.page_shift) / S::kGranules + 1;  // steps
-  const int64_t busy = w.units * (longest + kPad) / p.min_steps + 1;
-  p.ctas = (int)(p.whole ? w.units : std::min<int64_t>(w.ctas, busy));
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(p.ctas);
-  cfg.blockDim = dim3(32 * S::kWarps);
-  cfg.dynamicSmemBytes = sizeof(Smem);
-  cfg.stream = stream;
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  if (cudaLaunchKernelEx(&cfg, kernel, p) != cudaSuccess) return FPX_ERR_CUDA;
-  if (p.whole) return FPX_OK;
-  cfg.dynamicSmemBytes = 0;
-  // Few rows have many pieces each, many rows few: a block a row reads them all at once (one sequence of 131072
-  // tokens: 7.0 us with a loop over them, 2.5 with this), a warp a row leaves room for more rows (32 sequences of up
-  // to 32768: 20 us with a block a row, 5 with this).
-  const bool many = w.units * w.rows > 2 * kSms;
-  cfg.gridDim = many ? dim3((unsigned)w.units) : dim3((unsigned)w.units, w.rows);
-  cfg.blockDim = dim3(many ? 256 * NT : 512);
-  const auto merge = many ? paged_merge_rows_kernel<D, NT, S::kGranules> : paged_merge_pieces_kernel<D, NT, S::kGranules>;
-  if (cudaLaunchKernelEx(&cfg, merge, p) != cudaSuccess) return FPX_ERR_CUDA;
-  return FPX_OK;
+  return launch_decode<D, NT, S::kGranules>(paged_decode_kernel<FMT, D, NT, S::kGranules, S::kWarps, S::kStages, S::kOcc>, set,
+                                            32 * S::kWarps, (int)sizeof(Smem), S::kWarps, p, w, stream);
 }
 
 static bool decode_sizes_ok(int B, int Lq, int H, int Hkv) {
@@ -1146,7 +731,7 @@ extern "C" int fpx_paged_decode_attention(int format, const void *q, int64_t q_s
   if (!decode_sizes_ok(B, Lq, H, Hkv)) return FPX_ERR_UNSUPPORTED;
   const RowStrides qs(q_sb, q_sl, q_sh, B, Lq, H);
   if ((reinterpret_cast<uintptr_t>(q) & 15) || !qs.multiples_of(8)) return FPX_ERR_SHAPE;
-  const Layout w = layout_of(format, B, Lq, H, Hkv, d);
+  const DecodeLayout w = layout_of(format, B, Lq, H, Hkv, d);
   p.whole = whole_units(p.pv, w.units);
   if (!p.whole && (!workspace || workspace_bytes < w.bytes || (reinterpret_cast<uintptr_t>(workspace) & 15)))
     return FPX_ERR_WORKSPACE;
@@ -1157,13 +742,14 @@ extern "C" int fpx_paged_decode_attention(int format, const void *q, int64_t q_s
   p.B = B; p.Lq = Lq; p.H = H; p.Hkv = Hkv; p.group = H / Hkv; p.blocks = w.blocks;
   p.scale_log2 = (float)scale * kLog2e;
   // 32-bit counts of steps: what the table could name in all
-  if ((int64_t)B * w.blocks * Hkv * (((int64_t)max_pages << p.pv.page_shift) + kPad) > 0x7fffffff - (1 << 24))
+  if ((int64_t)B * w.blocks * Hkv * (((int64_t)max_pages << p.pv.page_shift) + kPad<1>) > 0x7fffffff - (1 << 24))
     return FPX_ERR_UNSUPPORTED;
   uint8_t *ws = static_cast<uint8_t *>(workspace);
   p.prefix = reinterpret_cast<int *>(ws);
   p.part_ml = reinterpret_cast<float *>(ws + w.prefix);
   p.part_o = reinterpret_cast<float *>(ws + w.prefix + w.ml);
   if (format == FPX_PAGES_INT4) {
+    if (w.nt > 2) return launch_paged_decode_tc(p, w, d, stream);
     if (d == 256) return launch<FPX_PAGES_INT4, 256, 1>(p, w, stream);
     return w.nt == 1 ? launch<FPX_PAGES_INT4, 128, 1>(p, w, stream) : launch<FPX_PAGES_INT4, 128, 2>(p, w, stream);
   }
