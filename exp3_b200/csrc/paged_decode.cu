@@ -660,14 +660,14 @@ constexpr int grid_ctas() {
 
 // Column tiles of a row block: two where one would leave rows over (16 rows at d = 128: 25.5 us in one block of two
 // tiles, 35 in two of one), but one for int4 at d = 256, whose registers two do not fit (16 rows: 59 us, 40 in two blocks).
-static DecodeLayout layout_of(int format, int B, int Lq, int H, int Hkv, int d) {
+// Many columns (`wide`): row blocks of 32 or 64 on tcgen05.
+static DecodeLayout layout_of(int format, int B, int Lq, int H, int Hkv, int d, bool wide) {
   DecodeLayout w{};
   const int64_t rows = (int64_t)Lq * (H / Hkv);
-  const bool tc = format == FPX_PAGES_INT4 && rows > 16;
-  w.nt = tc ? (rows > 32 ? 8 : 4) : rows > 8 && !(format == FPX_PAGES_INT4 && d == 256) ? 2 : 1;
+  w.nt = wide ? (rows > 32 ? 8 : 4) : rows > 8 && !(format == FPX_PAGES_INT4 && d == 256) ? 2 : 1;
   w.rows = 8 * w.nt;
   w.blocks = (int)((rows + w.rows - 1) / w.rows);
-  if (tc)
+  if (wide)
     w.ctas = kSms;
   else if (format == FPX_PAGES_INT4)
     w.ctas = d == 256 ? grid_ctas<FPX_PAGES_INT4, 256, 1>()
@@ -689,6 +689,16 @@ static bool whole_units(const PageView &pv, int64_t units) {
   const int64_t tokens = ((int64_t)pv.max_pages << pv.page_shift) * kGranule;
   return tokens <= (units >= 32 ? 1024 : 512);
 }
+
+// Whether the tcgen05 kernel takes int4 pages of more than 16 columns: not where the other one's row blocks are few (w is its
+// layout), since it begins a unit 2 to 4 us later. Us, mma.sync / tcgen05: 4 x 65536 tokens, d = 128, 20 columns 32.2 /
+// 26.8, 28 33.5 / 27.1, 56 55.1 / 37.9, 448 282 / 174; d = 256, 20 columns 51.2 / 41.4, 64 113 / 58.4; 1 x 8192, 56 columns
+// 10.9 / 12.8. Tables of 512 tokens, a CTA a unit: 8 x 4 KV heads, 56 columns 10.8 / 15.4; 32 x 4 22.9 / 16.2.
+static bool wide_units(const PageView &pv, const DecodeLayout &w) {
+  const int64_t tokens = ((int64_t)pv.max_pages << pv.page_shift) * kGranule;
+  return tokens * w.units > 65536 && !(whole_units(pv, w.units) && w.units <= w.ctas);
+}
+static bool may_be_wide(int format, int Lq, int H, int Hkv) { return format == FPX_PAGES_INT4 && Lq * (H / Hkv) > 16; }
 
 template <int FMT, int D, int NT>
 static int launch(PagedDecodeParams &p, const DecodeLayout &w, cudaStream_t stream) {
@@ -712,7 +722,8 @@ using namespace fpx;
 extern "C" size_t fpx_paged_decode_workspace_bytes(int format, int B, int Lq, int H, int Hkv, int d) {
   if ((format != FPX_PAGES_BF16 && format != FPX_PAGES_INT4) || (d != 128 && d != 256) || !decode_sizes_ok(B, Lq, H, Hkv))
     return 0;
-  return layout_of(format, B, Lq, H, Hkv, d).bytes;
+  const size_t bytes = layout_of(format, B, Lq, H, Hkv, d, false).bytes;
+  return may_be_wide(format, Lq, H, Hkv) ? std::max(bytes, layout_of(format, B, Lq, H, Hkv, d, true).bytes) : bytes;
 }
 
 extern "C" int fpx_paged_decode_attention(int format, const void *q, int64_t q_sb, int64_t q_sl, int64_t q_sh, int B,
@@ -731,7 +742,8 @@ extern "C" int fpx_paged_decode_attention(int format, const void *q, int64_t q_s
   if (!decode_sizes_ok(B, Lq, H, Hkv)) return FPX_ERR_UNSUPPORTED;
   const RowStrides qs(q_sb, q_sl, q_sh, B, Lq, H);
   if ((reinterpret_cast<uintptr_t>(q) & 15) || !qs.multiples_of(8)) return FPX_ERR_SHAPE;
-  const DecodeLayout w = layout_of(format, B, Lq, H, Hkv, d);
+  DecodeLayout w = layout_of(format, B, Lq, H, Hkv, d, false);
+  if (may_be_wide(format, Lq, H, Hkv) && wide_units(p.pv, w)) w = layout_of(format, B, Lq, H, Hkv, d, true);
   p.whole = whole_units(p.pv, w.units);
   if (!p.whole && (!workspace || workspace_bytes < w.bytes || (reinterpret_cast<uintptr_t>(workspace) & 15)))
     return FPX_ERR_WORKSPACE;
@@ -742,7 +754,7 @@ extern "C" int fpx_paged_decode_attention(int format, const void *q, int64_t q_s
   p.B = B; p.Lq = Lq; p.H = H; p.Hkv = Hkv; p.group = H / Hkv; p.blocks = w.blocks;
   p.scale_log2 = (float)scale * kLog2e;
   // 32-bit counts of steps: what the table could name in all
-  if ((int64_t)B * w.blocks * Hkv * (((int64_t)max_pages << p.pv.page_shift) + kPad<1>) > 0x7fffffff - (1 << 24))
+  if ((int64_t)B * w.blocks * Hkv * (((int64_t)max_pages << p.pv.page_shift) + kPad) > 0x7fffffff - (1 << 24))
     return FPX_ERR_UNSUPPORTED;
   uint8_t *ws = static_cast<uint8_t *>(workspace);
   p.prefix = reinterpret_cast<int *>(ws);

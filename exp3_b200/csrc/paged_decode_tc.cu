@@ -163,10 +163,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_decode_tc_kernel(const __
   } else if (work) {
     work = u.find(p);
   }
-  // 128 x (112 + 112 + 96 + 96 + 64) registers of the launch's 640 x 96
+  // 128 x (120 + 120 + 88 + 88 + 64) registers of the launch's 640 x 96
   if (warp < 8)
-    regs_inc<112>();
-  else if (warp >= 16)
+    regs_inc<120>();
+  else if (warp < 16)
+    regs_dec<88>();
+  else
     regs_dec<64>();
   int c = 0;  // tiles of this CTA so far: tile c lies in stage c % ST, S^T and P^T buffers c & 1
   bool ok = true;

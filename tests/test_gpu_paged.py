@@ -49,14 +49,14 @@ class Cache:
     """A pool of unwritten memory (NaN scales) with a shuffled page table; entries past a sequence's
     pages name no page."""
 
-    def __init__(self, form, lengths, kv_heads, dim, page, seed=0):
+    def __init__(self, form, lengths, kv_heads, dim, page, seed=0, table_tokens=0):
         g = torch.Generator().manual_seed(seed + 77)
         need = [max(1, -(-n // page)) for n in lengths]
         total = sum(need) + 2
         self.pool = paged.new_pool(total, kv_heads, dim, page, form, DEV)
         self.pool.view(torch.uint8).fill_(255)
         order = torch.randperm(total, generator=g).tolist()
-        table = torch.full((len(lengths), max(need) + 1), 1 << 30, dtype=torch.int32)
+        table = torch.full((len(lengths), max(max(need) + 1, table_tokens // page)), 1 << 30, dtype=torch.int32)
         for b, n in enumerate(need):
             table[b, :n] = torch.tensor([order.pop() for _ in range(n)])
         self.table = table.to(DEV)
@@ -187,10 +187,10 @@ def check(cache, lengths, starts, counts, q, kv, scale, out, lse):
 
 
 def attend(form, lengths, rows, heads, kv_heads, dim, page, seed=0, counts=None, starts=None, k_size=1.0, v_size=1.0,
-           scale=None, q_size=1.0):
+           scale=None, q_size=1.0, table_tokens=0):
     g = torch.Generator().manual_seed(seed)
     batch = len(lengths)
-    cache = Cache(form, lengths, kv_heads, dim, page, seed)
+    cache = Cache(form, lengths, kv_heads, dim, page, seed, table_tokens)
     counts = counts or [rows] * batch
     starts = starts or [n - c for n, c in zip(lengths, counts)]
     longest = max(lengths)
