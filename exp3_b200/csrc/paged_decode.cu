@@ -24,6 +24,8 @@
 // ring of bulk copies (no barrier between warps inside a unit). A unit inside one CTA is
 // finished there; the pieces of the others are merged in CTA order by the second launch, so
 // results do not depend on timing.
+//
+// More than 16 columns of int4 pages: paged_decode_tc.cu, where wide_units below says so.
 #include "paged_decode.cuh"
 
 namespace fpx {

@@ -95,7 +95,8 @@ def decode(**change):
     (-1, dict(q=None)), (-1, dict(out=None)), (-1, dict(Lq=0)), (-1, dict(format=3)), (-1, dict(pool=None)),
     (-1, dict(starts=None)), (-2, dict(H=3, Hkv=2)), (-3, dict(Lq=65)), (-3, dict(H=17)), (-3, dict(d=64)),
     (-3, dict(B=1 << 24)), (-2, dict(Lq=2, qs=(0, 260, 128))), (-2, dict(q=ctypes.c_void_p((1 << 20) + 8))), (-5, dict(max_pages=33, stride=33, ws=None)),
-    (-5, dict(max_pages=33, stride=33, ws_bytes=1000)), (-5, dict(max_pages=33, stride=33, ws=ctypes.c_void_p((1 << 20) + 8)))])
+    (-5, dict(max_pages=33, stride=33, ws_bytes=1000)), (-5, dict(Lq=16, max_pages=8192, stride=8192, ws=None)),
+    (-5, dict(Lq=40, max_pages=8192, stride=8192, ws_bytes=148 * 64 * 128 * 4)), (-5, dict(max_pages=33, stride=33, ws=ctypes.c_void_p((1 << 20) + 8)))])
 def test_decode_refuses(status, change):
     assert decode(**change) == status
 
