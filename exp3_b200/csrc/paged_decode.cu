@@ -14,8 +14,8 @@
 //      product with the groups' scales, and a group's scale multiplies the group's sum.
 //   V: codes become the fp16 n - 8 (two logic operations and one exact fma a pair); the scales
 //      r < 2 multiply the probabilities, in fp16 (11 bits: its rounding stays below the bf16 of the
-//      output). The row exponent 2^e joins the logit: u = exp2(s + e - m) <= 2^8 whatever the
-//      values' size, and the sum of weights takes u 2^-e.
+//      output; kLift keeps small ones off the subnormals). The row exponent 2^e joins the logit: u = exp2(s + e - m) <=
+//      2^14 whatever the values' size, and the sum of weights takes u 2^-e.
 //   bf16 pages: P is split in two bf16 terms, so that it does not round before the output does.
 //
 // Work is split evenly over the CTAs of one launch, whatever the sequences' lengths: the
@@ -76,9 +76,9 @@ struct Columns {
   float m[NT][2], l[NT][2];
 };
 
-// Raises the reference m where a logit has passed it by kRaise (always on a first finite logit),
+// Raises the reference m where a logit has passed the one that set it by kRaise (always on a first finite logit),
 // and rescales what was summed under the old one.
-template <int D, int NT, int GS>
+template <int FMT, int D, int NT, int GS>
 FPX_INLINE void follow(Columns<D, NT> &c, const float (&y)[GS][NT][4]) {
   float top[NT][2];
   bool up = false;
@@ -89,7 +89,7 @@ FPX_INLINE void follow(Columns<D, NT> &c, const float (&y)[GS][NT][4]) {
       top[n][e] = fmaxf(y[0][n][e], y[0][n][e + 2]);
 #pragma unroll
       for (int h = 1; h < GS; ++h) top[n][e] = tc::fmax3(top[n][e], y[h][n][e], y[h][n][e + 2]);
-      up |= top[n][e] > c.m[n][e] + kRaise;
+      up |= top[n][e] > c.m[n][e] + (kLift<FMT> + kRaise<FMT>);
     }
   if (!__any_sync(0xffffffffu, up)) return;
 #pragma unroll
@@ -100,7 +100,7 @@ FPX_INLINE void follow(Columns<D, NT> &c, const float (&y)[GS][NT][4]) {
       x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
       x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
       x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
-      const float m = fmaxf(c.m[n][e], x);
+      const float m = fmaxf(c.m[n][e], x - kLift<FMT>);
       const float keep = tc::ex2(c.m[n][e] - m);
       c.m[n][e] = m;
       c.l[n][e] *= keep;
@@ -519,7 +519,7 @@ __global__ void __launch_bounds__(32 * W, OCC) paged_decode_kernel(const __grid_
             for (int k = 0; k < 4; ++k)
               if (((gone >> h) & 1) || key0 + kGranule * h + g + 8 * (k >> 1) >= limit[n][k & 1]) y[h][n][k] = -INFINITY;
       }
-      follow<D, NT, GS>(c, y);
+      follow<FMT, D, NT, GS>(c, y);
 #pragma unroll
       for (int h = 0; h < GS; ++h) {
 #pragma unroll

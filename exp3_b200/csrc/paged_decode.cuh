@@ -27,7 +27,16 @@ struct PagedDecodeParams {
   float *part_ml;  // [ctas + units][8 NT][2]
 };
 
-constexpr float kRaise = 8.f;      // the running reference follows when a logit passes it by this (log2)
+// The running reference (log2) lies kLift below the logit that set it, and follows when one passes that by kRaise, so
+// probabilities are at most 2^(kLift + kRaise). int4 pages: fp16 probabilities, and their products with scales below 2, then
+// stay within fp16's range; a token whose weight is 2^-20 of the largest, more than which a million such tokens do not make up for,
+// keeps its scale's bits down to 2^-14, fp16's smallest normal number as a scale too. Without the lift u r vanished below
+// 2^-25 while the sum of weights kept the token: 131072 tokens 12 nats below one lost 5 % of a group 256 times smaller than the row's largest. bf16
+// pages: probabilities are two bf16 terms, which need none.
+template <int FMT>
+constexpr float kLift = FMT == FPX_PAGES_INT4 ? 10.f : 0.f;
+template <int FMT>
+constexpr float kRaise = FMT == FPX_PAGES_INT4 ? 4.f : 8.f;
 constexpr float kLowest = -3e38f;  // reference before any logit: below all of them, and finite
 
 // Keys that row block rb of sequence b needs: all up to its last row's position.

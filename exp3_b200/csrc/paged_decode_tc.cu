@@ -9,7 +9,7 @@
 // 2600 of its cycles a tile at d = 256, where HBM takes 1600). Only queries and probabilities, the B operands, do.
 //   K: fp16 (n - 8) s 2^-E, E the key's own exponent: 3 + 8 bits, exact down to 2^-30 of the key's largest group. The key is
 //      a lane of S^T, so 2^E, the row exponent e and 2^-e are registers of the thread that reads it.
-//   V: fp16 (n - 8) r, rounded once; probabilities fp16, at most 2^8. Both roundings stay below the output's bf16.
+//   V: fp16 (n - 8) r, rounded once; probabilities fp16, at most 2^14. Both roundings stay below the output's bf16.
 //
 // A CTA: warps 0-3 and 4-7 do the softmax of half the columns each (thread = key; neither half waits for the other), warps
 // 8-11 expand keys, warps 12-15 values (warp = 32 dims of each 128, the lanes that it may write), warp 16 issues the bulk
@@ -28,6 +28,7 @@ using namespace tc;
 
 constexpr int kTile = 128;            // keys
 constexpr int kGs = kTile / kGranule;  // granules of a step
+constexpr float kLift4 = kLift<FPX_PAGES_INT4>, kRaise4 = kRaise<FPX_PAGES_INT4>;
 constexpr int kTcThreads = 640;  // five warpgroups; one of the last one's warps only makes up its number
 
 // 16 rows (lanes) x 32 columns of TMEM: lane 4 g + t holds rows g and g + 8 of columns t, 4 + t, ..
@@ -294,7 +295,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_decode_tc_kernel(const __
           float top = y[0];
 #pragma unroll
           for (int n = 1; n + 1 < C; n += 2) top = fmax3(top, y[n], y[n + 1]);
-          up = fmaxf(top, y[C - 1]) > (fresh ? kLowest : kRaise);
+          up = fmaxf(top, y[C - 1]) > (fresh ? kLowest : kLift4 + kRaise4);
           // P^T's buffer: the product that read it last is complete
           if (c >= 2) ok = mbar_wait_warp(&sh.pv_done[c & 1], ((c - 2) >> 1) & 1, abort);
           tc_fence_before();
@@ -303,7 +304,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_decode_tc_kernel(const __
         }
         int all = agree(up);
         if (!(all & 2) && all) {
-          // Move the references to the tile's largest logits: the first time to them, later up only. A column that sees
+          // Move the references to kLift below the tile's largest logits: the first time there, later up only. A column that sees
           // no key of the first tile that has one sees none of the later ones either, and its reference counts for nothing.
           {
             float x[C];
@@ -318,7 +319,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_decode_tc_kernel(const __
           if (at < C) {
             const int n = c0 + at;
             const float most = fmaxf(fmaxf(sh.red[0][n], sh.red[1][n]), fmaxf(sh.red[2][n], sh.red[3][n]));
-            const float by = most == kLowest ? 0.f : fresh ? most : fmaxf(most, 0.f);
+            const float by = most == kLowest ? 0.f : fresh ? most - kLift4 : fmaxf(most - kLift4, 0.f);
             reinterpret_cast<float *>(&sh.column[n >> 1])[2 + (n & 1)] -= by;
             sh.by[n] = by;
             sh.keep[n] = fresh ? 0.f : ex2(-by);

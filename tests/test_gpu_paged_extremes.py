@@ -1,0 +1,57 @@
+"""Decode attention over pages where sizes lie far apart: weights, groups of a value row, value rows; values that are no
+numbers. Half steps h16 = 2^-11 (fp16) and h = 2^-8 (bf16)."""
+
+import math
+
+import pytest
+import torch
+
+from exp3_b200 import paged
+from paged_reference import attention
+from test_gpu_paged import Cache, DEV, cached_values, ints, no_device_error, randn  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+H16, H = 2.0 ** -11, 2.0 ** -8
+
+
+def whole_keys(g, n, dim):
+    """Keys of whole numbers times 2^-9 that the 4-bit form holds exactly: each group has a 7. Against queries of 1 and -1 every
+    product and sum of the logits is exact."""
+    k = torch.randint(-7, 8, (1, n, 1, dim), generator=g).float()
+    k.unflatten(-1, (-1, 32))[..., 0] = 7
+    return (k * 2.0 ** -9).to(torch.bfloat16)
+
+
+@pytest.mark.parametrize("nats", [12, 14])
+@pytest.mark.parametrize("dim,rows,heads", [(128, 1, 2), (128, 5, 2), (256, 1, 2), (128, 9, 2), (256, 9, 4)])
+def test_small_groups_keep_the_weight_of_many_unlikely_tokens(dim, rows, heads, nats):
+    """One key far above 131071 others, which together weigh as much or an eighth; groups of values 64 and 256 times smaller
+    than the row's largest. 450 sequences share the pages, so that a warp's run is long: what it loses, it loses of a quarter of the
+    tokens or more.
+
+    A product of probability and scale below 2^-14 rounds by up to 2^-25, so does a probability; the largest weight times value
+    exponent stands for at least 2^10. A code is at most 7, and 7 times the exponent is at most the row's largest value:
+    a token adds at most 3 * 2^-35 of the largest weighted value. Logits are exact here; 2^-16 is left for the exponentials and sums."""
+    g = torch.Generator().manual_seed(50)
+    n, batch, at = 131072, 450, 70001
+    k, v = whole_keys(g, n, dim), 1 + 0.25 * torch.randn(1, n, 1, dim, generator=g)
+    q = torch.where(torch.randn(dim, generator=g) > 0, 1.0, -1.0)
+    top = torch.full((dim,), 6.0)
+    top.unflatten(-1, (-1, 32))[..., 0] = 7.0
+    k[0, at, 0] = (q * top * 2.0 ** -6 * (128 / dim)).to(torch.bfloat16)  # 12.06 in all
+    scale = nats / 12.0
+    v *= torch.tensor([1.0, 1 / 64, 1 / 256, 1 / 4] * (dim // 128)).repeat_interleave(32)
+    v = v.to(torch.bfloat16)
+    cache = Cache("int4", [n], 1, dim, 64, seed=50)
+    paged.paged_append(k.to(DEV), v.to(DEV), cache.pool, cache.table, ints([0]))
+    kc, vc = cached_values("int4", k[0].float(), v[0])
+    assert torch.equal(kc, k[0].float())
+    queries = q.to(torch.bfloat16).expand(1, rows, heads, dim)
+    lse = torch.empty(batch, rows, heads, device=DEV)
+    out = paged.paged_decode_attention(queries.expand(batch, -1, -1, -1).to(DEV).contiguous(), cache.pool,
+                                       cache.table.expand(batch, -1).contiguous(), ints([n - rows] * batch), scale, lse=lse)
+    want, want_lse, size, most = attention(queries[0], kc, vc, n - rows, scale)
+    room = H * want.abs() + (2 * H16 + 2.0 ** -16) * size + 3 * n * 2.0 ** -35 * most[..., None]
+    off = (out.cpu().double() - want).abs()
+    assert (off <= room).all(), (off / room).amax((0, 1, 2))
+    assert ((lse.cpu().double() - want_lse).abs() <= 2.0 ** -17 * (1 + want_lse.abs())).all()
