@@ -15,7 +15,7 @@
 //   V: codes become the fp16 n - 8 (two logic operations and one exact fma a pair); the scales
 //      r < 2 multiply the probabilities, in fp16 (11 bits: its rounding stays below the bf16 of the
 //      output; kLift keeps small ones off the subnormals). The row exponent 2^e joins the logit: u = exp2(s + e - m) <=
-//      2^14 whatever the values' size, and the sum of weights takes u 2^-e.
+//      2^14 whatever the values' size, and the sum of weights takes u 2^-e (is_far: where e is large, 2^s itself).
 //   bf16 pages: P is split in two bf16 terms, so that it does not round before the output does.
 //
 // Work is split evenly over the CTAs of one launch, whatever the sequences' lengths: the
@@ -77,11 +77,12 @@ struct Columns {
 };
 
 // Raises the reference m where a logit has passed the one that set it by kRaise (always on a first finite logit),
-// and rescales what was summed under the old one.
+// and rescales what was summed under the old one. Where is_far says so, here or earlier in the part, it takes the sums of the
+// step's weights itself and leaves none to w; so that this costs others nothing, such steps all come through here.
 template <int FMT, int D, int NT, int GS>
-FPX_INLINE void follow(Columns<D, NT> &c, const float (&y)[GS][NT][4]) {
+FPX_INLINE void follow(Columns<D, NT> &c, const float (&y)[GS][NT][4], float (&w)[GS][2], bool &far) {
   float top[NT][2];
-  bool up = false;
+  bool up = far;
 #pragma unroll
   for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -101,15 +102,33 @@ FPX_INLINE void follow(Columns<D, NT> &c, const float (&y)[GS][NT][4]) {
       x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
       x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
       const float m = fmaxf(c.m[n][e], x - kLift<FMT>);
-      const float keep = tc::ex2(c.m[n][e] - m);
+      const float half = tc::ex2(0.5f * (c.m[n][e] - m)), keep = half * half;
       c.m[n][e] = m;
-      c.l[n][e] *= keep;
+      c.l[n][e] = c.l[n][e] * half * half;  // keep may lie below 2^-126 and this above
 #pragma unroll
       for (int i = 0; i < D / 16; ++i) {
         c.o[i][n][e] *= keep;
         c.o[i][n][e + 2] *= keep;
       }
     }
+  if constexpr (FMT == FPX_PAGES_INT4) {
+    float least = w[0][0];
+#pragma unroll
+    for (int h = 0; h < GS; ++h) least = fminf(least, fminf(w[h][0], w[h][1]));
+    far = far || __any_sync(0xffffffffu, is_far(least));
+    if (!far) return;
+#pragma unroll
+    for (int h = 0; h < GS; ++h)
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const float log_w = log2_of(w[h][k]);
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) c.l[n][e] += tc::ex2(y[h][n][2 * k + e] - c.m[n][e] + log_w);
+        w[h][k] = 0.f;
+      }
+  }
 }
 
 // Query fragments of a unit (B operands of S^T = K Q^T), column n = lane / 4 of each tile.
@@ -479,6 +498,7 @@ __global__ void __launch_bounds__(32 * W, OCC) paged_decode_kernel(const __grid_
     // covers the other's latencies.
     float y[GS][NT][4];
     Weights<FMT, NT> pw[GS];
+    bool far = false;  // as is_far has it
     auto weigh = [&](int i) {  // from the scores of step i, which lies in stage `get`, to its probabilities
       const uint32_t stage = ring + get * kBytes;
       const int key0 = (g0 + warp + W * i) * kStep;
@@ -493,16 +513,16 @@ __global__ void __launch_bounds__(32 * W, OCC) paged_decode_kernel(const __grid_
         tc::fence_proxy_async();  // before the next copy into this stage
         __syncwarp();
       }
-      float w[GS][2];  // 2^-e of the lane's two keys
+      float w[GS][2];  // 2^(kSumLift - e) of the lane's two keys
 #pragma unroll
       for (int h = 0; h < GS; ++h) {
         float e[2] = {0.f, 0.f};  // row exponents of the two keys' values
-        w[h][0] = w[h][1] = 1.f;
+        w[h][0] = w[h][1] = kSumUnit;
         if (FMT == FPX_PAGES_INT4) {
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
             e[k] = __uint_as_float(lds16(stage + h * G::kBytes + at.ve + 16 * k) << 16);
-            w[h][k] = ex2_neg(e[k]);
+            w[h][k] = tc::ex2(kSumLift - e[k]);
           }
         }
 #pragma unroll
@@ -519,7 +539,7 @@ __global__ void __launch_bounds__(32 * W, OCC) paged_decode_kernel(const __grid_
             for (int k = 0; k < 4; ++k)
               if (((gone >> h) & 1) || key0 + kGranule * h + g + 8 * (k >> 1) >= limit[n][k & 1]) y[h][n][k] = -INFINITY;
       }
-      follow<FMT, D, NT, GS>(c, y);
+      follow<FMT, D, NT, GS>(c, y, w, far);
 #pragma unroll
       for (int h = 0; h < GS; ++h) {
 #pragma unroll
@@ -617,18 +637,18 @@ __global__ void __launch_bounds__(32 * W, OCC) paged_decode_kernel(const __grid_
       float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
       for (int w = 0; w < W; ++w) {
-        const float s = tc::ex2(merge.m[w][r] - m);
+        const float half = tc::ex2(0.5f * (merge.m[w][r] - m)), s = half * half;
         const float4 x = *reinterpret_cast<const float4 *>(&merge.o[w][r][d]);
-        l = fmaf(merge.l[w][r], s, l);
+        l = fmaf(merge.l[w][r] * half, half, l);
         o.x = fmaf(x.x, s, o.x); o.y = fmaf(x.y, s, o.y); o.z = fmaf(x.z, s, o.z); o.w = fmaf(x.w, s, o.w);
       }
       if (whole) {
         const int row = (row0 + r) / p.group, h = mkvh * p.group + (row0 + r) % p.group;
-        const float inv = l == 0.f ? 0.f : 1.f / l;
+        const float inv = inverse_sum(l);
         __nv_bfloat16 *out = p.out + mb * p.o_sb + row * p.o_sl + h * p.o_sh + d;
         out[0] = __float2bfloat16_rn(o.x * inv); out[1] = __float2bfloat16_rn(o.y * inv);
         out[2] = __float2bfloat16_rn(o.z * inv); out[3] = __float2bfloat16_rn(o.w * inv);
-        if (p.lse && d == 0) p.lse[((int64_t)mb * p.Lq + row) * p.H + h] = l == 0.f ? -INFINITY : m * kLn2 + logf(l);
+        if (p.lse && d == 0) p.lse[((int64_t)mb * p.Lq + row) * p.H + h] = log_sum(m, l);
       } else {
         *reinterpret_cast<float4 *>(&p.part_o[(slot * kRows + r) * D + d]) = o;
         if (d == 0) *reinterpret_cast<float2 *>(&p.part_ml[2 * (slot * kRows + r)]) = make_float2(m, l);

@@ -105,7 +105,7 @@ struct alignas(1024) TcSmem {
   int limit[N];                   // first key that the column does not see
   int64_t out_at[N];              // element of `out` where its row begins; lse's at
   int lse_at[N];
-  float keep[N], by[N], sum[N], red[4][N];
+  float keep[N], by[N], sum[N], red[4][N];  // keep: square root of what a reference's move leaves of the sums
   int4 vote[2][2];                // of each half
   int gone[ST];                   // a bit a granule: its page is missing
   uint64_t full[ST], empty[ST], q_ready, k_ready[2], v_ready[2], p_ready[2], s_full[2], s_free[2], pv_done[2], drain[2];
@@ -183,10 +183,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_decode_tc_kernel(const __
     // ---- softmax: thread = key tid % 128 of the tile, columns c0 .. c0 + C - 1 ----
     const int half = warp >> 2, c0 = half * C, w4 = warp & 3, at = tid & 127;
     const uint32_t lanes = tmem + ((uint32_t)(32 * w4) << 16);
-    // The half's four warps agree: bit 0, some warp says so; bit 1, a wait gave up.
+    // The half's four warps agree: what some warp says; bit 1, a wait gave up.
     int ballots = 0;
-    auto agree = [&](bool any) {
-      const int mine = (__any_sync(0xffffffffu, any) ? 1 : 0) | (ok ? 0 : 2);
+    auto agree = [&](int what) {
+      const int mine = what | (ok ? 0 : 2);
       int4 *v = &sh.vote[half][ballots++ & 1];
       if (lane == 0) reinterpret_cast<int *>(v)[w4] = mine;
       named_sync(1 + half, 128);
@@ -247,10 +247,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_decode_tc_kernel(const __
       uint64_t l[C / 2];
 #pragma unroll
       for (int i = 0; i < C / 2; ++i) l[i] = 0;
-      bool fresh = true;  // the references are still zero
+      bool fresh = true, far = false;  // the references are still zero; as is_far has it
       for (int step = u.g0; step < u.g1; ++step, ++c) {
         const int st = c % ST, key = step * kTile + at;
-        float f = 0.f, e = 0.f, w = 0.f;  // the key's factor of S, row exponent, 2^-e
+        float f = 0.f, e = 0.f, w = 0.f;  // the key's factor of S, row exponent, 2^(kSumLift - e) or 0
         bool there = false, gone = false;
         if ((ok = mbar_wait_warp(&sh.full[st], (c / ST) & 1, abort))) {
           const uint32_t gran = smem_u32(sh.stage[st]) + (at >> 4) * G::kBytes;
@@ -269,7 +269,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_decode_tc_kernel(const __
           gone = missing;
           there = key < u.seen && !((missing >> (at >> 4)) & 1);
           e = there ? __uint_as_float(bits << 16) : 0.f;
-          w = there ? ex2_neg(e) : 0.f;
+          w = there ? ex2(kSumLift - e) : 0.f;
         }
         const bool edge = step * kTile + kTile > least || gone;
         const uint32_t s_at = lanes + S::kS + (c & 1) * N + c0;
@@ -302,7 +302,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_decode_tc_kernel(const __
           __syncwarp();
           if (lane == 0) mbar_arrive(&sh.s_free[c & 1]);
         }
-        int all = agree(up);
+        int all = agree(__any_sync(0xffffffffu, up) || far ? 1 : 0);
         if (!(all & 2) && all) {
           // Move the references to kLift below the tile's largest logits: the first time there, later up only. A column that sees
           // no key of the first tile that has one sees none of the later ones either, and its reference counts for nothing.
@@ -315,20 +315,22 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_decode_tc_kernel(const __
           }
           if (step > u.g0) ok = mbar_wait_warp(&sh.pv_done[(c - 1) & 1], ((c - 1) >> 1) & 1, abort);
           tc_fence_after();
-          all = agree(false);
+          all = agree(__any_sync(0xffffffffu, is_far(w) && w > 0.f) ? 4 : 0);
+          far = far || (all & 4);
           if (at < C) {
             const int n = c0 + at;
             const float most = fmaxf(fmaxf(sh.red[0][n], sh.red[1][n]), fmaxf(sh.red[2][n], sh.red[3][n]));
             const float by = most == kLowest ? 0.f : fresh ? most - kLift4 : fmaxf(most - kLift4, 0.f);
             reinterpret_cast<float *>(&sh.column[n >> 1])[2 + (n & 1)] -= by;
             sh.by[n] = by;
-            sh.keep[n] = fresh ? 0.f : ex2(-by);
+            sh.keep[n] = fresh ? 0.f : ex2(-0.5f * by);
           }
           named_sync(1 + half, 128);
           if (!(all & 2)) {
 #pragma unroll
             for (int i = 0; i < C / 2; ++i) {
-              l[i] = fmul2(l[i], *reinterpret_cast<const uint64_t *>(&sh.keep[c0 + 2 * i]));
+              const uint64_t half = *reinterpret_cast<const uint64_t *>(&sh.keep[c0 + 2 * i]);
+              l[i] = fmul2(fmul2(l[i], half), half);  // their product may lie below 2^-126 and this above
               y[2 * i] -= sh.by[c0 + 2 * i];
               y[2 * i + 1] -= sh.by[c0 + 2 * i + 1];
             }
@@ -341,12 +343,18 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_decode_tc_kernel(const __
                 tmem_ld8(o_at, o);
                 tmem_wait_ld();
 #pragma unroll
-                for (int k = 0; k < 8; ++k) o[k] *= sh.keep[c0 + n + k];
+                for (int k = 0; k < 8; ++k) o[k] *= sh.keep[c0 + n + k] * sh.keep[c0 + n + k];
                 tmem_st8(o_at, o);
               }
               tmem_wait_st();
             }
             fresh = false;
+            if (far) {  // the weights' own exponentials, and none left to w
+              const float log_w = log2_of(w);
+#pragma unroll
+              for (int i = 0; i < C / 2; ++i) l[i] = fadd2(l[i], pk2(ex2(y[2 * i] + log_w), ex2(y[2 * i + 1] + log_w)));
+              w = 0.f;
+            }
           }
           tc_fence_before();
         }
@@ -381,7 +389,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_decode_tc_kernel(const __
       }
       ok = mbar_wait_warp(&sh.pv_done[(c - 1) & 1], ((c - 1) >> 1) & 1, abort);
       tc_fence_after();
-      if (agree(false) & 2) {
+      if (agree(0) & 2) {
         ok = false;
         break;
       }
@@ -392,11 +400,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_decode_tc_kernel(const __
         const int n = c0 + at;
         const float sum = (sh.red[0][n] + sh.red[1][n]) + (sh.red[2][n] + sh.red[3][n]);
         const float m = sum == 0.f ? kLowest : -(reinterpret_cast<const float *>(&sh.column[n >> 1])[2 + (n & 1)]);
-        sh.sum[n] = sum == 0.f ? 0.f : 1.f / sum;
+        sh.sum[n] = inverse_sum(sum);
         if (!whole)
           *reinterpret_cast<float2 *>(&p.part_ml[2 * (slot * N + n)]) = make_float2(m, sum);
         else if (p.lse)
-          p.lse[sh.lse_at[n]] = sum == 0.f ? -INFINITY : m * kLn2 + logf(sum);
+          p.lse[sh.lse_at[n]] = log_sum(m, sum);
       }
       named_sync(1 + half, 128);
       // dims as the value codes' fragments have them: four neighbouring ones over two tiles of 16 lanes

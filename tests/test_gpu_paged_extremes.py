@@ -8,7 +8,7 @@ import torch
 
 from exp3_b200 import paged
 from paged_reference import attention
-from test_gpu_paged import Cache, DEV, cached_values, ints, no_device_error, randn  # noqa: F401
+from test_gpu_paged import Cache, DEV, cached_values, check, ints, no_device_error, randn  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 H16, H = 2.0 ** -11, 2.0 ** -8
@@ -55,3 +55,29 @@ def test_small_groups_keep_the_weight_of_many_unlikely_tokens(dim, rows, heads, 
     off = (out.cpu().double() - want).abs()
     assert (off <= room).all(), (off / room).amax((0, 1, 2))
     assert ((lse.cpu().double() - want_lse).abs() <= 2.0 ** -17 * (1 + want_lse.abs())).all()
+
+
+@pytest.mark.parametrize("exponent", [30, 70, 100, 124])
+@pytest.mark.parametrize("dim,rows,heads", [(128, 1, 4), (128, 3, 4), (256, 1, 4), (128, 3, 8), (256, 5, 8)])
+@pytest.mark.parametrize("n", [300, 20011])
+def test_value_rows_of_far_apart_sizes_weigh_as_they_should(exponent, dim, rows, heads, n):
+    """Rows of values about 2^exponent among rows of 1e-20 (exponent -60) and of zeros: each takes its weight, whose sum
+    divides the large ones. A first, a middle and a late one, so that sums stand before, between and behind them, in one
+    CTA and in pieces. Bounds as in test_gpu_paged.py's `check`."""
+    g = torch.Generator().manual_seed(51)
+    k, v, q = randn(g, 1, n, 1, dim), randn(g, 1, n, 1, dim, size=1e-20), randn(g, 1, rows, heads, dim)
+    v[:, ::3] = 0
+    for at, size in ((n // 2, 1.0), (n - rows - 3, 0.25), (n // 2 + 40, 0.5)):
+        v[:, at] = (randn(g, 1, dim).float().sign() * size * 2.0 ** exponent).to(torch.bfloat16)
+    cache = Cache("int4", [n], 1, dim, 64, seed=51, table_tokens=(1 << 17) * (rows * heads > 16))  # wide: tcgen05
+    paged.paged_append(k.to(DEV), v.to(DEV), cache.pool, cache.table, ints([0]))
+    for first, last in ((0, n), (n // 2 + 1, n), (n // 2 - 40, n // 2 + 1)):  # tokens from the first on and up to the last one
+        if (first, last) == (0, n):
+            table, shift = cache.table, 0
+        else:
+            table, shift = cache.table[:, first // 64:].contiguous(), first // 64 * 64
+        start = last - shift - rows
+        lse = torch.empty(1, rows, heads, device=DEV)
+        out = paged.paged_decode_attention(q.to(DEV), cache.pool, table, ints([start]), dim ** -0.5, lse=lse)
+        kv = [tuple(x[shift:last] for x in cached_values("int4", k[0].float(), v[0]))]
+        check(cache, [last - shift], [start], [rows], q.to(DEV), kv, dim ** -0.5, out, lse)
