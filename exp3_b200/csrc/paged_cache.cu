@@ -140,6 +140,21 @@ FPX_INLINE uint32_t codes4(const float (&x)[4], float s, float inv, bool quick) 
   return w;
 }
 
+// A value row's exponent from its largest amax / 7, and the factors to and from its scales. A row with an infinity or a NaN has
+// exponent 0 and scales 0 but where its groups hold them: its exponent joins the logit in attention, and 126 there would take
+// the other rows' bits.
+struct RowExponent {
+  int e;
+  float up, down;
+  FPX_INLINE explicit RowExponent(float top) {
+    e = min(max((int)((__float_as_uint(top) >> 23) & 255u) - 127, -60), 126);
+    const bool number = e < 126;  // finite values end below 2^125.2 * 7
+    e = number ? e : 0;
+    up = __uint_as_float((uint32_t)(e + 127) << 23);
+    down = number ? __uint_as_float((uint32_t)(127 - e) << 23) : 0.f;
+  }
+};
+
 // One row of K (VALUE false) or V into the granule of token t.
 template <int D, bool VALUE>
 FPX_INLINE void write_int4(uint8_t *gran, int t, const float (&x)[D / 128][4], int lane) {
@@ -158,18 +173,17 @@ FPX_INLINE void write_int4(uint8_t *gran, int t, const float (&x)[D / 128][4], i
   if (VALUE) {
     top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, 8));
     top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, 16));
-    const int e = min(max((int)((__float_as_uint(top) >> 23) & 255u) - 127, -60), 126);
-    const float up = __uint_as_float((uint32_t)(e + 127) << 23), down = __uint_as_float((uint32_t)(127 - e) << 23);
+    const RowExponent x2(top);
 #pragma unroll
     for (int J = 0; J < D / 128; ++J) {
-      const __half r = __float2half_rn(a[J] * down);
-      const float s = __half2float(r) * up;
+      const __half r = __float2half_rn(a[J] * x2.down);
+      const float s = __half2float(r) * x2.up;
       const uint32_t w = codes4(x[J], s, __frcp_rn(s), s > 0x1p-100f && s < 0x1p100f && __half2float(r) >= 0x1p-14f);
       *reinterpret_cast<uint16_t *>(gran + G::kVCodes + v_chunk(t, J, lane & 7) + 2 * j) = (uint16_t)w;
       if ((lane & 7) == 0)
         *reinterpret_cast<__half *>(gran + G::kVScales + (((t >> 1) * (D / 32) + 4 * J + j) * 2 + (t & 1)) * 2) = r;
     }
-    if (lane == 0) *reinterpret_cast<__nv_bfloat16 *>(gran + G::kVExps + 2 * t) = __float2bfloat16_rn((float)e);
+    if (lane == 0) *reinterpret_cast<__nv_bfloat16 *>(gran + G::kVExps + 2 * t) = __float2bfloat16_rn((float)x2.e);
   } else {
     const int p = (lane & 7) >> 1;
 #pragma unroll
@@ -416,16 +430,15 @@ FPX_INLINE void append_rows(const AppendParams &p, int b, int l, int pos, uint8_
       float top = max_nan(a[0], a[1]);
 #pragma unroll
       for (int o = 4; o < kLanes; o <<= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
-      const int e = min(max((int)((__float_as_uint(top) >> 23) & 255u) - 127, -60), 126);
-      const float up = __uint_as_float((uint32_t)(e + 127) << 23), down = __uint_as_float((uint32_t)(127 - e) << 23);
+      const RowExponent x2(top);
       if (!mine || !gran) continue;  // no lane of the warp waits for another below
       const int part = u & 3;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int dim = 8 * u + h * (D / 2), J = dim >> 7, j = (dim & 127) >> 5;
-        const __half r16 = __float2half_rn(a[h] * down);
+        const __half r16 = __float2half_rn(a[h] * x2.down);
         const __nv_bfloat16 b16 = __float2bfloat16_rn(a[h]);
-        const float sc = value ? __half2float(r16) * up : __bfloat162float(b16);
+        const float sc = value ? __half2float(r16) * x2.up : __bfloat162float(b16);
         const bool quick = sc > 0x1p-100f && sc < 0x1p100f && (!value || __half2float(r16) >= 0x1p-14f);
         const float inv = __frcp_rn(sc);
         const uint32_t lo = codes4({x[h][0], x[h][1], x[h][2], x[h][3]}, sc, inv, quick);
@@ -440,7 +453,7 @@ FPX_INLINE void append_rows(const AppendParams &p, int b, int l, int pos, uint8_
           if (part == 0) *reinterpret_cast<__nv_bfloat16 *>(page + G::kKScales + (t * (D / 32) + 4 * J + j) * 2) = b16;
         }
       }
-      if (value && u == 0) *reinterpret_cast<__nv_bfloat16 *>(page + G::kVExps + 2 * t) = __float2bfloat16_rn((float)e);
+      if (value && u == 0) *reinterpret_cast<__nv_bfloat16 *>(page + G::kVExps + 2 * t) = __float2bfloat16_rn((float)x2.e);
     }
   }
 }

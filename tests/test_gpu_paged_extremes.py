@@ -81,3 +81,24 @@ def test_value_rows_of_far_apart_sizes_weigh_as_they_should(exponent, dim, rows,
         out = paged.paged_decode_attention(q.to(DEV), cache.pool, table, ints([start]), dim ** -0.5, lse=lse)
         kv = [tuple(x[shift:last] for x in cached_values("int4", k[0].float(), v[0]))]
         check(cache, [last - shift], [start], [rows], q.to(DEV), kv, dim ** -0.5, out, lse)
+
+
+@pytest.mark.parametrize("value", [math.inf, math.nan])
+@pytest.mark.parametrize("dim,rows,heads", [(128, 1, 4), (128, 3, 4), (256, 1, 4), (128, 3, 8), (256, 5, 8)])
+@pytest.mark.parametrize("n", [300, 20011])
+def test_a_value_that_is_no_number_spoils_its_group_alone(value, dim, rows, heads, n):
+    """The group's dims are NaN for the rows that see it; the others are the sum of all other rows (this one reads back as
+    zero there), and so is the log-sum. Bounds as in test_gpu_paged.py's `check`."""
+    g = torch.Generator().manual_seed(52)
+    k, v, q = randn(g, 1, n, 1, dim), randn(g, 1, n, 1, dim), randn(g, 1, rows, heads, dim)
+    v[0, n // 3, 0, 40] = value
+    cache = Cache("int4", [n], 1, dim, 64, seed=52, table_tokens=(1 << 17) * (rows * heads > 16))
+    paged.paged_append(k.to(DEV), v.to(DEV), cache.pool, cache.table, ints([0]))
+    lse = torch.empty(1, rows, heads, device=DEV)
+    out = paged.paged_decode_attention(q.to(DEV), cache.pool, cache.table, ints([n - rows]), dim ** -0.5, lse=lse)
+    assert out[..., 32:64].isnan().all()
+    kc, vc = cached_values("int4", k[0].float(), v[0])
+    assert vc[n // 3, 0, 32:64].isnan().all() and (vc[n // 3, 0, :32] == 0).all() and (vc[n // 3, 0, 64:] == 0).all()
+    vc[..., 32:64] = 0
+    out[..., 32:64] = 0
+    check(cache, [n], [n - rows], [rows], q.to(DEV), [(kc, vc)], dim ** -0.5, out, lse)
