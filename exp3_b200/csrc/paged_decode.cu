@@ -370,6 +370,73 @@ FPX_INLINE void blank(uint32_t gran, int have, int lane) {
   }
 }
 
+FPX_INLINE void sts16(uint32_t a, uint16_t v) { asm volatile("st.shared.u16 [%0], %1;" ::"r"(a), "h"(v) : "memory"); }
+FPX_INLINE bool no_number_f16(uint32_t x) { return (x & 0x7c00u) == 0x7c00u; }
+FPX_INLINE bool no_number_bf16(uint32_t x) { return (x & 0x7f80u) == 0x7f80u; }
+
+// Tokens `first` .. have - 1 of a granule are seen by some columns and not by others, whose probability 0 times an
+// infinity or a NaN in the value would be NaN. Such values become zero in the stage, and the sums of the columns that see them
+// (limit: the first unseen key) NaN here. key0: the granule's first key.
+template <int FMT, int D, int NT>
+FPX_INLINE void settle(Columns<D, NT> &c, const int (&limit)[NT][2], uint32_t gran, int key0, int first, int have, int lane) {
+  using G = Granule<FMT, D>;
+  const int g = lane >> 2;
+  bool any = false;
+  if constexpr (FMT == FPX_PAGES_INT4) {
+    // a group of a row: its scale says so
+    auto place = [&](int token, int group) { return gran + G::kVScales + (((token >> 1) * (D / 32) + group) * 2 + (token & 1)) * 2; };
+    for (int i = lane; i < kGranule * (D / 32); i += 32) {
+      const int token = i % kGranule;
+      any |= token >= first && token < have && no_number_f16(lds16(place(token, i / kGranule)));
+    }
+    if (!__any_sync(0xffffffffu, any)) return;
+#pragma unroll 1
+    for (int token = first; token < have; ++token)
+#pragma unroll
+      for (int j = 0; j < D / 32; ++j) {
+        if (!no_number_f16(lds16(place(token, j)))) continue;
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            if (key0 + token < limit[n][e])
+              c.o[2 * j][n][e] = c.o[2 * j][n][e + 2] = c.o[2 * j + 1][n][e] = c.o[2 * j + 1][n][e + 2] = __uint_as_float(0x7fffffffu);
+      }
+    __syncwarp();
+    for (int i = lane; i < kGranule * (D / 32); i += 32) {
+      const int token = i % kGranule;
+      const uint32_t a = place(token, i / kGranule);
+      if (token >= first && token < have && no_number_f16(lds16(a))) sts16(a, 0);
+    }
+  } else {
+    auto place = [&](int token, int chunk) { return gran + token * G::kRow + 2 * D + ((chunk ^ (token & 7)) << 4); };
+    for (int i = lane + first * (D / 8); i < have * (D / 8); i += 32) {
+      const uint4 w = lds128(place(i / (D / 8), i % (D / 8)));
+      for (uint32_t x : {w.x, w.y, w.z, w.w}) any |= no_number_bf16(x) || no_number_bf16(x >> 16);
+    }
+    if (!__any_sync(0xffffffffu, any)) return;
+#pragma unroll 1
+    for (int token = first; token < have; ++token)
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {  // dims 16 i + 8 k + g
+          const uint32_t x = lds16(place(token, 2 * i + k) + 2 * g);
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+              if (no_number_bf16(x) && key0 + token < limit[n][e]) c.o[i][n][e + 2 * k] = __uint_as_float(0x7fffffffu);
+        }
+    __syncwarp();
+    for (int i = lane + first * (D / 8); i < have * (D / 8); i += 32) {
+      const uint32_t a = place(i / (D / 8), i % (D / 8));
+      for (int d = 0; d < 8; ++d)
+        if (no_number_bf16(lds16(a + 2 * d))) sts16(a + 2 * d, 0);
+    }
+  }
+}
+
 template <int FMT, int D, int NT, int GS, int W, int ST, int OCC>
 __global__ void __launch_bounds__(32 * W, OCC) paged_decode_kernel(const __grid_constant__ PagedDecodeParams p) {
   using G = Granule<FMT, D>;
@@ -509,6 +576,8 @@ __global__ void __launch_bounds__(32 * W, OCC) paged_decode_kernel(const __grid_
         for (int h = 0; h < GS; ++h) {
           const int have = (gone >> h) & 1 ? 0 : seen - key0 - kGranule * h;
           if (have < kGranule) blank<FMT, D>(stage + h * G::kBytes, have, lane);
+          const int first = max(least - key0 - kGranule * h, 0), last = min(have, kGranule);
+          if (first < last) settle<FMT, D, NT>(c, limit, stage + h * G::kBytes, key0 + kGranule * h, first, last, lane);
         }
         tc::fence_proxy_async();  // before the next copy into this stage
         __syncwarp();

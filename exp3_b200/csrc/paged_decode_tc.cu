@@ -78,6 +78,11 @@ FPX_INLINE float fold(float (&x)[C], int lane, F f) {
     }
   return C == 16 ? f(x[0], __shfl_xor_sync(0xffffffffu, x[0], 16)) : x[0];
 }
+// Scales that are no numbers as fp16's largest, times whose codes, n - 8 = 0, is zero.
+FPX_INLINE uint32_t numbers(uint32_t scales) {
+  const __half2 v = __hmin2(*reinterpret_cast<const __half2 *>(&scales), __half2half2(__ushort_as_half(0x7bff)));
+  return *reinterpret_cast<const uint32_t *>(&v);
+}
 FPX_INLINE uint32_t half2_of(float x) {
   uint32_t d;
   asm("cvt.rn.f16x2.f32 %0, %1, %1;" : "=r"(d) : "f"(x));
@@ -107,6 +112,9 @@ struct alignas(1024) TcSmem {
   int lse_at[N];
   float keep[N], by[N], sum[N], red[4][N];  // keep: square root of what a reference's move leaves of the sums
   int4 vote[2][2];                // of each half
+  // Of each half and group: first key, of the tiles with keys that some columns see and others do not, whose value's group is no number. The
+  // products take it as zero, since a probability 0 times it would be NaN; the columns that see it become NaN at the end.
+  int spoilt[2][D / 32];
   int gone[ST];                   // a bit a granule: its page is missing
   uint64_t full[ST], empty[ST], q_ready, k_ready[2], v_ready[2], p_ready[2], s_full[2], s_free[2], pv_done[2], drain[2];
   Scan<kTcThreads / 32> scan;
@@ -240,6 +248,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_decode_tc_kernel(const __
           sh.lse_at[n] = (int)(((int64_t)u.b * p.Lq + row) * p.H + head);
         }
       }
+      if (at < D / 32) sh.spoilt[half][at] = 0x7fffffff;
       fence_proxy_async();
       named_sync(1 + half, 128);
       if (lane == 0) mbar_arrive(&sh.q_ready);
@@ -263,11 +272,18 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_decode_tc_kernel(const __
           }
           const uint32_t bits = lds16(gran + G::kVExps + 2 * token);
           const int missing = sh.gone[st];
+          there = key < u.seen && !((missing >> (at >> 4)) & 1);
+          if (step * kTile + kTile > least) {
+#pragma unroll 1
+            for (int j = 0; j < D / 32; ++j) {
+              const uint32_t scale = lds16(gran + G::kVScales + (((token >> 1) * (D / 32) + j) * 2 + (token & 1)) * 2);
+              if (there && (scale & 0x7c00u) == 0x7c00u) atomicMin(&sh.spoilt[half][j], key);
+            }
+          }
           __syncwarp();
           if (lane == 0) mbar_arrive(&sh.empty[st]);
           f = __uint_as_float((uint32_t)(max((int)(top >> 23) & 255, 40) - 36) << 23);  // 2^E 2^-24
           gone = missing;
-          there = key < u.seen && !((missing >> (at >> 4)) & 1);
           e = there ? __uint_as_float(bits << 16) : 0.f;
           w = there ? ex2(kSumLift - e) : 0.f;
         }
@@ -416,6 +432,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_decode_tc_kernel(const __
         float o[8];
         tmem_ld8(lanes + S::kO + i / C * N + c0 + n, o);
         tmem_wait_ld();
+        const int spoilt = sh.spoilt[half][i / C * 4 + w4];
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          if (sh.limit[c0 + n + k] > spoilt) o[k] = __uint_as_float(0x7fffffffu);
         if (whole) {
 #pragma unroll
           for (int k = 0; k < 8; ++k)
@@ -500,6 +520,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_decode_tc_kernel(const __
     const uint32_t lanes = tmem + ((uint32_t)(32 * j) << 16);
     const uint32_t sel = j & 1 ? 0x7632 : 0x5410;
     for (bool more = true; more && ok; more = !p.whole && u.find(p)) {
+      const int least = (int)min((int64_t)u.seen, (int64_t)u.start + u.rb * N / p.group + 1);
       for (int step = u.g0; step < u.g1; ++step, ++c) {
         const int st = c % ST;
         ok = mbar_wait_warp(&sh.full[st], (c / ST) & 1, abort);
@@ -508,7 +529,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_decode_tc_kernel(const __
         tc_fence_after();
         const uint32_t stage = smem_u32(sh.stage[st]), v_at = lanes + S::kV + (VB == 2 ? (c & 1) * (D / 2) : 0);
         const int gone = sh.gone[st];
-        const bool edge = step * kTile + kTile > u.seen || gone;
+        const bool edge = step * kTile + kTile > least || gone;
 #pragma unroll 1
         for (int i = 0; i < J; ++i)
 #pragma unroll 1
@@ -521,10 +542,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_decode_tc_kernel(const __
               const uint4 va = lds128(at), vb = lds128(at + 512);  // token pairs t and t + 4
               const uint32_t scales = gran + G::kVScales + (t * (D / 32) + 4 * i + j) * 4;
               uint32_t ra = lds32(scales), rb = lds32(scales + D / 2);
-              if (edge) {  // tokens that are not there: their memory may hold anything
+              if (edge) {  // tokens that are not there: their memory may hold anything; values that are no numbers: see spoilt
                 const int have = (gone >> gi) & 1 ? 0 : u.seen - step * kTile - kGranule * gi;
                 ra &= (2 * t < have ? 0xffffu : 0u) | (2 * t + 1 < have ? 0xffff0000u : 0u);
                 rb &= (2 * t + 8 < have ? 0xffffu : 0u) | (2 * t + 9 < have ? 0xffff0000u : 0u);
+                ra = numbers(ra);
+                rb = numbers(rb);
               }
               const uint32_t u0 = j < 2 ? __byte_perm(va.x, va.z, sel) : __byte_perm(va.y, va.w, sel);
               const uint32_t u1 = j < 2 ? __byte_perm(vb.x, vb.z, sel) : __byte_perm(vb.y, vb.w, sel);

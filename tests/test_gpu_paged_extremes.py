@@ -102,3 +102,34 @@ def test_a_value_that_is_no_number_spoils_its_group_alone(value, dim, rows, head
     vc[..., 32:64] = 0
     out[..., 32:64] = 0
     check(cache, [n], [n - rows], [rows], q.to(DEV), [(kc, vc)], dim ** -0.5, out, lse)
+
+
+@pytest.mark.parametrize("value", [math.inf, -math.inf, math.nan])
+@pytest.mark.parametrize("form,dim,rows,heads", [("int4", 128, 4, 2), ("int4", 128, 5, 3), ("int4", 256, 4, 2), ("int4", 256, 3, 5), ("int4", 128, 7, 4), ("int4", 128, 5, 7),
+                                                 ("int4", 256, 9, 4), ("bf16", 128, 4, 2), ("bf16", 128, 7, 4), ("bf16", 256, 4, 2),
+                                                 ("bf16", 256, 9, 4)])
+@pytest.mark.parametrize("n", [40, 300, 20011])
+def test_a_value_that_is_no_number_reaches_no_row_before_it(value, form, dim, rows, heads, n):
+    """In the call's own rows, as a draft's tokens are: the rows before it are as they are without it; those that see it are spoilt
+    in its group (bf16 pages: its dim) alone. Bounds as in test_gpu_paged.py's `check`. An infinity in bf16 pages comes out as itself or
+    as NaN: its probability is a sum of two bf16 terms h + l with l of either sign or zero, and where l <= 0, h inf + l inf is NaN."""
+    g = torch.Generator().manual_seed(53)
+    k, v, q = randn(g, 1, n, 1, dim), randn(g, 1, n, 1, dim), randn(g, 1, rows, heads, dim)
+    for own in (rows // 2, rows - 1):
+        v2 = v.clone()
+        at = n - rows + own
+        v2[0, at, 0, 41] = value
+        cache = Cache(form, [n], 1, dim, 16, seed=53, table_tokens=(1 << 17) * (rows * heads > 16 and n > 40))
+        paged.paged_append(k.to(DEV), v2.to(DEV), cache.pool, cache.table, ints([0]))
+        lse = torch.empty(1, rows, heads, device=DEV)
+        out = paged.paged_decode_attention(q.to(DEV), cache.pool, cache.table, ints([n - rows]), dim ** -0.5, lse=lse)
+        kc, vc = cached_values(form, k[0].float(), v2[0])
+        spoilt = slice(32, 64) if form == "int4" else slice(41, 42)
+        assert not out[0, own:, :, spoilt].isfinite().any()
+        vc[at, :, spoilt] = 0  # the rows before it do not read it
+        where = (cache, [n], [n - rows], [own], q[:, :own].to(DEV), [(kc, vc)], dim ** -0.5, out[:, :own], lse[:, :own])
+        check(*where)
+        vc = vc.clone()
+        vc[..., spoilt] = 0
+        out[0, own:, :, spoilt] = 0
+        check(cache, [n], [n - rows + own], [rows - own], q[:, own:].to(DEV), [(kc, vc)], dim ** -0.5, out[:, own:], lse[:, own:])
