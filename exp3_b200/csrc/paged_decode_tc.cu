@@ -112,11 +112,12 @@ struct alignas(1024) TcSmem {
   int lse_at[N];
   float keep[N], by[N], sum[N], red[4][N];  // keep: square root of what a reference's move leaves of the sums
   int4 vote[2][2];                // of each half
-  // Of each half and group: first key, of the tiles with keys that some columns see and others do not, whose value's group is no number. The
-  // products take it as zero, since a probability 0 times it would be NaN; the columns that see it become NaN at the end.
-  int spoilt[2][D / 32];
+  // Of each group and key warp: first key, of the tiles with keys that some columns see and others do not, whose value's group is no number. The
+  // products take it as zero, since a probability 0 times it would be NaN; the columns that see it become NaN at the end. By part, in
+  // four places: key warps begin a part when the softmax may still have to read of the third part before it, and no earlier one.
+  int4 spoilt[4][D / 32];
   int gone[ST];                   // a bit a granule: its page is missing
-  uint64_t full[ST], empty[ST], q_ready, k_ready[2], v_ready[2], p_ready[2], s_full[2], s_free[2], pv_done[2], drain[2];
+  uint64_t full[ST], empty[ST], q_ready, k_ready[2], v_ready[2], p_ready[2], s_full[2], s_free[2], pv_done[2], spoilt_ready[4], drain[2];
   Scan<kTcThreads / 32> scan;
   uint32_t tmem;
   int abort;
@@ -147,6 +148,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_decode_tc_kernel(const __
       mbar_init(&sh.pv_done[i], 1);
       mbar_init(&sh.drain[i], 1);
     }
+    for (int i = 0; i < 4; ++i) mbar_init(&sh.spoilt_ready[i], 4);
     sh.abort = 0;
     fence_barrier_init();
   }
@@ -185,6 +187,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_decode_tc_kernel(const __
   else
     regs_dec<64>();
   int c = 0;  // tiles of this CTA so far: tile c lies in stage c % ST, S^T and P^T buffers c & 1
+  int parts = 0;
   bool ok = true;
 
   if (warp < 8 && work) {
@@ -248,7 +251,6 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_decode_tc_kernel(const __
           sh.lse_at[n] = (int)(((int64_t)u.b * p.Lq + row) * p.H + head);
         }
       }
-      if (at < D / 32) sh.spoilt[half][at] = 0x7fffffff;
       fence_proxy_async();
       named_sync(1 + half, 128);
       if (lane == 0) mbar_arrive(&sh.q_ready);
@@ -272,18 +274,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_decode_tc_kernel(const __
           }
           const uint32_t bits = lds16(gran + G::kVExps + 2 * token);
           const int missing = sh.gone[st];
-          there = key < u.seen && !((missing >> (at >> 4)) & 1);
-          if (step * kTile + kTile > least) {
-#pragma unroll 1
-            for (int j = 0; j < D / 32; ++j) {
-              const uint32_t scale = lds16(gran + G::kVScales + (((token >> 1) * (D / 32) + j) * 2 + (token & 1)) * 2);
-              if (there && (scale & 0x7c00u) == 0x7c00u) atomicMin(&sh.spoilt[half][j], key);
-            }
-          }
           __syncwarp();
           if (lane == 0) mbar_arrive(&sh.empty[st]);
           f = __uint_as_float((uint32_t)(max((int)(top >> 23) & 255, 40) - 36) << 23);  // 2^E 2^-24
           gone = missing;
+          there = key < u.seen && !((missing >> (at >> 4)) & 1);
           e = there ? __uint_as_float(bits << 16) : 0.f;
           w = there ? ex2(kSumLift - e) : 0.f;
         }
@@ -403,7 +398,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_decode_tc_kernel(const __
         const float sum = fold(x, lane, [](float a, float b) { return a + b; });
         if (lane < C) sh.red[w4][c0 + lane] = sum;
       }
-      ok = mbar_wait_warp(&sh.pv_done[(c - 1) & 1], ((c - 1) >> 1) & 1, abort);
+      ok = mbar_wait_warp(&sh.pv_done[(c - 1) & 1], ((c - 1) >> 1) & 1, abort) &&
+           mbar_wait_warp(&sh.spoilt_ready[parts & 3], (parts >> 2) & 1, abort);
       tc_fence_after();
       if (agree(0) & 2) {
         ok = false;
@@ -432,10 +428,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_decode_tc_kernel(const __
         float o[8];
         tmem_ld8(lanes + S::kO + i / C * N + c0 + n, o);
         tmem_wait_ld();
-        const int spoilt = sh.spoilt[half][i / C * 4 + w4];
+        const int4 first = sh.spoilt[parts & 3][i / C * 4 + w4];
+        const int spoilt = min(min(first.x, first.y), min(first.z, first.w));
+        if (spoilt != 0x7fffffff) {
 #pragma unroll
-        for (int k = 0; k < 8; ++k)
-          if (sh.limit[c0 + n + k] > spoilt) o[k] = __uint_as_float(0x7fffffffu);
+          for (int k = 0; k < 8; ++k)
+            if (sh.limit[c0 + n + k] > spoilt) o[k] = __uint_as_float(0x7fffffffu);
+        }
         if (whole) {
 #pragma unroll
           for (int k = 0; k < 8; ++k)
@@ -449,6 +448,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_decode_tc_kernel(const __
       }
       tc_fence_before();
       named_sync(1 + half, 128);  // the next part's queries take this one's place
+      ++parts;
       more = !p.whole && u.find(p);
     }
   } else if (warp < 12 && work) {
@@ -456,6 +456,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_decode_tc_kernel(const __
     const int w4 = warp & 3;
     const uint32_t lanes = tmem + ((uint32_t)(32 * w4) << 16);
     for (bool more = true; more && ok; more = !p.whole && u.find(p)) {
+      const int least = (int)min((int64_t)u.seen, (int64_t)u.start + u.rb * N / p.group + 1);
+      int4 *spoilt = sh.spoilt[parts & 3];  // a word of each is this warp's
+      if (lane < D / 32) reinterpret_cast<int *>(&spoilt[lane])[w4] = 0x7fffffff;
       for (int step = u.g0; step < u.g1; ++step, ++c) {
         const int st = c % ST;
         ok = mbar_wait_warp(&sh.full[st], (c / ST) & 1, abort);
@@ -508,11 +511,22 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_decode_tc_kernel(const __
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) {
-          mbar_arrive(&sh.k_ready[c & 1]);
-          mbar_arrive(&sh.empty[st]);
+        if (lane == 0) mbar_arrive(&sh.k_ready[c & 1]);
+        if (step * kTile + kTile > least) {  // lane: a key
+          const int key = step * kTile + 32 * w4 + lane, gi = 2 * w4 + (lane >> 4), token = lane & 15;
+          const bool there = key < u.seen && !((sh.gone[st] >> gi) & 1);
+#pragma unroll 1
+          for (int j = 0; j < D / 32; ++j) {
+            const uint32_t scale = lds16(stage + gi * G::kBytes + G::kVScales + ((token >> 1) * (D / 32) + j) * 4 + (token & 1) * 2);
+            if (there && (scale & 0x7c00u) == 0x7c00u) atomicMin(reinterpret_cast<int *>(&spoilt[j]) + w4, key);
+          }
         }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh.empty[st]);
       }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh.spoilt_ready[parts & 3]);
+      ++parts;
     }
   } else if (warp < 16 && work) {
     // ---- values: warp 12 + j expands the dims of group j of each 128 ----
@@ -608,7 +622,6 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_decode_tc_kernel(const __
   } else if (warp == 17 && work) {
     // ---- S^T = K Q^T ----
     const uint64_t desc = smem_desc_sw128(smem_u32(sh.q), 16, 1024);
-    int parts = 0;
     for (bool more = true; more && ok; more = !p.whole && u.find(p)) {
       ok = mbar_wait_warp(&sh.q_ready, parts++ & 1, abort);
       for (int step = u.g0; step < u.g1 && ok; ++step, ++c) {

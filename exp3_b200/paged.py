@@ -99,7 +99,7 @@ def paged_decode_attention(q, pool, page_table, starts, scale: float, counts=Non
     """Attention of q [B, Lq, H, d] bf16 to the cached tokens, causal by position: row i of sequence b
     sees positions 0 .. starts[b] + i, its own with them (append first). Returns bf16 [B, Lq, H, d]
     (``out`` if given); ``lse`` fp32 [B, Lq, H] takes the natural-log sums. Padding rows give 0 and -inf. An infinity or NaN in
-    a value of the call's own rows may reach the rows before it.
+    a value spoils its dim (4-bit pages: its group of 32) of the rows that see it, and nothing else.
 
     For the few rows of a decode or verification step: Lq <= 64. A longer continuation reads its
     prefix with ``paged_gather`` and runs ``prefill_attention``. ``ws`` is a uint8 workspace of

@@ -353,8 +353,8 @@ int fpx_paged_gather(int format, const void *pool, int pages, int page_size, con
 /* Attention of q [B, Lq, H, d] (16-byte aligned rows) to the cached keys, causal by position: a
  * row sees positions 0 .. its own, which fpx_paged_append has stored. Lq <= 64, H / Hkv <= 16,
  * B * Lq * H <= 2^24. out bf16 with element strides, lse fp32 [B, Lq, H] natural log or NULL;
- * padding rows give 0 and -inf. An infinity or NaN in a value of the call's own rows may reach the
- * rows before it. Bytes of workspace do not depend on the sequences' lengths; it
+ * padding rows give 0 and -inf. An infinity or NaN in a value spoils its dim (int4 pages: its group of 32) of the
+ * rows that see it, and nothing else. Bytes of workspace do not depend on the sequences' lengths; it
  * needs no initial value, and two calls that may overlap need two. Tables of up to 512 tokens
  * (max_pages * page_size) need none: NULL. */
 size_t fpx_paged_decode_workspace_bytes(int format, int B, int Lq, int H, int Hkv, int d);
