@@ -149,6 +149,8 @@ PyObject *decode(PyObject *const *a) {
   if (scale == -1.0 && PyErr_Occurred()) return nullptr;
   const at::Tensor *counts = tensor(a[5], "counts", true), *out = tensor(a[6], "out", true), *lse = tensor(a[7], "lse", true),
                    *ws = tensor(a[8], "ws", true);
+  // its bytes count from its address on, which strides of their own would not give
+  if (ws && !ws->is_contiguous()) refuse("ws must be contiguous");
   Device dev;
   for (const at::Tensor *t : {&q, &pool, &table, &starts, counts, out, lse, ws}) dev.add(t);
   if (q.dim() != 4) refuse("q must be [B, Lq, H, d]");

@@ -102,7 +102,7 @@ def paged_decode_attention(q, pool, page_table, starts, scale: float, counts=Non
     a value spoils its dim (4-bit pages: its group of 32) of the rows that see it, and nothing else.
 
     For the few rows of a decode or verification step: Lq <= 64. A longer continuation reads its
-    prefix with ``paged_gather`` and runs ``prefill_attention``. ``ws`` is a uint8 workspace of
+    prefix with ``paged_gather`` and runs ``prefill_attention``. ``ws`` is a contiguous uint8 workspace of
     ``paged_decode_workspace_bytes``; without it each call takes its own from torch's allocator, so calls on
     several streams or in several graphs share nothing."""
     return _binding().paged_decode_attention(q, pool, page_table, starts, scale, counts, out, lse, ws)
