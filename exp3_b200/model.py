@@ -541,8 +541,8 @@ class Qwen2Model:
 
     def _paged_step(self, tokens, cache, table):
         """One token of every active slot: fp32 logits [sequences, vocab]; moves ``cache.starts``."""
-        n = cache.sequences
-        h = torch.nn.functional.embedding(tokens, self.embed)
+        n, active = cache.sequences, cache.starts >= 0
+        h = torch.nn.functional.embedding(torch.where(active, tokens, 0), self.embed)  # inactive slots may hold any token
         x = self._rmsnorm(h, self.layers[0].ln1)
         for i in range(self.cfg.num_hidden_layers):
             if i > 0:
@@ -553,7 +553,7 @@ class Qwen2Model:
             attn = paged.paged_decode_attention(q, *where, self.scale)
             h, down = self._paged_rest(i, h, attn.view(n, -1))
         logits = self._logits(down, h)
-        cache.starts.add_((cache.starts >= 0).to(torch.int32))
+        cache.starts.add_(active)
         return logits
 
     def _paged_room(self, cache, steps):

@@ -1,0 +1,29 @@
+"""Steps of the paged model: tokens of inactive slots, and a step that does not end."""
+
+import pytest
+import torch
+
+from exp3_b200 import _capi
+from exp3_b200.model import AttentionSettings, Qwen2Model
+from test_gpu_model_paged import CFG, prompt
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("graph", [False, True])
+def test_any_token_may_stand_in_an_inactive_slot(graph):
+    model = Qwen2Model(CFG, seed=26, attention=AttentionSettings("dense"))
+    runs = []
+    for other in (0, -1, 1 << 40):
+        cache = model.new_cache(pages=20, page_size=16, format="int4", sequences=3, max_tokens=64)
+        tokens = torch.full((3,), other, device="cuda")
+        tokens[1] = model.prefill_paged(prompt(20, 2), cache, 1).argmax()
+        if graph:
+            runs.append(model.decode_paged_graph(tokens, 5, cache)[:, 1])
+            assert cache.lengths == [-1, 24, -1]
+        else:
+            runs.append(model.decode_paged(tokens, cache)[1])
+            assert cache.lengths == [-1, 21, -1]
+        assert cache.starts.tolist() == cache.lengths
+    assert torch.equal(runs[0], runs[1]) and torch.equal(runs[0], runs[2])
+    assert _capi.device_error() == 0
