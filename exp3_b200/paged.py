@@ -166,6 +166,8 @@ class PagedKVCache:
 
     def set_length(self, sequence: int, tokens: int) -> None:
         """The slot's next token stands at position ``tokens`` (negative: inactive)."""
+        if tokens > self.max_tokens:
+            raise FpxError(f"{tokens} tokens: a slot holds {self.max_tokens}")
         if tokens > len(self._held[sequence]) * self.page_size:
             raise FpxError(f"the slot's {len(self._held[sequence])} pages hold fewer than {tokens} tokens")
         self.lengths[sequence] = tokens

@@ -21,3 +21,13 @@ def test_a_workspace_that_is_not_contiguous_is_refused(ws):
         decode(ws=ws)
     with pytest.raises(_capi.FpxError, match="CUDA"):
         decode(ws=ws.contiguous())
+
+
+def test_a_slot_holds_no_more_than_its_tokens():
+    """Its last page has room behind max_tokens, where the model's rotation table ends."""
+    cache = paged.PagedKVCache(1, pages=8, kv_heads=1, page_size=64, sequences=1, max_tokens=100, device="cpu")
+    cache.reserve(0, 100)
+    cache.set_length(0, 100)
+    with pytest.raises(_capi.FpxError, match="100"):
+        cache.set_length(0, 101)
+    assert cache.lengths == [100] and cache.starts.tolist() == [100]
