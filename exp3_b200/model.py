@@ -587,24 +587,30 @@ class Qwen2Model:
         self._decode_comm()
         table, token = self._table(cache), first_tokens.clone()
 
-        def one_step():
-            token.copy_(self._paged_step(token, cache, table).argmax(-1))
+        def one_step(stepped=lambda: None):
+            logits = self._paged_step(token, cache, table)
+            stepped()
+            token.copy_(logits.argmax(-1))
 
+        # The cache's lengths follow each step, so that where a later one raises they say what the pages hold.
         side = torch.cuda.Stream(device=self.device)  # the eager first step warms the allocator up
         side.wait_stream(torch.cuda.current_stream(self.device))
-        with torch.cuda.stream(side):
-            one_step()
-        torch.cuda.current_stream(self.device).wait_stream(side)
+        try:
+            with torch.cuda.stream(side):
+                one_step(cache.advance)
+        finally:
+            torch.cuda.current_stream(self.device).wait_stream(side)
         out[1] = token
         if steps > 2:
-            graph = torch.cuda.CUDAGraph()
-            with torch.cuda.graph(graph):
-                one_step()
-            for i in range(2, steps):
-                graph.replay()
-                out[i] = token
-            del graph  # a graph holding NCCL calls must go before the process group
-        cache.advance(steps - 1)
+            with torch.cuda.device(self.device):
+                graph = torch.cuda.CUDAGraph()
+                with torch.cuda.graph(graph):
+                    one_step()
+                for i in range(2, steps):
+                    graph.replay()
+                    cache.advance()
+                    out[i] = token
+                del graph  # a graph holding NCCL calls must go before the process group
         return out
 
     def close_comm(self):

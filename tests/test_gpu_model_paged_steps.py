@@ -27,3 +27,31 @@ def test_any_token_may_stand_in_an_inactive_slot(graph):
         assert cache.starts.tolist() == cache.lengths
     assert torch.equal(runs[0], runs[1]) and torch.equal(runs[0], runs[2])
     assert _capi.device_error() == 0
+
+
+@pytest.mark.parametrize("fails", [1, 2])
+def test_a_step_that_raises_leaves_the_cache_as_the_last_whole_one(fails, monkeypatch):
+    """The first call of the graphed decode's step runs, the second is captured: whichever raises, host and device agree on the lengths,
+    and decoding goes on from there."""
+    model = Qwen2Model(CFG, seed=27, attention=AttentionSettings("dense"))
+    cache, other = (model.new_cache(pages=20, page_size=16, format="int4", sequences=2, max_tokens=64) for _ in range(2))
+    tokens = torch.zeros(2, dtype=torch.int64, device="cuda")
+    for c in (cache, other):
+        tokens[1] = model.prefill_paged(prompt(20, 3), c, 1).argmax()
+    step, calls = Qwen2Model._paged_step, []
+
+    def failing(self, *args):
+        calls.append(1)
+        if len(calls) == fails:
+            raise RuntimeError("out of memory")
+        return step(self, *args)
+
+    monkeypatch.setattr(Qwen2Model, "_paged_step", failing)
+    with pytest.raises(RuntimeError, match="out of memory"):
+        model.decode_paged_graph(tokens, 6, cache)
+    monkeypatch.undo()
+    done = fails - 1
+    assert cache.lengths == [-1, 20 + done] and cache.starts.tolist() == cache.lengths
+    for _ in range(done):
+        tokens = model.decode_paged(tokens, other).argmax(-1)
+    assert torch.equal(model.decode_paged(tokens, cache)[1], model.decode_paged(tokens, other)[1])
