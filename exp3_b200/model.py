@@ -491,9 +491,9 @@ class Qwen2Model:
         """fp32 logits of each row over the whole vocabulary."""
         logits = (self._rmsnorm(rows, self.norm, residual=residual) @ self.lm_head.t()).float()
         if self.vocab_sharded:
-            parts = torch.empty(self.tp_size, *logits.shape, dtype=logits.dtype, device=logits.device)
-            torch.distributed.all_gather_into_tensor(parts, logits, group=self.group)
-            logits = parts.transpose(0, 1).flatten(1)
+            parts = torch.empty(self.tp_size * logits.shape[0], logits.shape[1], dtype=logits.dtype, device=logits.device)
+            torch.distributed.all_gather_into_tensor(parts, logits, group=self.group)  # ranks one after another
+            logits = parts.view(self.tp_size, *logits.shape).transpose(0, 1).flatten(1)
         return logits
 
     @torch.inference_mode()

@@ -1,7 +1,12 @@
 """Host logic of the model's paged path on the CPU (tests/paged_model_cpu.py has the kernels' calls as plain torch)."""
 
+import datetime
+import os
+
 import pytest
 import torch
+import torch.distributed as dist
+import torch.multiprocessing as mp
 
 from paged_model_cpu import PlainModel, prompt, use_plain_calls
 
@@ -22,3 +27,49 @@ def test_any_token_may_stand_in_an_inactive_slot(plain):
         runs.append(model.decode_paged(tokens, cache)[1])
         assert cache.lengths == [-1, 21, -1] and cache.starts.tolist() == cache.lengths
     assert runs[0].isfinite().all() and torch.equal(runs[0], runs[1]) and torch.equal(runs[0], runs[2])
+
+
+def decode_run(model):
+    """Two prompts, one of them continued from its prefix, an empty slot, three steps: all logits."""
+    cache = model.new_cache(pages=40, page_size=16, format="bf16", sequences=3, max_tokens=256)
+    out = [model.prefill_paged(prompt(140, 5), cache, 0), model.prefill_paged(prompt(9, 6), cache, 2)]
+    out.append(model.prefill_paged(torch.cat((prompt(140, 5), prompt(12, 7))), cache, 0, reuse=140))
+    for tokens in ([3, -1, 5], [60, 7, 11], [0, -1, 63]):
+        logits = model.decode_paged(torch.tensor(tokens), cache)
+        out += [logits[0], logits[2]]
+    assert cache.lengths == [155, -1, 12]
+    return torch.stack(out)
+
+
+def tensor_parallel_rank(rank, world, port, path):
+    os.environ.update(MASTER_ADDR="127.0.0.1", MASTER_PORT=str(port))
+    torch.set_num_threads(2)
+    dist.init_process_group("gloo", rank=rank, world_size=world, timeout=datetime.timedelta(seconds=120))
+    try:
+        use_plain_calls(setattr)
+        model = PlainModel(seed=4, tp_rank=rank, tp_size=world)
+        assert model.vocab_sharded and len(model.kv) == max(1, 2 // world)
+        torch.save(decode_run(model), f"{path}/{rank}.pt")
+    finally:
+        dist.destroy_process_group()
+
+
+@pytest.mark.parametrize("world", [2, 4])
+def test_tensor_parallel_paged_decode(plain, tmp_path, world):
+    """Ranks that share KV heads out (2) and that share one group's query heads out (4) give one rank's logits, over the whole vocabulary in
+    its order, on every rank alike.
+
+    A rank's partial products round to bf16 (half a step 2^-8 of each) before they are summed, four times in the two layers, and
+    rounding of the residual stream adds as much: logits agree to a few 2^-8 of their size; shards in another order would not at all."""
+    want = decode_run(PlainModel(seed=4))
+    ctx = mp.get_context("spawn")
+    procs = [ctx.Process(target=tensor_parallel_rank, args=(r, world, 29547 + world, str(tmp_path))) for r in range(world)]
+    for p in procs:
+        p.start()
+    for p in procs:
+        p.join(timeout=300)
+    assert [p.exitcode for p in procs] == [0] * world
+    got = [torch.load(tmp_path / f"{r}.pt") for r in range(world)]
+    assert all(torch.equal(got[0], g) for g in got[1:])
+    off = (got[0] - want).square().sum(-1).sqrt() / want.square().sum(-1).sqrt()
+    assert (off <= 12 * 2.0 ** -8).all(), off
