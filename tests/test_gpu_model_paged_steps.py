@@ -3,7 +3,8 @@
 import pytest
 import torch
 
-from exp3_b200 import _capi
+from exp3_b200 import _capi, ops
+from exp3_b200.attention import METHODS
 from exp3_b200.model import AttentionSettings, Qwen2Model
 from test_gpu_model_paged import CFG, prompt
 
@@ -55,3 +56,32 @@ def test_a_step_that_raises_leaves_the_cache_as_the_last_whole_one(fails, monkey
     for _ in range(done):
         tokens = model.decode_paged(tokens, other).argmax(-1)
     assert torch.equal(model.decode_paged(tokens, cache)[1], model.decode_paged(tokens, other)[1])
+
+
+@pytest.mark.parametrize("reuse", [128, 700, 1100])
+@pytest.mark.parametrize("method,alpha", [(m, a) for m in METHODS for a in (0.08, 0.3)])
+def test_a_reused_prefix_is_read_as_keys_alone(method, alpha, reuse, monkeypatch):
+    """The prefix's queries are never computed. Whatever their memory holds (NaN here), the new rows' attention, with tiles left out and
+    tails, has the bits of a call on full queries."""
+    model = Qwen2Model(CFG, seed=28, attention=AttentionSettings(method, alpha, sink=1, window=1, last_full=1))
+    ids = prompt(1300, 51)
+    cache = model.new_cache(pages=30, format="bf16", max_tokens=1400)
+    model.prefill_paged(ids[:reuse], cache)
+    calls = []
+    kernel = ops.prefill_attention
+
+    def spy(q, k, v, *args, tile_range=None):
+        prefix = 128 * tile_range[0]
+        assert prefix == reuse // 128 * 128
+        full = torch.randn_like(q)
+        full[:, prefix:] = q[:, prefix:]
+        q[:, :prefix] = float("nan")
+        got = kernel(q, k, v, *args, tile_range=tile_range)
+        want = kernel(full, k, v, *args)
+        calls.append(torch.equal(got[:, prefix:], want[:, prefix:]))
+        return got
+
+    monkeypatch.setattr(ops, "prefill_attention", spy)
+    logits = model.prefill_paged(ids, cache, reuse=reuse)
+    assert calls == [True] * CFG.num_hidden_layers and logits.isfinite().all()
+    assert _capi.device_error() == 0
