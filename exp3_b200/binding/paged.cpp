@@ -323,4 +323,8 @@ PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_paged", nullptr, -1, g_methods}
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__paged() { return PyModule_Create(&g_module); }
+PyMODINIT_FUNC PyInit__paged() {
+  PyObject *module = PyModule_Create(&g_module);
+  if (module && PyModule_AddStringConstant(module, "TORCH_VERSION", FPX_TORCH_VERSION) < 0) Py_CLEAR(module);
+  return module;
+}

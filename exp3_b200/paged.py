@@ -68,8 +68,13 @@ def _binding():
     """The module that checks a call's tensors and makes the C call on their device's current stream."""
     if not BINDING_PATH.exists():
         raise FpxError(f"{BINDING_PATH} is missing: build it with `python -m exp3_b200.build`")
-    from . import _paged
-
+    try:
+        from . import _paged
+    except ImportError as e:
+        raise FpxError(f"{BINDING_PATH} does not load ({e}): build it again with `python -m exp3_b200.build`") from e
+    if _paged.TORCH_VERSION != torch.__version__:
+        raise FpxError(f"{BINDING_PATH} was built for torch {_paged.TORCH_VERSION}, this is {torch.__version__}: build it again with "
+                       "`python -m exp3_b200.build`")
     names = ("fpx_paged_append", "fpx_paged_gather", "fpx_paged_decode_attention", "fpx_paged_decode_workspace_bytes",
              "fpx_status_string")
     _paged.bind(*(ctypes.cast(getattr(lib(), name), ctypes.c_void_p).value for name in names), FpxError)
