@@ -81,7 +81,7 @@ struct Where {
   int format, dim, heads, pages, page_size, max_pages;
   void *pool;
   const int32_t *table, *starts, *counts;
-  int64_t stride, batch;
+  int64_t stride;
 };
 const int32_t *index_tensor(const at::Tensor *t, int64_t batch) {
   if (!t) return nullptr;
@@ -124,7 +124,6 @@ Where where(const at::Tensor &pool, const at::Tensor &table, const at::Tensor &s
   w.stride = batch > 1 ? table.stride(0) : table.size(1);
   w.starts = index_tensor(&starts, batch);
   w.counts = index_tensor(counts, batch);
-  w.batch = batch;
   return w;
 }
 
@@ -149,6 +148,9 @@ PyObject *decode(PyObject *const *a) {
   if (scale == -1.0 && PyErr_Occurred()) return nullptr;
   const at::Tensor *counts = tensor(a[5], "counts", true), *out = tensor(a[6], "out", true), *lse = tensor(a[7], "lse", true),
                    *ws = tensor(a[8], "ws", true);
+  if (q.dim() == 4 && q.size(1) > FPX_PAGED_MAX_ROWS)
+    refuse(std::to_string(q.size(1)) + " query rows a sequence: one call takes " + std::to_string(FPX_PAGED_MAX_ROWS) +
+           " (paged_gather and prefill_attention take longer continuations)");
   // its bytes count from its address on, which strides of their own would not give
   if (ws && !ws->is_contiguous()) refuse("ws must be contiguous");
   Device dev;

@@ -557,15 +557,6 @@ struct GatherRows {
   uint32_t live, zero;
   bool wide;  // the output's rows are 16-byte aligned
 };
-FPX_INLINE void gather_store(const GatherRows &o, __nv_bfloat16 *dst, uint4 v) {  // eight dims
-  if (o.wide) {
-    *reinterpret_cast<uint4 *>(dst) = v;
-  } else {
-    *reinterpret_cast<uint2 *>(dst) = make_uint2(v.x, v.y);
-    *reinterpret_cast<uint2 *>(dst + 4) = make_uint2(v.z, v.w);
-  }
-}
-
 // bf16(n - 8) s of a word of eight codes, correctly rounded (both factors are bf16): codes become 128 + n by an
 // and-or of two of them, four dims apart, 136 is taken off exactly, and the products are put back in order.
 FPX_INLINE uint4 scaled8(uint32_t w, __nv_bfloat162 s) {
@@ -605,7 +596,7 @@ FPX_INLINE void gather_int4(const GatherRows &o, const uint8_t *gran, int lane) 
       for (int j = 0; j < 4; ++j) {
         const uint32_t u = j < 2 ? sc.x : sc.y;
         const uint32_t s = __byte_perm(u, u, j & 1 ? 0x3232 : 0x1010);
-        gather_store(o, dst + 32 * j, scaled8(words[j], *reinterpret_cast<const __nv_bfloat162 *>(&s)));
+        store8(dst + 32 * j, scaled8(words[j], *reinterpret_cast<const __nv_bfloat162 *>(&s)), o.wide);
       }
     }
   const int vg = lane & 7;
@@ -666,7 +657,7 @@ FPX_INLINE void gather_bf16(const GatherRows &o, const uint8_t *gran, int lane) 
     for (int k = 0; k < kAhead; ++k) {
       const int i = i0 + 32 * k, token = i / (2 * kChunks), c = i % kChunks;
       if (((o.live | o.zero) >> token) & 1)
-        gather_store(o, ((i / kChunks) & 1 ? o.v + token * o.v_sl : o.k + token * o.k_sl) + 8 * c, w[k]);
+        store8(((i / kChunks) & 1 ? o.v + token * o.v_sl : o.k + token * o.k_sl) + 8 * c, w[k], o.wide);
     }
   }
 }

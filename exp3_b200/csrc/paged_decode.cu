@@ -802,7 +802,7 @@ static int launch(PagedDecodeParams &p, const DecodeLayout &w, cudaStream_t stre
 }
 
 static bool decode_sizes_ok(int B, int Lq, int H, int Hkv) {
-  return B > 0 && Lq > 0 && Lq <= 64 && H > 0 && Hkv > 0 && H % Hkv == 0 && H / Hkv <= 16 && Hkv <= 65535 &&
+  return B > 0 && Lq > 0 && Lq <= FPX_PAGED_MAX_ROWS && H > 0 && Hkv > 0 && H % Hkv == 0 && H / Hkv <= 16 && Hkv <= 65535 &&
          (int64_t)B * Lq * H <= (1 << 24);
 }
 

@@ -31,7 +31,7 @@ from ._capi import FpxError, lib
 
 FORMATS = {"bf16": 0, "int4": 1}
 BINDING_PATH = Path(__file__).resolve().parent / "_paged.so"
-MAX_ROWS = 64  # query rows of a sequence in one paged_decode_attention
+MAX_ROWS = 64  # query rows of a sequence in one paged_decode_attention (FPX_PAGED_MAX_ROWS)
 
 
 def row_elements(format: str, head_dim: int) -> int:
@@ -106,7 +106,7 @@ def paged_decode_attention(q, pool, page_table, starts, scale: float, counts=Non
     (``out`` if given); ``lse`` fp32 [B, Lq, H] takes the natural-log sums. Padding rows give 0 and -inf. An infinity or NaN in
     a value spoils its dim (4-bit pages: its group of 32) of the rows that see it, and nothing else.
 
-    For the few rows of a decode or verification step: Lq <= 64. A longer continuation reads its
+    For the few rows of a decode or verification step: Lq <= MAX_ROWS. A longer continuation reads its
     prefix with ``paged_gather`` and runs ``prefill_attention``. ``ws`` is a contiguous uint8 workspace of
     ``paged_decode_workspace_bytes``; without it each call takes its own from torch's allocator, so calls on
     several streams or in several graphs share nothing."""

@@ -350,8 +350,10 @@ int fpx_paged_gather(int format, const void *pool, int pages, int page_size, con
                      int Hkv, int d, void *k, int64_t k_sb, int64_t k_sl, int64_t k_sh, void *v, int64_t v_sb,
                      int64_t v_sl, int64_t v_sh, int zero_padding, fpx_stream_t stream);
 
+#define FPX_PAGED_MAX_ROWS 64 /* query rows of a sequence in one fpx_paged_decode_attention */
+
 /* Attention of q [B, Lq, H, d] (16-byte aligned rows) to the cached keys, causal by position: a
- * row sees positions 0 .. its own, which fpx_paged_append has stored. Lq <= 64, H / Hkv <= 16,
+ * row sees positions 0 .. its own, which fpx_paged_append has stored. Lq <= FPX_PAGED_MAX_ROWS, H / Hkv <= 16,
  * B * Lq * H <= 2^24. out bf16 with element strides, lse fp32 [B, Lq, H] natural log or NULL;
  * padding rows give 0 and -inf. An infinity or NaN in a value spoils its dim (int4 pages: its group of 32) of the
  * rows that see it, and nothing else. Bytes of workspace do not depend on the sequences' lengths; it

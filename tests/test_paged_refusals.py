@@ -31,3 +31,9 @@ def test_a_slot_holds_no_more_than_its_tokens():
     with pytest.raises(_capi.FpxError, match="100"):
         cache.set_length(0, 101)
     assert cache.lengths == [100] and cache.starts.tolist() == [100]
+
+
+def test_more_query_rows_than_a_call_takes_are_refused_by_name():
+    for rows, match in ((paged.MAX_ROWS, "CUDA"), (paged.MAX_ROWS + 1, "65 query rows")):
+        with pytest.raises(_capi.FpxError, match=match):
+            decode(q=torch.zeros(1, rows, 4, 128, dtype=torch.bfloat16))
