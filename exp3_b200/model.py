@@ -509,6 +509,7 @@ class Qwen2Model:
             raise ValueError(f"the slot holds {max(0, cache.lengths[sequence])} tokens, {reuse} cannot be reused")
         prefix = min(reuse, length - 1) // ops.BLOCK_SIZE * ops.BLOCK_SIZE
         cache.reserve(sequence, length)
+        cache.set_length(sequence, prefix or -1)  # all that the slot holds if a layer raises: the rows behind are overwritten
         cfg, a = self.cfg, self.attn
         hq, hkv, d, dev = len(self.qh), len(self.kv), cfg.head_dim, self.device
         at = lambda n: torch.tensor([n], dtype=torch.int32, device=dev)  # noqa: E731

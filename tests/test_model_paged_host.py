@@ -73,3 +73,31 @@ def test_tensor_parallel_paged_decode(plain, tmp_path, world):
     assert all(torch.equal(got[0], g) for g in got[1:])
     off = (got[0] - want).square().sum(-1).sqrt() / want.square().sum(-1).sqrt()
     assert (off <= 12 * 2.0 ** -8).all(), off
+
+
+@pytest.mark.parametrize("reuse,length", [(0, -1), (140, 128)])
+def test_a_prefill_that_raises_leaves_what_is_whole(plain, monkeypatch, reuse, length):
+    """Rows behind the reused tiles are overwritten layer by layer: a slot whose prefill raised holds those tiles, or nothing."""
+    import exp3_b200.model as model_module
+
+    model = PlainModel(seed=6)
+    cache = model.new_cache(pages=40, page_size=16, format="bf16", sequences=2, max_tokens=256)
+    model.prefill_paged(prompt(140, 5), cache, 1)
+    longer = torch.cat((prompt(140, 5), prompt(12, 7)))
+    want = model.prefill_paged(longer, model.new_cache(pages=40, page_size=16, format="bf16", max_tokens=256))
+    ops, calls = model_module.ops, []
+
+    class Failing(ops):
+        @staticmethod
+        def prefill_attention(*args, **kw):
+            calls.append(1)
+            if len(calls) == 2:
+                raise RuntimeError("out of memory")
+            return ops.prefill_attention(*args, **kw)
+
+    monkeypatch.setattr(model_module, "ops", Failing)
+    with pytest.raises(RuntimeError, match="out of memory"):
+        model.prefill_paged(longer, cache, 1, reuse=reuse)
+    assert cache.lengths == [-1, length] and cache.starts.tolist() == cache.lengths
+    got = model.prefill_paged(longer, cache, 1, reuse=max(length, 0))
+    assert cache.lengths == [-1, 152] and torch.allclose(got, want, atol=2e-2 * want.abs().max().item())
