@@ -169,8 +169,7 @@ FPX_INLINE void load_queries(Queries<FMT, D, NT> &f, const PagedDecodeParams &p,
       top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
       const int up = top == 0 ? 0 : min(14 + 127 - (int)(top >> 23), 103);  // at least 14 - 128
       const float mul = __uint_as_float((uint32_t)(127 + up) << 23);
-      // Codes stand for n 2^-24. At 2^127 it stops: a query above 2^116 picks one key whatever its logits' size.
-      const float back = p.scale_log2 * __uint_as_float((uint32_t)min(127 + 24 - up, 254) << 23);
+      const float back = logit_factor(p.scale_log2, up);
       f.scale[n][0] = __shfl_sync(0xffffffffu, back, 8 * t);
       f.scale[n][1] = __shfl_sync(0xffffffffu, back, 8 * t + 4);
 #pragma unroll

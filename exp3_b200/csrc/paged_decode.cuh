@@ -226,6 +226,13 @@ FPX_INLINE uint32_t pack_f16(float lo, float hi) {
   __half2 v = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<uint32_t *>(&v);
 }
+// From products of codes, n 2^-24 of them, and a query times 2^up to log2 units: scale_log2 2^(24 - up). A query above 2^116 may take
+// it past a float, and then picks one key whatever its logits' size: there it ends at 2^124, which leaves the products room.
+FPX_INLINE float logit_factor(float scale_log2, int up) {
+  const int f = 24 - up;
+  const float x = scale_log2 * __uint_as_float((uint32_t)(127 + min(f, 127)) << 23);
+  return f > 127 ? fminf(fmaxf(x * __uint_as_float((uint32_t)f << 23), -0x1p124f), 0x1p124f) : x;
+}
 // Of a key's 2^(kSumLift - e): whether e passes 15, and its log2.
 FPX_INLINE bool is_far(float w) { return w < kSumUnit / 0x1p15f; }
 FPX_INLINE float log2_of(float w) { return (float)((int)(__float_as_uint(w) >> 23) - 127); }

@@ -243,8 +243,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_decode_tc_kernel(const __
           }
         if (at % kT == 0) {
           float *col = reinterpret_cast<float *>(&sh.column[n >> 1]);
-          // codes' factor stands 2^24 lower; at 2^127 it stops: a query above 2^116 picks one key whatever its logits' size
-          col[n & 1] = p.scale_log2 * __uint_as_float((uint32_t)min(127 + 24 - up, 254) << 23);
+          col[n & 1] = logit_factor(p.scale_log2, up);
           col[2 + (n & 1)] = 0.f;
           sh.limit[n] = live ? (int)min((int64_t)u.seen, (int64_t)u.start + row + 1) : u.seen;
           sh.out_at[n] = u.b * p.o_sb + (int64_t)row * p.o_sl + (int64_t)head * p.o_sh;

@@ -133,3 +133,19 @@ def test_a_value_that_is_no_number_reaches_no_row_before_it(value, form, dim, ro
         vc[..., spoilt] = 0
         out[0, own:, :, spoilt] = 0
         check(cache, [n], [n - rows + own], [rows - own], q[:, own:].to(DEV), [(kc, vc)], dim ** -0.5, out[:, own:], lse[:, own:])
+
+
+@pytest.mark.parametrize("form", ["int4", "bf16"])
+@pytest.mark.parametrize("dim,rows,heads", [(128, 1, 4), (256, 2, 4), (128, 3, 8)])
+@pytest.mark.parametrize("exponent", [110, 118, 122])
+def test_large_queries_under_a_small_scale(form, dim, rows, heads, exponent):
+    """The scale brings their logits to ordinary sizes; bf16 pages sum 256 products of up to 2^122 * 2^4, below 2^128. Bounds as in test_gpu_paged.py's `check`."""
+    g = torch.Generator().manual_seed(54)
+    n = 500
+    k, v, q = randn(g, 1, n, 1, dim, size=0.5), randn(g, 1, n, 1, dim), randn(g, 1, rows, heads, dim) * 2.0 ** exponent
+    cache = Cache(form, [n], 1, dim, 64, seed=54, table_tokens=(1 << 17) * (rows * heads > 16))
+    paged.paged_append(k.to(DEV), v.to(DEV), cache.pool, cache.table, ints([0]))
+    lse = torch.empty(1, rows, heads, device=DEV)
+    scale = dim ** -0.5 * 2.0 ** -exponent
+    out = paged.paged_decode_attention(q.to(DEV), cache.pool, cache.table, ints([n - rows]), scale, lse=lse)
+    check(cache, [n], [n - rows], [rows], q.to(DEV), [cached_values(form, k[0].float(), v[0])], scale, out, lse)
