@@ -78,6 +78,8 @@ FPX_INLINE float fold(float (&x)[C], int lane, F f) {
     }
   return C == 16 ? f(x[0], __shfl_xor_sync(0xffffffffu, x[0], 16)) : x[0];
 }
+// Whether a tile may have keys that are not there, or that some columns see and others do not.
+FPX_INLINE bool edge_tile(int step, int seen) { return step * kTile + kTile > seen - FPX_PAGED_MAX_ROWS; }
 // Scales that are no numbers as fp16's largest, times whose codes, n - 8 = 0, is zero.
 FPX_INLINE uint32_t numbers(uint32_t scales) {
   const __half2 v = __hmin2(*reinterpret_cast<const __half2 *>(&scales), __half2half2(__ushort_as_half(0x7bff)));
@@ -112,7 +114,7 @@ struct alignas(1024) TcSmem {
   int lse_at[N];
   float keep[N], by[N], sum[N], red[4][N];  // keep: square root of what a reference's move leaves of the sums
   int4 vote[2][2];                // of each half
-  // Of each group and key warp: first key, of the tiles with keys that some columns see and others do not, whose value's group is no number. The
+  // Of each group and key warp: first key of the edge tiles whose value's group is no number. The
   // products take it as zero, since a probability 0 times it would be NaN; the columns that see it become NaN at the end. By part, in
   // four places: key warps begin a part when the softmax may still have to read of the third part before it, and no earlier one.
   int4 spoilt[4][D / 32];
@@ -179,11 +181,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_decode_tc_kernel(const __
   } else if (work) {
     work = u.find(p);
   }
-  // 128 x (120 + 120 + 88 + 88 + 64) registers of the launch's 640 x 96
+  // 128 x (128 + 128 + 80 + 80 + 64) registers of the launch's 640 x 96
   if (warp < 8)
-    regs_inc<120>();
+    regs_inc<128>();
   else if (warp < 16)
-    regs_dec<88>();
+    regs_dec<80>();
   else
     regs_dec<64>();
   int c = 0;  // tiles of this CTA so far: tile c lies in stage c % ST, S^T and P^T buffers c & 1
@@ -455,9 +457,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_decode_tc_kernel(const __
     const int w4 = warp & 3;
     const uint32_t lanes = tmem + ((uint32_t)(32 * w4) << 16);
     for (bool more = true; more && ok; more = !p.whole && u.find(p)) {
-      const int least = (int)min((int64_t)u.seen, (int64_t)u.start + u.rb * N / p.group + 1);
-      int4 *spoilt = sh.spoilt[parts & 3];  // a word of each is this warp's
-      if (lane < D / 32) reinterpret_cast<int *>(&spoilt[lane])[w4] = 0x7fffffff;
+      if (lane < D / 32) reinterpret_cast<int *>(&sh.spoilt[parts & 3][lane])[w4] = 0x7fffffff;  // a word of each is this warp's
       for (int step = u.g0; step < u.g1; ++step, ++c) {
         const int st = c % ST;
         ok = mbar_wait_warp(&sh.full[st], (c / ST) & 1, abort);
@@ -511,13 +511,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_decode_tc_kernel(const __
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&sh.k_ready[c & 1]);
-        if (step * kTile + kTile > least) {  // lane: a key
+        if (edge_tile(step, u.seen)) {  // lane: a key
           const int key = step * kTile + 32 * w4 + lane, gi = 2 * w4 + (lane >> 4), token = lane & 15;
           const bool there = key < u.seen && !((sh.gone[st] >> gi) & 1);
 #pragma unroll 1
           for (int j = 0; j < D / 32; ++j) {
             const uint32_t scale = lds16(stage + gi * G::kBytes + G::kVScales + ((token >> 1) * (D / 32) + j) * 4 + (token & 1) * 2);
-            if (there && (scale & 0x7c00u) == 0x7c00u) atomicMin(reinterpret_cast<int *>(&spoilt[j]) + w4, key);
+            if (there && (scale & 0x7c00u) == 0x7c00u) atomicMin(reinterpret_cast<int *>(&sh.spoilt[parts & 3][j]) + w4, key);
           }
         }
         __syncwarp();
@@ -533,7 +533,6 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_decode_tc_kernel(const __
     const uint32_t lanes = tmem + ((uint32_t)(32 * j) << 16);
     const uint32_t sel = j & 1 ? 0x7632 : 0x5410;
     for (bool more = true; more && ok; more = !p.whole && u.find(p)) {
-      const int least = (int)min((int64_t)u.seen, (int64_t)u.start + u.rb * N / p.group + 1);
       for (int step = u.g0; step < u.g1; ++step, ++c) {
         const int st = c % ST;
         ok = mbar_wait_warp(&sh.full[st], (c / ST) & 1, abort);
@@ -542,7 +541,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_decode_tc_kernel(const __
         tc_fence_after();
         const uint32_t stage = smem_u32(sh.stage[st]), v_at = lanes + S::kV + (VB == 2 ? (c & 1) * (D / 2) : 0);
         const int gone = sh.gone[st];
-        const bool edge = step * kTile + kTile > least || gone;
+        const bool edge = edge_tile(step, u.seen) || gone;
 #pragma unroll 1
         for (int i = 0; i < J; ++i)
 #pragma unroll 1
