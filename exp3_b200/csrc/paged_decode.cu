@@ -748,8 +748,8 @@ constexpr int grid_ctas() {
   return kSms * Shape<FMT, D, NT>::kOcc;
 }
 
-// Column tiles of a row block: two where one would leave rows over (16 rows at d = 128: 25.5 us in one block of two
-// tiles, 35 in two of one), but one for int4 at d = 256, whose registers two do not fit (16 rows: 59 us, 40 in two blocks).
+// Column tiles of a row block: two where one would leave rows over (16 rows at d = 128: 25.6 us in one block of two
+// tiles, 35 in two of one), but one for int4 at d = 256, whose registers two do not fit (16 rows: 59 us, 42 in two blocks).
 // Many columns (`wide`): row blocks of 32 or 64 on tcgen05.
 static DecodeLayout layout_of(int format, int B, int Lq, int H, int Hkv, int d, bool wide) {
   DecodeLayout w{};
@@ -773,17 +773,18 @@ static DecodeLayout layout_of(int format, int B, int Lq, int H, int Hkv, int d, 
 }
 
 // Short tables: a CTA a unit, one launch and no workspace. Four KV heads, us in one launch / in two, int4: 1 sequence of 256
-// tokens 5.6 / 8.2, 512 7.4 / 8.4, 1024 10.8 / 8.4; 37 sequences 6.7 / 11.1, 8.4 / 16.2, 11.8 / 14.0; bf16: 5.5 / 7.5, 7.4 /
-// 7.7, 11.0 / 7.5 and 5.8 / 9.6, 9.7 / 13.3, 15.7 / 19.4.
+// tokens 6.0 / 8.0, 512 7.7 / 8.0, 1024 11.0 / 8.0; 37 sequences 6.8 / 10.2, 8.5 / 14.9, 12.0 / 13.4; bf16: 5.6 / 7.0, 7.5 /
+// 7.0, 11.5 / 7.1 and 5.8 / 9.1, 10.1 / 13.3, 15.7 / 19.2. Tables as wide as the sequences: the rule sees the table's width, and where that is more
+// than they need (a cache of long slots), short sequences take two launches.
 static bool whole_units(const PageView &pv, int64_t units) {
   const int64_t tokens = ((int64_t)pv.max_pages << pv.page_shift) * kGranule;
   return tokens <= (units >= 32 ? 1024 : 512);
 }
 
 // Whether the tcgen05 kernel takes int4 pages of more than 16 columns: not where the other one's row blocks are few (w is its
-// layout), since it begins a unit 2 to 4 us later. Us, mma.sync / tcgen05: 4 x 65536 tokens, d = 128, 20 columns 32.2 /
-// 26.8, 28 33.5 / 27.1, 56 55.1 / 37.9, 448 282 / 174; d = 256, 20 columns 51.2 / 41.4, 64 113 / 58.4; 1 x 8192, 56 columns
-// 10.9 / 12.8. Tables of 512 tokens, a CTA a unit: 8 x 4 KV heads, 56 columns 10.8 / 15.4; 32 x 4 22.9 / 16.2.
+// layout), since it begins a unit 2 to 4 us later. Us, mma.sync / tcgen05: 4 x 65536 tokens, d = 128, 20 columns 33.8 /
+// 27.7, 28 35.0 / 27.9, 56 56.2 / 38.9, 448 281 / 175; d = 256, 20 columns 54.5 / 42.7, 64 115 / 59.5; 1 x 8192, 56 columns
+// 11.3 / 13.1. Tables of 512 tokens, a CTA a unit: 8 x 4 KV heads, 56 columns 10.9 / 15.7; 32 x 4 23.3 / 17.1. Tables as wide as the sequences, as above.
 static bool wide_units(const PageView &pv, const DecodeLayout &w) {
   const int64_t tokens = ((int64_t)pv.max_pages << pv.page_shift) * kGranule;
   return tokens * w.units > 65536 && !(whole_units(pv, w.units) && w.units <= w.ctas);

@@ -43,7 +43,7 @@ constexpr float kLowest = -3e38f;  // reference before any logit: below all of t
 // A weight is u 2^-e, while u < 2^-126 is zero. Where no row's exponent has moved the reference by more than 15, that loses less than a
 // 2^50th of the sum. Once one has (is_far), the weights are exponentials of their own: values of 2^60 beside values of
 // 2^-60. That code runs where the reference moves, and only costs calls without such values its place there: 14.5 -> 14.8 us for 32641 tokens,
-// 65.2 -> 65.5 for the ragged batch of 32, 37.9 -> 39.6 for 56 columns of 4 x 65536.
+// 65.2 -> 65.5 for a ragged batch of 32.
 constexpr float kSumLift = 24.f, kSumUnit = 0x1p24f;
 
 // Keys that row block rb of sequence b needs: all up to its last row's position.
@@ -63,8 +63,8 @@ FPX_INLINE int item_keys(const PagedDecodeParams &p, int start, int count, int r
 template <int GS>
 FPX_INLINE int steps_of(int keys) { return (int)(((unsigned)keys + GS * kGranule - 1) / (GS * kGranule)); }
 // What a unit counts in the partition: its steps and, in front of them, what beginning a unit costs a CTA
-// (queries, first copies, merge) in steps. 28 columns of 4 x 65536 tokens in steps of 128: 30.3 us with one, 29.3 with two,
-// 27.0 with four and six, 28.1 with eight.
+// (queries, first copies, merge) in steps. 28 columns of 4 x 65536 tokens in steps of 128: 31.1 us with one, 30.4 with two,
+// 27.9 with four and six, 29.0 with eight.
 constexpr int kPad = 4;
 FPX_INLINE int padded(int steps) { return steps ? steps + kPad : 0; }
 

@@ -15,8 +15,8 @@
 // 8-11 expand keys, warps 12-15 values (warp = 32 dims of each 128, the lanes that it may write), warp 16 issues the bulk
 // copies, warps 17 and 18 the products. The next tile's scores are computed while this one's softmax runs.
 //
-// Measured (4 sequences of 65536 tokens, one KV head, us of one call): d = 128, 28 columns 27.1, 56 columns 37.9, 448 columns 174; d =
-// 256, 20 columns 41.4, 64 columns 58.4. What bounds it: the latency of the softmax warps (2000 to 2500 cycles a tile at d =
+// Measured (4 sequences of 65536 tokens, one KV head, us of one call): d = 128, 28 columns 27.9, 56 columns 38.8, 448 columns 175; d =
+// 256, 20 columns 42.7, 64 columns 59.4. What bounds it: the latency of the softmax warps (2000 to 2500 cycles a tile at d =
 // 128, where a product takes the tensor core 63 cycles whatever its columns and 16 of them 1000), the expansion of values
 // (1400, and 2700 at d = 256) and the issue of products (100 to 150 cycles each); 8 us of it begin and merge.
 #include "paged_decode.cuh"

@@ -226,7 +226,8 @@ class Qwen2Model:
 
     def _decode_comm(self):
         """The decode step's small all-reduces go over NVLink peer memory (exp3_b200.comm) when
-        ``peer_all_reduce`` is set and the model is tensor parallel."""
+        ``peer_all_reduce`` is set and the model is tensor parallel: up to eight rows of the hidden size. A
+        paged step of more slots all-reduces through the process group."""
         if self.tp_size > 1 and self.peer_all_reduce and self._peer_ar is None:
             from .comm import PeerAllReduce
             self._peer_ar = PeerAllReduce(self.group, self.device, max_elems=8 * self.cfg.hidden_size)
@@ -501,7 +502,8 @@ class Qwen2Model:
         """One forward over a prompt into a slot of ``cache``; returns the last token's fp32 logits.
 
         ``reuse`` tokens of the prompt are in the slot already (an earlier turn): whole 128-token tiles of
-        them are read back from the pages, and only the rows behind are computed and stored."""
+        them are read back from the pages, and only the rows behind are computed and stored. Under tensor parallelism its
+        all-reduces are not overlapped (``prefill_logits`` has the row-chunk pipeline)."""
         if input_ids.dim() != 1 or input_ids.shape[0] == 0:
             raise ValueError("input_ids must be 1-D and hold a token")
         length = input_ids.shape[0]
