@@ -21,7 +21,8 @@
 //             [-60, 126], r = fp16(amax / 7 * 2^-e). r is below 2 whatever the values' size, so
 //             the attention kernel multiplies it into fp16 probabilities; 2^e joins the logit.
 // code = round-half-even(x / s) + 8, in 1 .. 15. A group with an infinity or a NaN reads back
-// as NaN; the other groups of such a value row as zero, and its exponent is 0.
+// as NaN. The other groups of such a value row have the scales of exponent 126, which is zero below 2^101; where all are, the row's
+// exponent is -60.
 #pragma once
 
 #include <cuda_fp16.h>

@@ -140,18 +140,36 @@ FPX_INLINE uint32_t codes4(const float (&x)[4], float s, float inv, bool quick) 
   return w;
 }
 
-// A value row's exponent from its largest amax / 7, and the factors to and from its scales. A row with an infinity or a NaN has
-// exponent 0 and scales 0 but where its groups hold them: its exponent joins the logit in attention, and 126 there would take
-// the other rows' bits.
+// A value row's exponent and the factors to and from its scales, from the lane's N groups (a: amax / 7) and the lanes of the row, FIRST,
+// 2 FIRST .. < LANES apart. An infinity or a NaN among them means exponent 126, where the scales of other groups below 2^101 are
+// zero. Where they all are, it is -60, as for a row of zeros: it joins the logit in attention, and 126 there would take the other
+// rows' bits.
+template <int N, int FIRST, int LANES>
 struct RowExponent {
   int e;
   float up, down;
-  FPX_INLINE explicit RowExponent(float top) {
+  FPX_INLINE explicit RowExponent(const float (&a)[N]) {
+    float top = a[0];
+#pragma unroll
+    for (int i = 1; i < N; ++i) top = max_nan(top, a[i]);
+#pragma unroll
+    for (int o = FIRST; o < LANES; o <<= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
     e = min(max((int)((__float_as_uint(top) >> 23) & 255u) - 127, -60), 126);
-    const bool number = e < 126;  // finite values end below 2^125.2 * 7
-    e = number ? e : 0;
     up = __uint_as_float((uint32_t)(e + 127) << 23);
-    down = number ? __uint_as_float((uint32_t)(127 - e) << 23) : 0.f;
+    down = __uint_as_float((uint32_t)(127 - e) << 23);
+    const bool number = e < 126;  // finite ones end at 2^125.2
+    if (__any_sync(0xffffffffu, !number)) {
+      float most = 0.f;  // of the others
+#pragma unroll
+      for (int i = 0; i < N; ++i) most = a[i] < INFINITY ? fmaxf(most, a[i]) : most;
+#pragma unroll
+      for (int o = FIRST; o < LANES; o <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+      if (!number && __half2float(__float2half_rn(most * down)) == 0.f) {
+        e = -60;
+        up = 0x1p-60f;
+        down = 0.f;
+      }
+    }
   }
 };
 
@@ -161,19 +179,15 @@ FPX_INLINE void write_int4(uint8_t *gran, int t, const float (&x)[D / 128][4], i
   using G = Granule<FPX_PAGES_INT4, D>;
   const int j = lane >> 3;
   float a[D / 128];
-  float top = 0.f;
 #pragma unroll
   for (int J = 0; J < D / 128; ++J) {
     float m = max_nan(max_nan(fabsf(x[J][0]), fabsf(x[J][1])), max_nan(fabsf(x[J][2]), fabsf(x[J][3])));
 #pragma unroll
     for (int o = 1; o < 8; o <<= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
     a[J] = seventh(m);
-    top = max_nan(top, a[J]);
   }
   if (VALUE) {
-    top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, 8));
-    top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, 16));
-    const RowExponent x2(top);
+    const RowExponent<D / 128, 8, 32> x2(a);
 #pragma unroll
     for (int J = 0; J < D / 128; ++J) {
       const __half r = __float2half_rn(a[J] * x2.down);
@@ -427,10 +441,7 @@ FPX_INLINE void append_rows(const AppendParams &p, int b, int l, int pos, uint8_
         m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, 2));
         a[h] = seventh(m);
       }
-      float top = max_nan(a[0], a[1]);
-#pragma unroll
-      for (int o = 4; o < kLanes; o <<= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
-      const RowExponent x2(top);
+      const RowExponent<2, 4, kLanes> x2(a);
       if (!mine || !gran) continue;  // no lane of the warp waits for another below
       const int part = u & 3;
 #pragma unroll

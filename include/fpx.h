@@ -334,7 +334,8 @@ size_t fpx_paged_page_bytes(int format, int Hkv, int d, int page_size);
  * 8), or NULL: no rotation. Padding rows are left as they are, unless zero_padding is set. Head rows are
  * 8-byte aligned, strides multiples of 4 elements. With zero_padding != 0, padding rows (and skipped ones) of q_out and
  * k_out become zero. A group (32 dims) with an infinity or
- * a NaN reads back from int4 pages as NaN, and the other groups of such a value row as zero. */
+ * a NaN reads back from int4 pages as NaN, and the other groups of such a value row as zero (values above 2^104
+ * with a few bits). */
 int fpx_paged_append(int format, const void *q, int64_t q_sb, int64_t q_sl, int64_t q_sh, const void *k,
                      int64_t k_sb, int64_t k_sl, int64_t k_sh, const void *v, int64_t v_sb, int64_t v_sl,
                      int64_t v_sh, int B, int L, int H, int Hkv, int d, const float *rope, int rope_len, int rotary,

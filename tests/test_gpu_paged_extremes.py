@@ -149,3 +149,38 @@ def test_large_queries_under_a_small_scale(form, dim, rows, heads, exponent):
     scale = dim ** -0.5 * 2.0 ** -exponent
     out = paged.paged_decode_attention(q.to(DEV), cache.pool, cache.table, ints([n - rows]), scale, lse=lse)
     check(cache, [n], [n - rows], [rows], q.to(DEV), [cached_values(form, k[0].float(), v[0])], scale, out, lse)
+
+
+@pytest.mark.parametrize("dim,rotary", [(128, 128), (256, 64)])
+def test_large_values_beside_one_that_is_no_number_keep_their_bits(dim, rotary):
+    """Equal to the restatement's: such a row has the largest exponent, at which values below 2^101 * 7 have no bits and larger ones some."""
+    g = torch.Generator().manual_seed(55)
+    k, v = randn(g, 1, 40, 2, dim), randn(g, 1, 40, 2, dim)
+    for t in range(40):
+        v[0, t, :, 32:64] *= 2.0 ** (90 + t)
+        v[0, t, t % 2, 64 if t % 3 else 96] = (math.inf, math.nan, -math.inf)[t % 3]
+    cache = Cache("int4", [40], 2, dim, 16, seed=55)
+    where = (cache.pool, cache.table, ints([0]))
+    paged.paged_append(k.to(DEV), v.to(DEV), *where, rope=paged.rope_table(40, rotary, device=DEV))
+    got = paged.paged_gather(*where, None, 40)[1][0].cpu()
+    want = cached_values("int4", k[0].float(), v[0])[1].to(torch.bfloat16)
+    torch.testing.assert_close(got, want, rtol=0, atol=0, equal_nan=True)
+    assert want.isnan().any(-1).any(1).all() and (want[:, :, 32:64] != 0).any(-1).any(1).tolist().count(True) > 20
+
+
+@pytest.mark.parametrize("dim,rows,heads", [(128, 1, 4), (256, 1, 4), (128, 3, 8)])
+def test_tiny_values_beside_one_that_is_no_number(dim, rows, heads):
+    """The row that holds it weighs as one of zeros does: values of 1e-12 in the other rows keep their bits."""
+    g = torch.Generator().manual_seed(56)
+    n = 300
+    k, v, q = randn(g, 1, n, 1, dim), randn(g, 1, n, 1, dim, size=1e-12), randn(g, 1, rows, heads, dim)
+    v[0, n // 3, 0, 40] = math.inf
+    cache = Cache("int4", [n], 1, dim, 64, seed=56, table_tokens=(1 << 17) * (rows * heads > 16))
+    paged.paged_append(k.to(DEV), v.to(DEV), cache.pool, cache.table, ints([0]))
+    lse = torch.empty(1, rows, heads, device=DEV)
+    out = paged.paged_decode_attention(q.to(DEV), cache.pool, cache.table, ints([n - rows]), dim ** -0.5, lse=lse)
+    assert out[..., 32:64].isnan().all()
+    kc, vc = cached_values("int4", k[0].float(), v[0])
+    vc[..., 32:64] = 0
+    out[..., 32:64] = 0
+    check(cache, [n], [n - rows], [rows], q.to(DEV), [(kc, vc)], dim ** -0.5, out, lse)
