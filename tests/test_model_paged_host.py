@@ -1,7 +1,6 @@
 """Host logic of the model's paged path on the CPU (tests/paged_model_cpu.py has the kernels' calls as plain torch)."""
 
 import datetime
-import os
 
 import pytest
 import torch
@@ -41,10 +40,10 @@ def decode_run(model):
     return torch.stack(out)
 
 
-def tensor_parallel_rank(rank, world, port, path):
-    os.environ.update(MASTER_ADDR="127.0.0.1", MASTER_PORT=str(port))
+def tensor_parallel_rank(rank, world, path):
     torch.set_num_threads(2)
-    dist.init_process_group("gloo", rank=rank, world_size=world, timeout=datetime.timedelta(seconds=120))
+    dist.init_process_group("gloo", init_method=f"file://{path}/store", rank=rank, world_size=world,
+                            timeout=datetime.timedelta(seconds=120))
     try:
         use_plain_calls(setattr)
         model = PlainModel(seed=4, tp_rank=rank, tp_size=world)
@@ -63,7 +62,7 @@ def test_tensor_parallel_paged_decode(plain, tmp_path, world):
     rounding of the residual stream adds as much: logits agree to a few 2^-8 of their size; shards in another order would not at all."""
     want = decode_run(PlainModel(seed=4))
     ctx = mp.get_context("spawn")
-    procs = [ctx.Process(target=tensor_parallel_rank, args=(r, world, 29547 + world, str(tmp_path))) for r in range(world)]
+    procs = [ctx.Process(target=tensor_parallel_rank, args=(r, world, str(tmp_path))) for r in range(world)]
     for p in procs:
         p.start()
     for p in procs:
